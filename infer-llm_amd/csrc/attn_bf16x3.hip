@@ -56,6 +56,7 @@
 //     and V two tiles ahead (equal); blocks in pairs of a long and a short one
 //     (0.6B 3000 286 against 241 with the longest first).
 #include "attn_bf16x3.hpp"
+#include "batch.hpp"
 #include "bf16x3.hpp"
 #include "coherent.hpp"
 #include "ikv_common.hpp"
@@ -97,11 +98,11 @@ __device__ __forceinline__ void load_dims(__amdgpu_buffer_rsrc_t r, unsigned off
   }
 }
 
-template <int DT, int RW, int KG, int MINW, bool PAGED>
+template <int DT, int RW, int KG, int MINW, bool PAGED, bool PACKED>
 __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
     const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
     float *__restrict__ out, int n_head_kv, int G, int dim, int n_rows, int n_kv, int n_past,
-    int n_blocks, float scale_log2, ikv::Pages pages) {
+    int n_blocks, float scale_log2, ikv::Pages pages, ikv::PackedSeqs seqs) {
   constexpr int D = 32 * DT;
   constexpr int KS = D / 16;       // MFMA steps of Q K^T
   constexpr int NT = RW * 64;      // threads of a key group
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
   __shared__ floatx4 s_o[BLOCKED ? RW * 64 * 4 * DT : 1];
 
   const int g = blockIdx.x % n_head_kv;
-  const int item = blockIdx.x / n_head_kv;
+  int item = blockIdx.x / n_head_kv;
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wv / RW, slot = wv % RW;
@@ -122,6 +123,23 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
   const int r32 = lane & 31, c2 = lane >> 5;
   const int n_head = n_head_kv * G;
   const int stride = n_head_kv * dim;  // floats of a token row
+  if constexpr (PACKED) {  // one sequence's rows, cache and sizes from here on
+    ikv::PackedBlock b;
+    if (!ikv::packed_block<BR>(seqs, G, item, b)) return;
+    item = b.item;
+    n_blocks = b.n_blocks;
+    n_rows = b.rows * G;
+    n_past = b.past;
+    n_kv = b.past + b.rows;
+    q += static_cast<size_t>(b.first) * n_head * dim;
+    out += static_cast<size_t>(b.first) * n_head * dim;
+    if constexpr (PAGED) {
+      pages.table += b.seq * seqs.stride;
+    } else {
+      k += static_cast<size_t>(b.first) * stride;
+      v += static_cast<size_t>(b.first) * stride;
+    }
+  }
 
   // staging: a thread's K items (a key's 8 dims) and V item (VD dims of 8 keys)
   unsigned kof[VD][2];
@@ -635,11 +653,23 @@ void launch(const float *q, const float *k, const float *v, float *out, int n_he
   const int n_blocks = (n_rows + BR - 1) / BR;
   const unsigned grid = static_cast<unsigned>(n_blocks) * n_head_kv;
   if (pg)
-    attn_bf16x3_kernel<DT, RW, KG, MINW, true><<<grid, RW * KG * 64, 0, s>>>(
-        q, k, v, out, n_head_kv, G, dim, n_rows, n_kv, n_past, n_blocks, sl2, *pg);
+    attn_bf16x3_kernel<DT, RW, KG, MINW, true, false><<<grid, RW * KG * 64, 0, s>>>(
+        q, k, v, out, n_head_kv, G, dim, n_rows, n_kv, n_past, n_blocks, sl2, *pg, ikv::PackedSeqs{});
   else
-    attn_bf16x3_kernel<DT, RW, KG, MINW, false><<<grid, RW * KG * 64, 0, s>>>(
-        q, k, v, out, n_head_kv, G, dim, n_rows, n_kv, n_past, n_blocks, sl2, ikv::Pages{});
+    attn_bf16x3_kernel<DT, RW, KG, MINW, false, false><<<grid, RW * KG * 64, 0, s>>>(
+        q, k, v, out, n_head_kv, G, dim, n_rows, n_kv, n_past, n_blocks, sl2, ikv::Pages{}, ikv::PackedSeqs{});
+}
+
+template <int DT, int RW, int KG, int MINW>
+void launch_packed(const float *q, const float *k, const float *v, float *out, int n_head_kv, int G,
+                   int dim, float sl2, const ikv::Pages *pg, const ikv::PackedSeqs &seqs, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(ikv::packed_blocks(seqs.n_rows, seqs.n_seq, G, 32 * RW) * n_head_kv);
+  if (pg)
+    attn_bf16x3_kernel<DT, RW, KG, MINW, true, true><<<grid, RW * KG * 64, 0, s>>>(
+        q, k, v, out, n_head_kv, G, dim, 0, 0, 0, 0, sl2, *pg, seqs);
+  else
+    attn_bf16x3_kernel<DT, RW, KG, MINW, false, true><<<grid, RW * KG * 64, 0, s>>>(
+        q, k, v, out, n_head_kv, G, dim, 0, 0, 0, 0, sl2, ikv::Pages{}, seqs);
 }
 
 }  // namespace
@@ -715,6 +745,33 @@ int attn_bf16x3(const float *q, const float *k, const float *v, const Pages *pag
       IKV_A3(4, 2, 2, 1);
   } else {
     if (us(kForms64[0]) <= us(kForms64[1]))
+      IKV_A3(2, 2, 2, 2);
+    else
+      IKV_A3(2, 1, 4, 1);
+  }
+#undef IKV_A3
+  return launch_status();
+}
+
+int attn_bf16x3_packed(const float *q, const float *k, const float *v, const Pages *pages, float *out,
+                       int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, float scale,
+                       hipStream_t s) {
+  const int G = n_head / n_head_kv;
+  if (!attn_bf16x3_supported(q, k, v, out, n_head, n_head_kv, head_dim, seqs.n_rows + seqs.n_seq,
+                             seqs.capacity, 0))
+    return -ENOTSUP;
+  if (packed_blocks(seqs.n_rows, seqs.n_seq, G, 32) * n_head_kv > INT_MAX) return -EOVERFLOW;
+  if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
+  const float sl2 = scale * kLog2e;
+  const int64_t blocks = static_cast<int64_t>(seqs.n_rows) * G / 32 * n_head_kv;  // of 32 rows
+#define IKV_A3(...) launch_packed<__VA_ARGS__>(q, k, v, out, n_head_kv, G, head_dim, sl2, pages, seqs, s)
+  if (head_dim > 64) {
+    if (blocks >= 8 * kCUs)
+      IKV_A3(4, 4, 1, 1);
+    else
+      IKV_A3(4, 2, 2, 1);
+  } else {
+    if (blocks >= 4 * kCUs)
       IKV_A3(2, 2, 2, 2);
     else
       IKV_A3(2, 1, 4, 1);

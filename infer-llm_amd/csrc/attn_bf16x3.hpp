@@ -6,6 +6,7 @@
 
 #include <cstdint>
 
+#include "batch.hpp"
 #include "ikv_common.hpp"
 
 namespace ikv {
@@ -20,5 +21,12 @@ bool attn_bf16x3_supported(const void *q, const void *k, const void *v, const vo
 int attn_bf16x3(const float *q, const float *k, const float *v, const Pages *pages, float *out,
                 int n_head, int n_head_kv, int head_dim, int64_t n_q, int64_t n_kv, int64_t n_past,
                 float scale, hipStream_t s);
+
+// Packed prompts (batch.hpp): k and v packed as q is, or, with pages, pools
+// read through the table of each sequence (pages->table: the first one's).
+// n_rows > 0 and n_seq > 0. -ENOTSUP for what attn_bf16x3_supported refuses.
+int attn_bf16x3_packed(const float *q, const float *k, const float *v, const Pages *pages, float *out,
+                       int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, float scale,
+                       hipStream_t s);
 
 }  // namespace ikv

@@ -24,6 +24,7 @@
 // One query token (a decode step): the split form below.
 #include "attn_bf16x3.hpp"
 #include "attn_generic.hpp"
+#include "batch.hpp"
 #include "ikv_common.hpp"
 
 #include <algorithm>
@@ -55,11 +56,11 @@ constexpr int64_t kPiecesMinKeys = 96;
 constexpr int kTileRowsPerWave = 4;  // 8 measured slower (fewer workgroups, more registers)
 constexpr int kTileRows = 4 * kTileRowsPerWave;  // query rows per workgroup
 
-template <int DL>  // dims per lane: head_dim <= 64 * DL
+template <int DL, bool PACKED>  // dims per lane: head_dim <= 64 * DL
 __global__ __launch_bounds__(256) void generic_tile_kernel(
     const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
     float *__restrict__ out, int n_head, int n_head_kv, int dim, int n_q, int n_kv, int n_past,
-    float scale_log2, bool paged, ikv::Pages pg, bool vec4) {
+    float scale_log2, bool paged, ikv::Pages pg, bool vec4, ikv::PackedSeqs seqs) {
   constexpr int KT = DL <= 2 ? 64 : 128 / DL;  // keys per tile: 64, 64, 32, 16
   constexpr int LPK = 64 / KT;                 // lanes per key in the score phase
   constexpr int DA = 64 * DL;                  // dims held (zeros past head_dim)
@@ -72,12 +73,28 @@ __global__ __launch_bounds__(256) void generic_tile_kernel(
   __shared__ __attribute__((aligned(16))) float s_p[4][RW][KT];
   const int G = n_head / n_head_kv;
   const int g = static_cast<int>(blockIdx.x) % n_head_kv;
-  const int blk = static_cast<int>(blockIdx.x) / n_head_kv;
+  int blk = static_cast<int>(blockIdx.x) / n_head_kv;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n_rows = n_q * G;
-  const int r0 = blk * kTileRows;
   const size_t tok_stride = static_cast<size_t>(n_head_kv) * dim;
   const size_t head_off = static_cast<size_t>(g) * dim;
+  if constexpr (PACKED) {  // one sequence's rows, cache and sizes from here on
+    ikv::PackedBlock b;
+    if (!ikv::packed_block<kTileRows>(seqs, G, blk, b)) return;
+    blk = b.n_blocks - 1 - b.item;
+    n_q = b.rows;
+    n_past = b.past;
+    n_kv = b.past + b.rows;
+    q += static_cast<size_t>(b.first) * n_head * dim;
+    out += static_cast<size_t>(b.first) * n_head * dim;
+    if (paged) {
+      pg.table += b.seq * seqs.stride;
+    } else {
+      k += b.first * tok_stride;
+      v += b.first * tok_stride;
+    }
+  }
+  const int n_rows = n_q * G;
+  const int r0 = blk * kTileRows;
 
   // the block's query rows, pre-scaled, zero past head_dim and past the rows
   for (int i = tid; i < kTileRows * DA; i += 256) {
@@ -193,7 +210,24 @@ __global__ __launch_bounds__(256) void generic_tile_kernel(
     for (int i = 0; i < RW; ++i)
 #pragma unroll
       for (int t = 0; t < DL; ++t) o[i][t] *= alpha[i];
-    for (int j4 = 0; j4 < KT; j4 += 4) {  // 4 keys: the rows' weights as one 16-byte read
+    int j_plain = KT;  // keys that are added by their weights alone
+    if constexpr (PACKED) {
+      // the tile of a row's last keys: a masked key weighs 0, but 0 times an
+      // infinite value is NaN, so each row takes the keys that it sees
+      if (kb + KT - 1 > n_past + (r0 + wave * RW) / G) {
+        j_plain = 0;
+        for (int j = 0; j < KT; ++j) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            if (kb + j > n_past + tok[i]) continue;
+            const float pj = s_p[wave][i][j];
+#pragma unroll
+            for (int t = 0; t < DL; ++t) o[i][t] = fmaf(pj, s_v[j * DP + lane + 64 * t], o[i][t]);
+          }
+        }
+      }
+    }
+    for (int j4 = 0; j4 < j_plain; j4 += 4) {  // 4 keys: the rows' weights as one 16-byte read
       float vd[4][DL];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -701,16 +735,43 @@ int attn_generic(const float *q, const float *k, const float *v, const Pages *pa
   // aligned
   const bool vec4 = head_dim % 4 == 0 && aligned16(k) && aligned16(v);
 #define IKV_GENERIC_TILE(DD)                                                                  \
-  generic_tile_kernel<DD><<<grid, 256, 0, s>>>(q, k, v, out, n_head, n_head_kv, head_dim,     \
-                                               static_cast<int>(n_q), static_cast<int>(n_kv), \
-                                               static_cast<int>(n_past), sl2, pages != nullptr, pgv, \
-                                               vec4)
+  generic_tile_kernel<DD, false><<<grid, 256, 0, s>>>(                                       \
+      q, k, v, out, n_head, n_head_kv, head_dim, static_cast<int>(n_q), static_cast<int>(n_kv), \
+      static_cast<int>(n_past), sl2, pages != nullptr, pgv, vec4, PackedSeqs{})
   switch (dl) {
     case 1: IKV_GENERIC_TILE(1); break;
     case 2: IKV_GENERIC_TILE(2); break;
     case 4: IKV_GENERIC_TILE(4); break;
     default: IKV_GENERIC_TILE(8); break;
   }
+#undef IKV_GENERIC_TILE
+  return launch_status();
+}
+
+int attn_generic_packed(const float *q, const float *k, const float *v, const Pages *pages, float *out,
+                        int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, float scale,
+                        hipStream_t s) {
+  if (!generic_attn_shape(n_head, n_head_kv, head_dim)) return -ENOTSUP;
+  const int G = n_head / n_head_kv;
+  if (seqs.n_rows > INT_MAX / 4 / n_head) return -EOVERFLOW;
+  const int64_t blocks = packed_blocks(seqs.n_rows, seqs.n_seq, G, kTileRows);
+  if (blocks * n_head_kv > INT_MAX) return -EOVERFLOW;
+  if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
+  const unsigned grid = static_cast<unsigned>(blocks * n_head_kv);
+  const float sl2 = scale * kLog2e;
+  const Pages pgv = pages ? *pages : Pages{};
+  const bool vec4 = head_dim % 4 == 0 && aligned16(k) && aligned16(v);
+#define IKV_GENERIC_TILE(DD)                                                                       \
+  generic_tile_kernel<DD, true><<<grid, 256, 0, s>>>(q, k, v, out, n_head, n_head_kv, head_dim, 0, 0, 0, \
+                                                     sl2, pages != nullptr, pgv, vec4, seqs)
+  if (head_dim <= 64)
+    IKV_GENERIC_TILE(1);
+  else if (head_dim <= 128)
+    IKV_GENERIC_TILE(2);
+  else if (head_dim <= 256)
+    IKV_GENERIC_TILE(4);
+  else
+    IKV_GENERIC_TILE(8);
 #undef IKV_GENERIC_TILE
   return launch_status();
 }

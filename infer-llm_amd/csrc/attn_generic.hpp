@@ -6,6 +6,7 @@
 
 #include <cstdint>
 
+#include "batch.hpp"
 #include "ikv_common.hpp"
 
 namespace ikv {
@@ -24,6 +25,13 @@ bool generic_attn_shape(int n_head, int n_head_kv, int head_dim);
 int attn_generic(const float *q, const float *k, const float *v, const Pages *pages, float *out,
                  int n_head, int n_head_kv, int head_dim, int64_t n_q, int64_t n_kv,
                  int64_t n_past, float scale, hipStream_t s);
+
+// Packed prompts (batch.hpp): k and v packed as q is, or, with pages, pools
+// read through the table of each sequence (pages->table: the first one's).
+// Any alignment. n_rows > 0 and n_seq > 0.
+int attn_generic_packed(const float *q, const float *k, const float *v, const Pages *pages, float *out,
+                        int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, float scale,
+                        hipStream_t s);
 
 // One query token (a decode step) over keys [0, n_kv): the same result as
 // attn_generic with n_q = 1 and n_past = n_kv - 1 (within the path's float

@@ -1,0 +1,62 @@
+// attn_packed.hip — causal attention over several prompts, packed one behind
+// the other (ikv_attn_prefill_packed_f32 and its paged form): the checks, and
+// the choice between the two kernels that run them, the bf16-piece one
+// (attn_bf16x3.hip) and, for head sizes and alignments that it does not take,
+// the generic one (attn_generic.hip). Each workgroup finds its sequence from
+// row_start (packed_block in batch.hpp) and then works as on a prompt alone, so
+// every row's result is that of its sequence whatever it is packed with.
+#include "attn_bf16x3.hpp"
+#include "attn_generic.hpp"
+#include "batch.hpp"
+
+namespace {
+
+int prefill_packed(const float *q, const float *k, const float *v, const ikv::Pages *pages,
+                   ikv::PackedSeqs seqs, int64_t n_rows, float *out, int n_head, int n_head_kv,
+                   int head_dim, float scale, void *stream) {
+  if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || n_rows < 0) return -EINVAL;
+  if (!ikv::generic_attn_shape(n_head, n_head_kv, head_dim)) return -ENOTSUP;
+  if (n_rows == 0 || seqs.n_seq == 0) return 0;
+  if (!q || !k || !v || !out || !seqs.row_start) return -EINVAL;
+  if (n_rows > INT_MAX / 8 / n_head) return -EOVERFLOW;
+  seqs.n_rows = static_cast<int>(n_rows);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int rc = ikv::attn_bf16x3_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale, s);
+  if (rc != -ENOTSUP) return rc;
+  return ikv::attn_generic_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale, s);
+}
+
+}  // namespace
+
+extern "C" int ikv_attn_prefill_packed_f32(const float *q, const float *k, const float *v,
+                                           const int32_t *row_start, int64_t n_seq, int64_t n_rows,
+                                           float *out, int n_head, int n_head_kv, int head_dim,
+                                           float scale, int32_t *status, void *stream) {
+  if (n_seq < 0) return -EINVAL;
+  if (n_seq > ikv::kMaxSeqs) return -EOVERFLOW;
+  ikv::PackedSeqs seqs;
+  seqs.row_start = row_start;
+  seqs.n_seq = static_cast<int>(n_seq);
+  seqs.capacity = static_cast<int>(ikv::kMaxSeqTokens) - 1;
+  seqs.status = status;
+  return prefill_packed(q, k, v, nullptr, seqs, n_rows, out, n_head, n_head_kv, head_dim, scale, stream);
+}
+
+extern "C" int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_pool, const float *v_pool,
+                                                 const ikv_kv_batch *batch, const int32_t *row_start,
+                                                 const int32_t *n_past, int64_t n_rows, float *out,
+                                                 int n_head, int n_head_kv, int head_dim, float scale,
+                                                 void *stream) {
+  ikv::BatchPages b;
+  if (const int rc = ikv::batch_arg(batch, b)) return rc;
+  ikv::PackedSeqs seqs;
+  seqs.row_start = row_start;
+  seqs.n_past = n_past;
+  seqs.n_seq = b.n_seq;
+  seqs.capacity = b.capacity;
+  seqs.stride = b.stride;
+  seqs.status = b.status;
+  const ikv::Pages pages{b.tables, b.bt, b.n_blocks, b.status};
+  return prefill_packed(q, k_pool, v_pool, &pages, seqs, n_rows, out, n_head, n_head_kv, head_dim, scale,
+                        stream);
+}

@@ -1,0 +1,126 @@
+// batch.hpp — several sequences in one launch: the descriptors of
+// include/ikv_batch.h as the kernels see them, and the search for the sequence
+// that a packed row or block belongs to.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/ikv_batch.h"
+#include "ikv_common.hpp"
+
+namespace ikv {
+
+constexpr int64_t kMaxSeqs = 1 << 20;       // n_seq
+constexpr int64_t kMaxSeqTokens = 1 << 28;  // tokens of one sequence
+
+// Block tables of several sequences (ikv_kv_batch).
+struct BatchPages {
+  const int32_t *tables = nullptr;
+  int64_t stride = 0;  // entries per sequence
+  int bt = 0;
+  int n_blocks = 0;
+  int capacity = 0;  // tokens that a table covers
+  int n_seq = 0;
+  int *status = nullptr;
+};
+
+inline int batch_arg(const ikv_kv_batch *b, BatchPages &out) {
+  if (!b || !b->block_tables || b->table_stride <= 0 || b->block_tokens <= 0 ||
+      b->block_tokens % 64 != 0 || b->n_pool_blocks <= 0 || b->n_seq < 0)
+    return -EINVAL;
+  if (b->block_tokens > INT_MAX / b->n_pool_blocks || b->n_seq > kMaxSeqs ||
+      b->block_tokens > kMaxSeqTokens / b->table_stride)
+    return -EOVERFLOW;
+  out.tables = b->block_tables;
+  out.stride = b->table_stride;
+  out.bt = static_cast<int>(b->block_tokens);
+  out.n_blocks = static_cast<int>(b->n_pool_blocks);
+  out.capacity = static_cast<int>(b->table_stride * b->block_tokens);
+  out.n_seq = static_cast<int>(b->n_seq);
+  out.status = b->status;
+  return 0;
+}
+
+// One sequence's table.
+__device__ __forceinline__ Pages pages_of(const BatchPages &b, int seq) {
+  return Pages{b.tables + seq * b.stride, b.bt, b.n_blocks, b.status};
+}
+
+// The last i in [0, n) for which at_most(i) holds, or -1, for a predicate that
+// holds up to some i and not behind it; by a whole wave, 64 probes a round (two
+// rounds up to 4096). Whatever the predicate says, the result is in [-1, n).
+template <class F>
+__device__ __forceinline__ int wave_find_last(int n, F &&at_most) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, span = n;
+  for (;;) {
+    const int step = (span + 63) / 64;
+    const bool hit = lane * step < span && at_most(lo + lane * step);
+    const int hits = __builtin_popcountll(__builtin_amdgcn_ballot_w64(hit));
+    if (hits == 0) return lo - 1;  // (in the first round only, if at all)
+    lo += (hits - 1) * step;
+    if (step == 1) return lo;
+    span = min(step, span - (hits - 1) * step);
+  }
+}
+
+// By the first workgroup of a launch: IKV_STATUS_POSITION where row_start does
+// not ascend within [0, n_rows].
+__device__ __forceinline__ void check_row_start(const int32_t *row_start, int n_seq, int64_t n_rows, int *status) {
+  if (blockIdx.x != 0 || !status) return;
+  bool bad = false;
+  for (int s = threadIdx.x; s < n_seq; s += blockDim.x)
+    bad |= row_start[s] < 0 || row_start[s + 1] < row_start[s] || row_start[s + 1] > n_rows;
+  if (bad) raise_status(status, IKV_STATUS_POSITION);
+}
+
+// Prompts packed one behind the other: sequence s has rows [row_start[s],
+// row_start[s + 1]) of q, behind n_past[s] cached tokens.
+struct PackedSeqs {
+  const int32_t *row_start = nullptr;
+  const int32_t *n_past = nullptr;  // NULL: none
+  int n_seq = 0;
+  int n_rows = 0;    // of q, all sequences
+  int capacity = 0;  // tokens that a sequence may have
+  int64_t stride = 0;  // block table entries per sequence
+  int *status = nullptr;
+};
+
+// One block of `block` query rows (row = token * G + query head of the group)
+// of one sequence.
+struct PackedBlock {
+  int seq, first, rows, past;  // the sequence, its first row, its rows, its history
+  int n_blocks, item;          // its blocks, and which of them
+};
+
+// An upper bound on the blocks of all sequences: block_base(n_seq).
+__host__ __device__ inline int64_t packed_blocks(int64_t n_rows, int64_t n_seq, int G, int block) {
+  return n_rows * G / block + n_seq;
+}
+
+// The block that workgroup `item` takes, or false where there is none. Sequence
+// s may take items from row_start[s] * G / block + s on: that leaves it at least
+// the blocks that it has, whatever the lengths, so no list of blocks is needed.
+template <int BLOCK>
+__device__ __forceinline__ bool packed_block(const PackedSeqs &p, int G, int item, PackedBlock &b) {
+  check_row_start(p.row_start, p.n_seq, p.n_rows, p.status);
+  auto base = [&](int s) { return min(max(p.row_start[s], 0), p.n_rows) * G / BLOCK + s; };
+  b.seq = wave_find_last(p.n_seq, [&](int s) { return base(s) <= item; });
+  if (b.seq < 0) return false;
+  b.first = p.row_start[b.seq];
+  const int end = p.row_start[b.seq + 1];
+  b.past = p.n_past ? p.n_past[b.seq] : 0;
+  b.item = item - base(b.seq);
+  if (b.first < 0 || end < b.first || end > p.n_rows) return false;  // (check_row_start raises)
+  b.rows = end - b.first;
+  if (b.past < 0 || b.past > p.capacity - b.rows) {
+    if (b.rows > 0 && threadIdx.x == 0) raise_status(p.status, IKV_STATUS_POSITION);
+    return false;
+  }
+  b.n_blocks = (b.rows * G + BLOCK - 1) / BLOCK;
+  return b.item < b.n_blocks;
+}
+
+}  // namespace ikv

@@ -37,7 +37,17 @@ class KvPages(ctypes.Structure):
 
 _c_pages = ctypes.POINTER(KvPages)
 
-# name -> (restype, argtypes); include/ikv.h, then include/ikv_model.h
+
+class KvBatch(ctypes.Structure):
+    """ikv_kv_batch (include/ikv_batch.h): the block tables of several sequences."""
+    _fields_ = [("block_tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("block_tokens", ctypes.c_int64), ("n_pool_blocks", ctypes.c_int64),
+                ("n_seq", ctypes.c_int64), ("status", ctypes.c_void_p)]
+
+
+_c_batch = ctypes.POINTER(KvBatch)
+
+# name -> (restype, argtypes); include/ikv.h, ikv_batch.h, then ikv_model.h
 SIGNATURES = {
     "ikv_version": (ctypes.c_char_p, []),
     "ikv_append_f32": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_size_t, _c_void_p]),
@@ -121,6 +131,22 @@ SIGNATURES = {
         _c_int,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_float,
          _c_void_p, _c_void_p, _c_int64, _c_void_p, _c_void_p],
+    ),
+    # include/ikv_batch.h
+    "ikv_append_packed_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_int64,
+         _c_size_t, _c_void_p],
+    ),
+    "ikv_attn_prefill_packed_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_void_p, _c_int, _c_int,
+         _c_int, _c_float, _c_void_p, _c_void_p],
+    ),
+    "ikv_attn_prefill_packed_paged_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_int64, _c_void_p,
+         _c_int, _c_int, _c_int, _c_float, _c_void_p],
     ),
     # include/ikv_model.h
     "ikv_mul_mat_f32": (
@@ -548,6 +574,149 @@ def attn_prefill_paged(q, k_pool, v_pool, table, block_tokens: int, n_past: int 
                                            _ptr(out), n_head, n_head_kv, D, n_q, n_kv, n_past,
                                            scale, _stream(stream))
     _check("ikv_attn_prefill_paged_f32", rc)
+    return out
+
+
+# ----------------------------------------------------------------------------
+# a step over several sequences (include/ikv_batch.h): the pools as above, a
+# block table per sequence ([n_seq, blocks] int32), and the sequences' sizes as
+# device int32 tensors, which a captured call reads anew at every replay
+# ----------------------------------------------------------------------------
+
+def _operands(device, **tensors):
+    """Contiguous tensors on `device`: float32 ones, or int32 where the name
+    ends in _i. None is left out."""
+    torch = _torch()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        want = torch.int32 if name.endswith("_i") else torch.float32
+        if t.dtype is not want:
+            raise TypeError(f"{name.removesuffix('_i')} must be {want}, got {t.dtype}")
+        if t.device != device or not t.is_cuda:
+            raise ValueError(f"{name.removesuffix('_i')} must be on the device of the others")
+        if not t.is_contiguous():
+            raise ValueError(f"{name.removesuffix('_i')} must be contiguous")
+
+
+class _Here:
+    """The current device and stream as they are."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def _on(device, stream):
+    """The context of a launch on `device`: its current stream, or `stream`.
+    What is allocated in it belongs to that stream."""
+    torch = _torch()
+    if stream is None:
+        if torch.cuda.is_initialized() and torch._C._cuda_getDevice() == device.index:
+            return _here
+        return torch.cuda.stream(torch.cuda.current_stream(device))
+    if stream.device != device:
+        raise ValueError("stream and tensors must be on one device")
+    return torch.cuda.stream(stream)
+
+
+def kv_batch(tables, block_tokens: int, pool, status=None) -> KvBatch:
+    """The ikv_kv_batch descriptor of device int32 block tables [n_seq, blocks]
+    over `pool` (and the V pool of its shape)."""
+    if tables.dim() != 2:
+        raise ValueError("tables must be [n_seq, blocks]")
+    if block_tokens <= 0 or pool.shape[0] % block_tokens:
+        raise ValueError("pool rows must be whole blocks")
+    n_seq, width = tables.shape
+    return KvBatch(tables.data_ptr(), width, block_tokens, pool.shape[0] // block_tokens, n_seq,
+                   _ptr(status))
+
+
+def _need_pools(k_pool, v_pool, n_head_kv: int, head_dim: int) -> None:
+    if k_pool.dim() != 3 or k_pool.shape != v_pool.shape:
+        raise ValueError("k_pool and v_pool must be of one shape [rows, n_head_kv, head_dim]")
+    if k_pool.shape[1] != n_head_kv or k_pool.shape[2] != head_dim:
+        raise ValueError("the pools' heads differ from the rows'")
+
+
+def append_packed(k_pool, v_pool, k_rows, v_rows, tables, block_tokens: int, row_start,
+                  first_token=None, *, status=None, stream=None) -> None:
+    """Rows [row_start[s], row_start[s + 1]) of k_rows and v_rows [n, n_head_kv, D]
+    become sequence s's tokens first_token[s].. (0.. without it) in the pools."""
+    dev = k_pool.device
+    _operands(dev, k_pool=k_pool, v_pool=v_pool, k_rows=k_rows, v_rows=v_rows, tables_i=tables,
+              row_start_i=row_start, first_token_i=first_token, status_i=status)
+    if k_rows.dim() != 3 or k_rows.shape != v_rows.shape:
+        raise ValueError("k_rows and v_rows must be of one shape [rows, n_head_kv, head_dim]")
+    n_rows, n_head_kv, D = k_rows.shape
+    _need_pools(k_pool, v_pool, n_head_kv, D)
+    bt = kv_batch(tables, block_tokens, k_pool, status)
+    if row_start.numel() != bt.n_seq + 1:
+        raise ValueError("row_start must hold n_seq + 1 rows")
+    if first_token is not None and first_token.numel() != bt.n_seq:
+        raise ValueError("first_token must hold a token per sequence")
+    with _on(dev, stream):
+        _check("ikv_append_packed_f32",
+               load().ikv_append_packed_f32(_ptr(k_pool), _ptr(v_pool), _ptr(k_rows), _ptr(v_rows),
+                                            ctypes.byref(bt), _ptr(row_start), _ptr(first_token),
+                                            n_rows, n_head_kv * D * 4, _stream()))
+
+
+def attn_prefill_packed(q, k, v, row_start, *, out=None, scale: float = 0.0, status=None,
+                        stream=None):
+    """Causal attention of several prompts packed one behind the other: rows
+    [row_start[s], row_start[s + 1]) of q [n, n_head, D] and of k, v
+    [n, n_head_kv, D]. Rows of no sequence are left as `out` has them (an `out`
+    that is allocated here: undefined)."""
+    torch = _torch()
+    dev = q.device
+    _operands(dev, q=q, k=k, v=v, out=out, row_start_i=row_start, status_i=status)
+    n_rows, n_head, D = q.shape
+    if k.dim() != 3 or k.shape != v.shape or k.shape[0] != n_rows or k.shape[2] != D:
+        raise ValueError("k and v must be [rows of q, n_head_kv, head_dim]")
+    if row_start.numel() < 1:
+        raise ValueError("row_start must hold n_seq + 1 rows")
+    if out is not None and out.shape != q.shape:
+        raise ValueError("out must be of q's shape")
+    with _on(dev, stream):
+        if out is None:
+            out = torch.empty_like(q)
+        _check("ikv_attn_prefill_packed_f32",
+               load().ikv_attn_prefill_packed_f32(_ptr(q), _ptr(k), _ptr(v), _ptr(row_start),
+                                                  row_start.numel() - 1, n_rows, _ptr(out), n_head,
+                                                  k.shape[1], D, scale, _ptr(status), _stream()))
+    return out
+
+
+def attn_prefill_packed_paged(q, k_pool, v_pool, tables, block_tokens: int, row_start, n_past=None,
+                              *, out=None, scale: float = 0.0, status=None, stream=None):
+    """attn_prefill_packed over paged pools that hold the new rows already, each
+    sequence's queries behind n_past[s] cached tokens (none without it)."""
+    torch = _torch()
+    dev = q.device
+    _operands(dev, q=q, k_pool=k_pool, v_pool=v_pool, out=out, tables_i=tables,
+              row_start_i=row_start, n_past_i=n_past, status_i=status)
+    n_rows, n_head, D = q.shape
+    _need_pools(k_pool, v_pool, k_pool.shape[-2], D)
+    bt = kv_batch(tables, block_tokens, k_pool, status)
+    if row_start.numel() != bt.n_seq + 1:
+        raise ValueError("row_start must hold n_seq + 1 rows")
+    if n_past is not None and n_past.numel() != bt.n_seq:
+        raise ValueError("n_past must hold a count per sequence")
+    if out is not None and out.shape != q.shape:
+        raise ValueError("out must be of q's shape")
+    with _on(dev, stream):
+        if out is None:
+            out = torch.empty_like(q)
+        _check("ikv_attn_prefill_packed_paged_f32",
+               load().ikv_attn_prefill_packed_paged_f32(
+                   _ptr(q), _ptr(k_pool), _ptr(v_pool), ctypes.byref(bt), _ptr(row_start),
+                   _ptr(n_past), n_rows, _ptr(out), n_head, k_pool.shape[1], D, scale, _stream()))
     return out
 
 

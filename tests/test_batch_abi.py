@@ -1,0 +1,87 @@
+"""The entry points of a step over several sequences (include/ikv_batch.h) on
+the CPU: what they refuse before touching a device. No kernel is launched."""
+import ctypes
+import errno
+
+import pytest
+
+import ikv
+
+P = 4096  # a non-null, 16-byte aligned "device" address; never dereferenced
+
+
+def _batch(tables=P, stride=4, bt=64, pool=8, n_seq=3, status=None):
+    return ctypes.byref(ikv.KvBatch(tables, stride, bt, pool, n_seq, status))
+
+
+BAD_BATCHES = [
+    (None, errno.EINVAL),
+    (dict(tables=None), errno.EINVAL),
+    (dict(stride=0), errno.EINVAL), (dict(stride=-1), errno.EINVAL),
+    (dict(bt=0), errno.EINVAL), (dict(bt=32), errno.EINVAL), (dict(bt=-64), errno.EINVAL),
+    (dict(bt=100), errno.EINVAL),
+    (dict(pool=0), errno.EINVAL), (dict(n_seq=-1), errno.EINVAL),
+    (dict(pool=1 << 26), errno.EOVERFLOW),            # 2^32 pool rows
+    (dict(n_seq=(1 << 20) + 1), errno.EOVERFLOW),
+    (dict(stride=(1 << 22) + 1), errno.EOVERFLOW),    # past 2^28 tokens of a sequence
+]
+
+
+def _append(kp=P, vp=P, kr=P, vr=P, batch="ok", start=P, first=None, n=10, row_bytes=4096):
+    b = _batch() if batch == "ok" else batch
+    return ikv.load().ikv_append_packed_f32(kp, vp, kr, vr, b, start, first, n, row_bytes, None)
+
+
+@pytest.mark.parametrize("batch,code", BAD_BATCHES)
+def test_append_packed_refuses_a_bad_batch(batch, code):
+    assert _append(batch=None if batch is None else _batch(**batch)) == -code
+
+
+def test_append_packed_refuses_bad_arguments():
+    for name in ("kp", "vp", "kr", "vr", "start"):
+        assert _append(**{name: None}) == -errno.EINVAL, name
+    for name in ("kp", "vp", "kr", "vr"):
+        assert _append(**{name: P + 2}) == -errno.EINVAL, name
+    assert _append(row_bytes=6) == -errno.EINVAL
+    assert _append(n=-1) == -errno.EINVAL
+    assert _append(n=1 << 31) == -errno.EOVERFLOW
+    # nothing to do: nothing is launched
+    assert _append(n=0) == 0
+    assert _append(row_bytes=0) == 0
+    assert _append(batch=_batch(n_seq=0)) == 0
+
+
+def _packed(q=P, k=P, v=P, start=P, n_seq=3, n=10, out=P, n_head=16, n_head_kv=8, dim=128):
+    return ikv.load().ikv_attn_prefill_packed_f32(q, k, v, start, n_seq, n, out, n_head, n_head_kv, dim,
+                                                  0.0, None, None)
+
+
+def _packed_paged(q=P, k=P, v=P, batch="ok", start=P, past=None, n=10, out=P, n_head=16, n_head_kv=8,
+                  dim=128):
+    b = _batch() if batch == "ok" else batch
+    return ikv.load().ikv_attn_prefill_packed_paged_f32(q, k, v, b, start, past, n, out, n_head,
+                                                        n_head_kv, dim, 0.0, None)
+
+
+@pytest.mark.parametrize("batch,code", BAD_BATCHES)
+def test_packed_prefill_refuses_a_bad_batch(batch, code):
+    assert _packed_paged(batch=None if batch is None else _batch(**batch)) == -code
+
+
+@pytest.mark.parametrize("call", [_packed, _packed_paged])
+def test_packed_prefill_refuses_bad_arguments(call):
+    for name in ("q", "k", "v", "start", "out"):
+        assert call(**{name: None}) == -errno.EINVAL, name
+    assert call(n_head=12) == -errno.EINVAL  # not a multiple of n_head_kv
+    assert call(n_head=0) == -errno.EINVAL
+    assert call(n_head_kv=0) == -errno.EINVAL
+    assert call(dim=0) == -errno.EINVAL
+    assert call(dim=513) == -errno.ENOTSUP
+    assert call(n=-1) == -errno.EINVAL
+    assert call(n=1 << 25) == -errno.EOVERFLOW
+    assert call(n=0) == 0  # nothing is launched
+    if call is _packed:
+        assert call(n_seq=-1) == -errno.EINVAL
+        assert call(n_seq=(1 << 20) + 1) == -errno.EOVERFLOW
+        assert call(n_seq=1 << 20, n=1, n_head=4096, n_head_kv=4096) == -errno.EOVERFLOW  # 2^32 blocks
+        assert call(n_seq=0) == 0

@@ -1,0 +1,198 @@
+"""Causal attention over packed prompts, against 64 bits: contiguous and paged,
+with histories, empty sequences and rows of no sequence."""
+import pytest
+import torch
+
+import ikv
+from batch_ref import NORMAL_REL, assert_near, attention64, attention_bound, rows_of, starts, tables_for
+
+pytestmark = pytest.mark.gpu
+
+FILL = -777.0
+
+# query heads, KV heads, head_dim: the piece kernel's (multiples of 4 up to
+# 128), and the generic one's
+HEADS = [(16, 8, 128), (4, 4, 64), (12, 4, 64), (8, 1, 80), (6, 2, 4), (5, 5, 36),
+         (3, 1, 65), (4, 2, 200), (2, 1, 512), (2, 2, 1)]
+# rows of each sequence
+ROWS = [[1], [1, 1, 1], [3, 0, 1, 0, 40], [130, 1, 64, 65, 33], [0, 0, 300], [2] * 70 + [90]]
+
+
+def _inputs(dev, seed, n, heads, kv, dim):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    return rnd(n, heads, dim), rnd(n, kv, dim), rnd(n, kv, dim)
+
+
+def _dev32(x, dev):
+    return torch.as_tensor(x, dtype=torch.int32).to(dev)
+
+
+@pytest.mark.parametrize("heads,kv,dim", HEADS)
+@pytest.mark.parametrize("rows", ROWS, ids=lambda r: f"{len(r)}seqs{sum(r)}")
+def test_packed_prompts(dev, heads, kv, dim, rows):
+    n, pad = sum(rows), 5
+    q, k, v = _inputs(dev, 3 + n + dim, n + pad, heads, kv, dim)
+    for t in (q, k, v):  # rows of no sequence: not read
+        t[n:] = float("nan")
+    out = torch.full_like(q, FILL)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    ikv.attn_prefill_packed(q, k, v, _dev32(starts(rows), dev), out=out, status=status)
+    assert status.item() == 0
+    assert (out[n:] == FILL).all()
+    at = 0
+    for r in rows:
+        if r:
+            s = slice(at, at + r)
+            assert_near(out[s], attention64(q[s], k[s], v[s], 0), attention_bound(q[s], k[s], v[s]))
+        at += r
+
+
+def _paged(dev, seed, rows, past, bt, heads, kv, dim):
+    """q, pools, tables, and every sequence's own keys and values."""
+    total = [r + p for r, p in zip(rows, past)]
+    tables, blocks = tables_for(total, bt, seed)
+    q, _, _ = _inputs(dev, seed, sum(rows), heads, kv, dim)
+    pools = [torch.full((blocks * bt, kv, dim), float("nan"), device=dev) for _ in range(2)]
+    own = []
+    for s, n in enumerate(total):
+        _, k, v = _inputs(dev, seed + 1 + s, n, heads, kv, dim)
+        at = torch.tensor(rows_of(tables, s, bt, range(n)), dtype=torch.long, device=dev)
+        pools[0][at], pools[1][at] = k, v
+        own.append((k, v))
+    return q, pools, tables, own
+
+
+@pytest.mark.parametrize("heads,kv,dim", HEADS)
+@pytest.mark.parametrize("rows,past,bt", [([1], [0], 64), ([1, 5, 0, 70], [63, 64, 9, 0], 64),
+                                          ([40, 129], [700, 1], 128), ([3] * 66, list(range(66)), 64)])
+def test_packed_prompts_on_pages(dev, heads, kv, dim, rows, past, bt):
+    """Pool rows that hold no token of a sequence are NaN, entries behind its
+    blocks are -1: neither is read."""
+    q, pools, tables, own = _paged(dev, 5 + sum(rows) + dim, rows, past, bt, heads, kv, dim)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = ikv.attn_prefill_packed_paged(q, *pools, _dev32(tables, dev), bt, _dev32(starts(rows), dev),
+                                        _dev32(past, dev), status=status)
+    assert status.item() == 0
+    at = 0
+    for r, p, (k, v) in zip(rows, past, own):
+        if r:
+            qs = q[at:at + r]
+            assert_near(out[at:at + r], attention64(qs, k, v, p), attention_bound(qs, k, v))
+        at += r
+
+
+def test_packed_prompts_of_every_size_class(dev):
+    """Few rows and many take different forms of the kernel."""
+    for heads, kv, dim, n in ((16, 8, 128, 500), (16, 8, 128, 4200), (32, 8, 64, 400), (32, 8, 64, 3000)):
+        rows = [n // 2, n // 3, n - n // 2 - n // 3]
+        q, k, v = _inputs(dev, n, n, heads, kv, dim)
+        out = ikv.attn_prefill_packed(q, k, v, _dev32(starts(rows), dev))
+        at = 0
+        for r in rows:
+            s = slice(at, at + r)
+            assert_near(out[s], attention64(q[s], k[s], v[s], 0), attention_bound(q[s], k[s], v[s]))
+            at += r
+
+
+def test_packed_prompts_scale(dev):
+    q, k, v = _inputs(dev, 9, 50, 4, 2, 64)
+    out = ikv.attn_prefill_packed(q, k, v, _dev32([0, 20, 50], dev), scale=0.5)
+    for s in (slice(0, 20), slice(20, 50)):
+        assert_near(out[s], attention64(q[s], k[s], v[s], 0, 0.5), attention_bound(q[s], k[s], v[s], 0.5),
+                    rel=4 * NORMAL_REL)  # scores four times as large
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 8, 128), (3, 1, 65)])
+def test_packed_prompts_keep_nan_and_infinity_to_their_rows(dev, heads, kv, dim):
+    """A NaN key of one sequence, an infinite value of its last token: only the
+    rows that see them have them."""
+    rows = [40, 30, 50]
+    q, k, v = _inputs(dev, 21, 120, heads, kv, dim)
+    clean = ikv.attn_prefill_packed(q, k, v, _dev32(starts(rows), dev))
+    k[55] = float("nan")           # token 15 of sequence 1
+    v[119, :, 0] = float("inf")    # the last token of sequence 2
+    out = ikv.attn_prefill_packed(q, k, v, _dev32(starts(rows), dev))
+    for s in (slice(0, 40), slice(70, 119)):
+        assert_near(out[s], clean[s].cpu().double(), 2 * attention_bound(q[s], k[s], v[s].clamp(max=10)),
+                    2 * NORMAL_REL)
+    assert_near(out[40:55], clean[40:55].cpu().double(),
+                2 * attention_bound(q[40:55], k[40:55], v[40:55]), 2 * NORMAL_REL)
+    assert torch.isnan(out[55:70]).all()
+    assert torch.isinf(out[119, :, 0]).all() and torch.isfinite(out[119, :, 1:]).all()
+
+
+def test_packed_prompts_skip_what_does_not_fit(dev):
+    """Sequences past their table or of a negative history are left as they
+    were and flagged; blocks outside the pool read block 0 and are flagged."""
+    rows, bt = [10, 10, 10], 64
+    q, pools, tables, own = _paged(dev, 77, rows, [0, 0, 0], bt, 4, 2, 64)
+    start, tab = _dev32(starts(rows), dev), _dev32(tables, dev)
+    for past in ([0, 55, 0], [0, -1, 0]):
+        out = torch.full_like(q, FILL)
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        ikv.attn_prefill_packed_paged(q, *pools, tab, bt, start, _dev32(past, dev), out=out, status=status)
+        assert status.item() == ikv.STATUS_POSITION
+        assert (out[10:20] == FILL).all()
+        for s in (0, 2):
+            at = slice(10 * s, 10 * s + 10)
+            assert_near(out[at], attention64(q[at], *own[s], 0), attention_bound(q[at], *own[s]))
+    tab[1, 0] = 10 ** 6
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    ikv.attn_prefill_packed_paged(q, pools[0].nan_to_num(), pools[1].nan_to_num(), tab, bt, start, status=status)
+    assert status.item() == ikv.STATUS_BLOCK
+    for bad in ([0, 20, 10, 30], [0, 10, 20, 31], [-1, 10, 20, 30]):
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        ikv.attn_prefill_packed(q, q[:, :2].contiguous(), q[:, :2].contiguous(), _dev32(bad, dev), status=status)
+        assert status.item() == ikv.STATUS_POSITION
+
+
+def test_packed_prompts_replay_with_new_sizes(dev):
+    heads, kv, dim, n = 12, 4, 64, 200
+    q, k, v = _inputs(dev, 31, n, heads, kv, dim)
+    start = _dev32([0, 50, 100, 200], dev)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ikv.attn_prefill_packed(q, k, v, start, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ikv.attn_prefill_packed(q, k, v, start, out=out)
+    for sizes in ([50, 50, 100], [200, 0, 0], [1, 198, 1], [0, 70, 30]):
+        start.copy_(torch.from_numpy(starts(sizes)))
+        q.normal_()
+        out.fill_(FILL)
+        graph.replay()
+        torch.cuda.synchronize()
+        at = 0
+        for r in sizes:
+            s = slice(at, at + r)
+            if r:
+                assert_near(out[s], attention64(q[s], k[s], v[s], 0), attention_bound(q[s], k[s], v[s]))
+            at += r
+        assert (out[at:] == FILL).all()
+
+
+def test_packed_prompts_on_another_stream(dev):
+    """What the call allocates belongs to the stream that it runs on."""
+    q, k, v = _inputs(dev, 41, 300, 16, 8, 128)
+    start = _dev32([0, 100, 300], dev)
+    want = ikv.attn_prefill_packed(q, k, v, start)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = [ikv.attn_prefill_packed(q, k, v, start, stream=side) for _ in range(4)]
+    side.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_packed_prompts_refuse_mixed_operands(dev):
+    q, k, v = _inputs(dev, 1, 4, 4, 2, 16)
+    start = _dev32([0, 4], dev)
+    for change, error in ((dict(k=k.half()), TypeError), (dict(row_start=start.long()), TypeError),
+                          (dict(v=v.cpu()), ValueError), (dict(k=k[:3]), ValueError),
+                          (dict(q=q.transpose(0, 1)), ValueError), (dict(k=k[..., :8].contiguous(), v=v[..., :8].contiguous()), ValueError),
+                          (dict(out=q[:3].clone()), ValueError), (dict(row_start=start[:0]), ValueError)):
+        with pytest.raises(error):
+            ikv.attn_prefill_packed(**{**dict(q=q, k=k, v=v, row_start=start), **change})
