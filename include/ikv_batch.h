@@ -100,6 +100,38 @@ int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_pool, const
                                       const int32_t *n_past, int64_t n_rows, float *out, int n_head,
                                       int n_head_kv, int head_dim, float scale, void *stream);
 
+/* ---------------------------------------------------------------------
+ * Decode attention of one new token of each sequence over a paged cache, the
+ * contexts' total length split over the compute units and joined.
+ *   q, out   [n_seq][n_head][head_dim]
+ *   n_kv     [n_seq] int32: the keys of each sequence, its new token's among
+ *            them. 0 is an idle slot: its out row is zeros and nothing else of
+ *            it is read or written. A negative length or one that the table
+ *            does not cover raises IKV_STATUS_POSITION and is taken for 0.
+ *   k_new, v_new  NULL, or the new tokens' rows [n_seq][n_head_kv][head_dim]:
+ *            row n_kv[s] - 1 of sequence s is then read from them and written
+ *            to the pools (other sequences' rows of the call must not be among
+ *            the rows that are written; a row whose block entry is outside the
+ *            pool is read and not written).
+ *   scale    softmax scale; <= 0 selects 1/sqrtf(head_dim)
+ *   workspace  device memory of ikv_attn_decode_batch_workspace_bytes() bytes,
+ *            16-byte aligned; nothing is expected in it or left in it. It does
+ *            not depend on the number of sequences or their lengths. Launches
+ *            that share it must be ordered (one stream); concurrent ones race.
+ * Any head_dim up to 512 (else -ENOTSUP) and any n_head that n_head_kv divides;
+ * 4-byte aligned operands. A result depends on the other sequences' lengths by
+ * the order of its sums, and on nothing else of them; equal calls give equal
+ * bits. -EINVAL: a missing or small workspace; -EOVERFLOW: n_head_kv * head_dim
+ * past 2^23.
+ * ------------------------------------------------------------------- */
+size_t ikv_attn_decode_batch_workspace_bytes(int n_head, int n_head_kv, int head_dim);
+
+int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,
+                              const ikv_kv_batch *batch, const int32_t *n_kv, const float *k_new,
+                              const float *v_new, float *out, int n_head, int n_head_kv,
+                              int head_dim, float scale, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,544 @@
+// attn_decode_batch.hip — one new token of each of several sequences over a
+// paged KV cache (ikv_attn_decode_batch_f32): GQA attention over contexts of
+// different lengths, the new rows' append fused.
+//
+// HBM bounds it: every K and V row is read once and takes 4 G flops a float.
+//
+//   * The work is cut into units of KT keys of one KV head of one sequence, in
+//     the order (sequence, KV head, keys). The workgroups take equal runs of
+//     units, however the lengths differ, from n_kv as it stands on the device:
+//     each workgroup adds up the lengths itself.
+//   * A run may end inside a (sequence, head): the workgroup then leaves the
+//     maximum, sum and weighted values of its part in the workspace (at most
+//     two parts a workgroup, so the workspace depends on no length), and a
+//     second launch joins the parts in their order.
+//   * LPK lanes hold a key row, NV 16-byte pieces each, so a wave loads 64 / LPK
+//     keys at once; the scores need only the sum over LPK lanes, and each group
+//     of LPK lanes has a running maximum and sums of its own, which meet when
+//     the run leaves the head. The maximum moves only when a score exceeds it
+//     by 2^8.
+//   * A sequence's next 64 block table entries are held one per lane.
+#include "batch.hpp"
+#include "coherent.hpp"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int kCUs = 256;       // MI355X compute units
+constexpr int kWaves = 4;       // of a workgroup
+constexpr int kGroups = 2 * kCUs;
+constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
+constexpr int kMaxDim = 512;
+constexpr int kAhead = 2;  // keys of a lane group loaded at once
+
+struct Args {
+  const float *q;
+  float *k, *v;
+  const float *k_new, *v_new;
+  float *out;
+  const int32_t *n_kv;
+  ikv::BatchPages b;
+  int n_head_kv, G, dim;
+  int passes;  // a KV head's query heads are taken GQ at a time
+  float scale_log2;
+  float *part;
+};
+
+// Keys of a sequence; 0 for an idle slot and for a length that is out of range.
+__device__ __forceinline__ int keys_of(const Args &a, int seq) {
+  const int n = a.n_kv[seq];
+  return n > 0 && n <= a.b.capacity ? n : 0;
+}
+
+__device__ __forceinline__ long long wave_prefix(long long x) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const long long y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// A place in the list of units: unit `tile` of `tiles` of head pass `item`.
+struct Place {
+  int seq, keys, tiles, item, tile;
+};
+
+template <int KT>
+struct Plan {
+  long long total, chunk;
+
+  __device__ static int tiles_of(int keys) { return (keys + KT - 1) / KT; }
+
+  __device__ Plan(const Args &a) {
+    const int lane = threadIdx.x & 63;
+    long long t = 0;
+    for (int s = lane; s < a.b.n_seq; s += 64) t += tiles_of(keys_of(a, s));
+    total = __shfl(wave_prefix(t), 63, 64) * (static_cast<long long>(a.n_head_kv) * a.passes);
+    chunk = (total + kGroups - 1) / kGroups;
+  }
+
+  // where unit u (< total) is
+  __device__ Place at(const Args &a, long long u) const {
+    const int lane = threadIdx.x & 63;
+    const long long items = static_cast<long long>(a.n_head_kv) * a.passes;
+    long long base = 0;
+    Place p{};
+    for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
+      const int keys = s0 + lane < a.b.n_seq ? keys_of(a, s0 + lane) : 0;
+      const long long mine = tiles_of(keys) * items;
+      const long long upto = base + wave_prefix(mine);
+      const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > u);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        p.seq = s0 + l;
+        p.keys = __builtin_amdgcn_readlane(keys, l);
+        p.tiles = tiles_of(p.keys);
+        const long long r = u - __shfl(upto - mine, l, 64);
+        p.item = static_cast<int>(r / p.tiles);
+        p.tile = static_cast<int>(r - static_cast<long long>(p.item) * p.tiles);
+        p.item = __builtin_amdgcn_readfirstlane(p.item);
+        p.tile = __builtin_amdgcn_readfirstlane(p.tile);
+        return p;
+      }
+      base = __shfl(upto, 63, 64);
+    }
+    return p;  // (not reached for u < total)
+  }
+
+  // the first unit of the next head pass
+  __device__ void next(const Args &a, Place &p) const {
+    p.tile = 0;
+    if (++p.item < a.n_head_kv * a.passes) return;
+    p.item = 0;
+    const int lane = threadIdx.x & 63;
+    for (int s0 = p.seq + 1; s0 < a.b.n_seq; s0 += 64) {
+      const int keys = s0 + lane < a.b.n_seq ? keys_of(a, s0 + lane) : 0;
+      const unsigned long long some = __builtin_amdgcn_ballot_w64(keys > 0);
+      if (some) {
+        const int l = __builtin_ctzll(some);
+        p.seq = s0 + l;
+        p.keys = __builtin_amdgcn_readlane(keys, l);
+        p.tiles = tiles_of(p.keys);
+        return;
+      }
+    }
+  }
+};
+
+template <int LPK>
+__device__ __forceinline__ float lanes_sum(float x) {  // over a key's lanes
+  x += ikv::dpp<ikv::kDppXor1>(x);
+  x += ikv::dpp<ikv::kDppXor2>(x);
+  x += ikv::dpp<ikv::kDppHalfMirror>(x);
+  if constexpr (LPK >= 16) x += ikv::dpp<ikv::kDppMirror>(x);
+  if constexpr (LPK >= 32) {
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  return x;
+}
+
+constexpr int kDppRor8 = 0x128;  // lane i <-> i ^ 8 within 16 lanes
+
+// f over the lanes that hold the same dims of the wave's keys
+template <int LPK, class F>
+__device__ __forceinline__ float across_keys(float x, F &&f) {
+  if constexpr (LPK <= 8) x = f(x, ikv::dpp<kDppRor8>(x));
+  if constexpr (LPK <= 16) {
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  }
+  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+
+__device__ __forceinline__ float weight(float m, float top) {  // of sums kept at maximum m
+  return m == -INFINITY ? 0.f : ikv::fast_exp2(m - top);
+}
+
+// The workspace: (maximum, sum) of each part's heads, then their values. Part
+// 2 w is workgroup w's of a head that began before its run, 2 w + 1 of one that
+// goes on behind it.
+template <int GQ, int DP>
+struct Parts {
+  float *ml, *o;
+  __device__ explicit Parts(float *p) : ml(p), o(p + static_cast<size_t>(kGroups) * 2 * GQ * 2) {}
+  __device__ float *ml_of(int part, int h) const { return ml + (static_cast<size_t>(part) * GQ + h) * 2; }
+  __device__ float *o_of(int part, int h) const { return o + (static_cast<size_t>(part) * GQ + h) * DP; }
+};
+
+template <int LPK, int NV, int GQ, bool VEC>
+__global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_kernel(Args a) {
+  constexpr int KPW = 64 / LPK;               // keys that a wave loads at once
+  constexpr int KT = kWaves * kAhead * KPW;   // keys of a unit
+  constexpr int DP = LPK * NV * 4;            // dims held
+  static_assert(64 % KT == 0, "a unit stays within a block");
+  __shared__ float s_m[kWaves][GQ], s_l[kWaves][GQ];
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][GQ][DP];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = lane % LPK, grp = lane / LPK;
+  const int n_head = a.n_head_kv * a.G;
+  const int stride = a.n_head_kv * a.dim;  // floats of a token row
+
+  // slots without keys: a zero row, and the flag where the length is no length
+  for (int s = blockIdx.x; s < a.b.n_seq; s += gridDim.x) {
+    if (keys_of(a, s) > 0) continue;
+    if (a.n_kv[s] != 0 && threadIdx.x == 0) ikv::raise_status(a.b.status, IKV_STATUS_POSITION);
+    float *o = a.out + static_cast<size_t>(s) * n_head * a.dim;
+    for (int d = threadIdx.x; d < n_head * a.dim; d += kWaves * 64) o[d] = 0.f;
+  }
+
+  const Plan<KT> plan(a);
+  long long u = plan.chunk * blockIdx.x;
+  const long long end = min(plan.total, u + plan.chunk);
+  if (u >= end) return;
+  Place p = plan.at(a, u);
+  unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int d = 4 * (l + LPK * n);
+    off[n] = d < a.dim ? static_cast<unsigned>(d) * 4 : 0x80000000u;
+  }
+  auto load = [&](__amdgpu_buffer_rsrc_t r, unsigned at, int n) -> float4 {  // piece n of the row at `at`
+    if constexpr (VEC) {
+      return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(r, at + off[n], 0, 0));
+    } else {
+      const int d = 4 * (l + LPK * n);
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                             r, d + e < a.dim ? at + (d + e) * 4u : 0x80000000u, 0, 0));
+      return make_float4(x[0], x[1], x[2], x[3]);
+    }
+  };
+  auto whole_row = [&](const float *row) {  // a row of head_dim floats on its own
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(row), 0, a.dim * 4, ikv::kBufWord3);
+  };
+  auto store = [&](float *row, int n, float4 x) {
+    const int d = 4 * (l + LPK * n);
+    if constexpr (VEC) {
+      if (d < a.dim) *reinterpret_cast<float4 *>(row + d) = x;
+    } else {
+      const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < a.dim) row[d + e] = y[e];
+    }
+  };
+
+  while (u < end) {
+    // the run's part of one (sequence, KV head, pass): tiles [p.tile, last)
+    const int last = static_cast<int>(min(static_cast<long long>(p.tiles), p.tile + (end - u)));
+    const int g = p.item / a.passes, h0 = p.item % a.passes * GQ;
+    const int heads = min(GQ, a.G - h0);
+    const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
+    const size_t head0 = static_cast<size_t>(p.seq) * n_head + g * a.G + h0;
+    float4 qv[GQ][NV], o[GQ][NV];
+    float m[GQ], sum[GQ];
+#pragma unroll
+    for (int h = 0; h < GQ; ++h) {
+      m[h] = -INFINITY;
+      sum[h] = 0.f;
+      const auto r = whole_row(a.q + (head0 + min(h, heads - 1)) * a.dim);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        qv[h][n] = ikv::scale4(a.scale_log2, load(r, 0, n));
+        o[h][n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    // block table entries, 64 at a time, one per lane, checked as they are read
+    const int last_blk = (p.keys - 1) / pg.bt;
+    int blk = p.tile * KT / pg.bt, in_blk = p.tile * KT % pg.bt, ent0 = blk, ent = 0;
+    auto entries = [&]() {
+      ent0 = blk;
+      ent = pg.table[min(blk + lane, last_blk)];
+      if (static_cast<unsigned>(ent) >= static_cast<unsigned>(pg.n_blocks)) {
+        ikv::raise_status(pg.status, IKV_STATUS_BLOCK);
+        ent = -1;
+      }
+    };
+    entries();
+    float4 kr[kAhead][NV], vr[kAhead][NV];
+    const int mine = wave * kAhead * KPW + grp;  // this lane's first key of a unit, then + KPW
+    // row of the tile at (blk, in_blk), moved on to the next tile; ~row of
+    // block 0's where the entry names no block
+    auto next_row = [&]() -> long long {
+      const int e = __builtin_amdgcn_readlane(ent, blk - ent0);
+      const long long row = e < 0 ? ~static_cast<long long>(in_blk) : static_cast<long long>(e) * pg.bt + in_blk;
+      in_blk += KT;
+      if (in_blk == pg.bt) {
+        in_blk = 0;
+        if (++blk - ent0 >= 64) entries();
+      }
+      return row;
+    };
+    auto fetch = [&](const float *pool, const float *fresh, long long row, int tile, float4 (&x)[kAhead][NV]) {
+      const int rows = min(KT, p.keys - tile * KT);
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float *>(pool + (row < 0 ? ~row : row) * stride + g * a.dim), 0,
+          ((rows - 1) * stride + a.dim) * 4, ikv::kBufWord3);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int key = mine + KPW * i;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) x[i][n] = load(r, static_cast<unsigned>(key) * stride * 4u, n);
+      }
+      if (fresh && tile == p.tiles - 1) {  // the new token's row comes from the caller
+        const auto f = whole_row(fresh + static_cast<size_t>(p.seq) * stride + g * a.dim);
+        float *const to = const_cast<float *>(pool) + (row + rows - 1) * stride + g * a.dim;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (mine + KPW * i == rows - 1) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+              x[i][n] = load(f, 0, n);
+              if (row >= 0 && h0 == 0) store(to, n, x[i][n]);
+            }
+          }
+        }
+      }
+    };
+
+    long long row = next_row();
+    fetch(a.k, a.k_new, row, p.tile, kr);
+    fetch(a.v, a.v_new, row, p.tile, vr);
+    for (int t = p.tile; t < last; ++t) {
+      float s[kAhead][GQ];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const bool seen = t * KT + mine + KPW * i < p.keys;
+#pragma unroll
+        for (int h = 0; h < GQ; ++h) {
+          float x = 0.f;
+#pragma unroll
+          for (int n = 0; n < NV; ++n) x += ikv::dot4(qv[h][n], kr[i][n]);
+          s[i][h] = lanes_sum<LPK>(x);
+          if (!seen) s[i][h] = -INFINITY;
+        }
+      }
+      const bool more = t + 1 < last;
+      if (more) {
+        row = next_row();
+        fetch(a.k, a.k_new, row, t + 1, kr);
+      }
+      bool move = false;
+#pragma unroll
+      for (int h = 0; h < GQ; ++h)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) move |= s[i][h] > m[h] + kRescale;
+      if (__builtin_amdgcn_ballot_w64(move) != 0) {
+#pragma unroll
+        for (int h = 0; h < GQ; ++h) {
+          float top = m[h];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) top = fmaxf(top, s[i][h]);
+          const float f = weight(m[h], top);
+          m[h] = top;
+          sum[h] *= f;
+#pragma unroll
+          for (int n = 0; n < NV; ++n) o[h][n] = ikv::scale4(f, o[h][n]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < GQ; ++h) {
+        const float ref = m[h] == -INFINITY ? 0.f : m[h];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const float w = ikv::fast_exp2(s[i][h] - ref);
+          sum[h] += w;
+#pragma unroll
+          for (int n = 0; n < NV; ++n) o[h][n] = ikv::fma4(w, vr[i][n], o[h][n]);
+        }
+      }
+      if (more) fetch(a.v, a.v_new, row, t + 1, vr);
+    }
+
+    // the lane groups and the waves meet
+#pragma unroll
+    for (int h = 0; h < GQ; ++h) {
+      const float top = across_keys<LPK>(m[h], [](float x, float y) { return fmaxf(x, y); });
+      const float f = weight(m[h], top);
+      auto add = [](float x, float y) { return x + y; };
+      const float all = across_keys<LPK>(sum[h] * f, add);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const float4 x = ikv::scale4(f, o[h][n]);
+        const float4 y = make_float4(across_keys<LPK>(x.x, add), across_keys<LPK>(x.y, add),
+                                     across_keys<LPK>(x.z, add), across_keys<LPK>(x.w, add));
+        if (grp == 0) *reinterpret_cast<float4 *>(&s_o[wave][h][4 * (l + LPK * n)]) = y;
+      }
+      if (lane == 0) {
+        s_m[wave][h] = top;
+        s_l[wave][h] = all;
+      }
+    }
+    __syncthreads();
+    const bool whole = p.tile == 0 && last == p.tiles;
+    const Parts<GQ, DP> parts(a.part);
+    const int part = 2 * static_cast<int>(blockIdx.x) + (p.tile == 0 ? 1 : 0);
+    for (int i = threadIdx.x; i < GQ * DP; i += kWaves * 64) {
+      const int h = i / DP, d = i % DP;
+      if (h >= heads) break;
+      float top = s_m[0][h];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][h]);
+      float all = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = weight(s_m[w][h], top);
+        all = fmaf(f, s_l[w][h], all);
+        x = fmaf(f, s_o[w][h][d], x);
+      }
+      if (whole) {
+        if (d < a.dim) a.out[(head0 + h) * a.dim + d] = x / all;
+      } else {
+        parts.o_of(part, h)[d] = x;
+        if (d == 0) {
+          parts.ml_of(part, h)[0] = top;
+          parts.ml_of(part, h)[1] = all;
+        }
+      }
+    }
+    __syncthreads();
+    u += last - p.tile;
+    plan.next(a, p);
+  }
+}
+
+// Joins the parts of the head pass that begins in workgroup blockIdx.x's run
+// and goes on behind it: that workgroup's, then one of each run it goes through.
+template <int LPK, int NV, int GQ>
+__global__ __launch_bounds__(256) void decode_batch_join_kernel(Args a) {
+  constexpr int KT = kWaves * kAhead * (64 / LPK);
+  constexpr int DP = LPK * NV * 4;
+  __shared__ float s_top[GQ], s_all[GQ];
+  const Plan<KT> plan(a);
+  const long long begin = plan.chunk * blockIdx.x, end = min(plan.total, begin + plan.chunk);
+  if (begin >= end || end == plan.total) return;
+  const Place p = plan.at(a, end - 1);
+  if (p.tile + 1 == p.tiles) return;            // it ends with the run
+  if (end - 1 - p.tile < begin) return;         // it began before the run
+  const int w0 = blockIdx.x;
+  const int n = static_cast<int>((end - 1 - p.tile + p.tiles - 1) / plan.chunk) - w0 + 1;  // parts
+  const int h0 = p.item % a.passes * GQ, g = p.item / a.passes;
+  const int heads = min(GQ, a.G - h0);
+  const Parts<GQ, DP> parts(a.part);
+  auto part = [&](int i) { return i == 0 ? 2 * w0 + 1 : 2 * (w0 + i); };
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int h = wave; h < heads; h += 4) {
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, parts.ml_of(part(i), h)[0]);
+    top = ikv::wave_max(top);
+    float all = 0.f;
+    for (int i = lane; i < n; i += 64) {
+      const float *ml = parts.ml_of(part(i), h);
+      all = fmaf(weight(ml[0], top), ml[1], all);
+    }
+    all = ikv::wave_sum(all);
+    if (lane == 0) {
+      s_top[h] = top;
+      s_all[h] = all;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * DP; i += 256) {
+    const int h = i / DP, d = i % DP;
+    if (d >= a.dim) continue;
+    const float top = s_top[h];
+    float x = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j)
+      x = fmaf(weight(parts.ml_of(part(j), h)[0], top), parts.o_of(part(j), h)[d], x);
+    a.out[((static_cast<size_t>(p.seq) * a.n_head_kv + g) * a.G + h0 + h) * a.dim + d] = x / s_all[h];
+  }
+}
+
+// The form of a shape: lanes per key and 16-byte pieces of a lane (head_dim up
+// to 16 LPK NV / 4), query heads taken at once.
+struct Form {
+  int lpk, nv, gq;
+};
+Form form_of(int G, int dim) {
+  Form f;
+  f.lpk = dim <= 128 ? 8 : dim <= 256 ? 16 : 32;
+  f.nv = dim <= 128 ? (dim + 31) / 32 : 4;
+  f.gq = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8;
+  return f;
+}
+
+template <int LPK, int NV, int GQ>
+int launch(const Args &a, bool vec, hipStream_t s) {
+  if (vec)
+    decode_batch_kernel<LPK, NV, GQ, true><<<kGroups, kWaves * 64, 0, s>>>(a);
+  else
+    decode_batch_kernel<LPK, NV, GQ, false><<<kGroups, kWaves * 64, 0, s>>>(a);
+  decode_batch_join_kernel<LPK, NV, GQ><<<kGroups, 256, 0, s>>>(a);
+  return ikv::launch_status();
+}
+
+}  // namespace
+
+extern "C" size_t ikv_attn_decode_batch_workspace_bytes(int n_head, int n_head_kv, int head_dim) {
+  if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || head_dim > kMaxDim) return 0;
+  const Form f = form_of(n_head / n_head_kv, head_dim);
+  return static_cast<size_t>(kGroups) * 2 * f.gq * (f.lpk * f.nv * 4 + 2) * sizeof(float);
+}
+
+extern "C" int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,
+                                         const ikv_kv_batch *batch, const int32_t *n_kv,
+                                         const float *k_new, const float *v_new, float *out, int n_head,
+                                         int n_head_kv, int head_dim, float scale, void *workspace,
+                                         size_t workspace_bytes, void *stream) {
+  Args a;
+  if (const int rc = ikv::batch_arg(batch, a.b)) return rc;
+  if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0) return -EINVAL;
+  if (head_dim > kMaxDim) return -ENOTSUP;
+  if (a.b.n_seq == 0) return 0;
+  if (!q || !k_pool || !v_pool || !n_kv || !out || (k_new == nullptr) != (v_new == nullptr)) return -EINVAL;
+  if (!workspace || !ikv::aligned16(workspace) ||
+      workspace_bytes < ikv_attn_decode_batch_workspace_bytes(n_head, n_head_kv, head_dim))
+    return -EINVAL;
+  // a unit's rows are one buffer range; a sequence's heads index in int
+  if (n_head_kv > INT_MAX / (64 * 4) / head_dim || n_head > INT_MAX / head_dim) return -EOVERFLOW;
+  const int G = n_head / n_head_kv;
+  const Form f = form_of(G, head_dim);
+  if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
+  a.q = q;
+  a.k = k_pool;
+  a.v = v_pool;
+  a.k_new = k_new;
+  a.v_new = v_new;
+  a.out = out;
+  a.n_kv = n_kv;
+  a.n_head_kv = n_head_kv;
+  a.G = G;
+  a.dim = head_dim;
+  a.passes = (G + f.gq - 1) / f.gq;
+  a.scale_log2 = scale * ikv::kLog2e;
+  a.part = static_cast<float *>(workspace);
+  bool vec = head_dim % 4 == 0;
+  for (const void *x : {static_cast<const void *>(q), static_cast<const void *>(k_pool),
+                        static_cast<const void *>(v_pool), static_cast<const void *>(k_new),
+                        static_cast<const void *>(v_new)})
+    vec = vec && ikv::aligned16(x);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define IKV_GQ(LPK, NV)                                 \
+  switch (f.gq) {                                       \
+    case 1: return launch<LPK, NV, 1>(a, vec, s);       \
+    case 2: return launch<LPK, NV, 2>(a, vec, s);       \
+    case 4: return launch<LPK, NV, 4>(a, vec, s);       \
+    default: return launch<LPK, NV, 8>(a, vec, s);      \
+  }
+  if (f.lpk == 32) IKV_GQ(32, 4)
+  if (f.lpk == 16) IKV_GQ(16, 4)
+  if (f.nv == 4) IKV_GQ(8, 4)
+  if (f.nv == 3) IKV_GQ(8, 3)
+  if (f.nv == 2) IKV_GQ(8, 2)
+  IKV_GQ(8, 1)
+#undef IKV_GQ
+}

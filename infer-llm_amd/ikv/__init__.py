@@ -148,6 +148,12 @@ SIGNATURES = {
         [_c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_int64, _c_void_p,
          _c_int, _c_int, _c_int, _c_float, _c_void_p],
     ),
+    "ikv_attn_decode_batch_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
+    "ikv_attn_decode_batch_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+         _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_size_t, _c_void_p],
+    ),
     # include/ikv_model.h
     "ikv_mul_mat_f32": (
         _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_void_p]),
@@ -717,6 +723,49 @@ def attn_prefill_packed_paged(q, k_pool, v_pool, tables, block_tokens: int, row_
                load().ikv_attn_prefill_packed_paged_f32(
                    _ptr(q), _ptr(k_pool), _ptr(v_pool), ctypes.byref(bt), _ptr(row_start),
                    _ptr(n_past), n_rows, _ptr(out), n_head, k_pool.shape[1], D, scale, _stream()))
+    return out
+
+
+def decode_batch_workspace(n_head: int, n_head_kv: int, head_dim: int, device="cuda"):
+    """Workspace of attn_decode_batch for these heads: any number of sequences,
+    any lengths (reusable across ordered launches)."""
+    torch = _torch()
+    nbytes = int(load().ikv_attn_decode_batch_workspace_bytes(n_head, n_head_kv, head_dim))
+    return torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device)
+
+
+def attn_decode_batch(q, k_pool, v_pool, tables, block_tokens: int, n_kv, *, k_new=None, v_new=None,
+                      out=None, scale: float = 0.0, status=None, workspace=None, stream=None):
+    """Decode attention of one new token per sequence: q [n_seq, n_head, D] over
+    the n_kv[s] keys of each sequence (0: an idle slot, a zero row); with k_new
+    and v_new [n_seq, n_head_kv, D] the last of them is taken from there and
+    appended."""
+    torch = _torch()
+    dev = q.device
+    _operands(dev, q=q, k_pool=k_pool, v_pool=v_pool, k_new=k_new, v_new=v_new, out=out,
+              workspace=workspace, tables_i=tables, n_kv_i=n_kv, status_i=status)
+    n_seq, n_head, D = q.shape
+    n_head_kv = k_pool.shape[-2]
+    _need_pools(k_pool, v_pool, n_head_kv, D)
+    bt = kv_batch(tables, block_tokens, k_pool, status)
+    if bt.n_seq != n_seq or n_kv.numel() != n_seq:
+        raise ValueError("tables and n_kv must hold an entry per row of q")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_new is not None and (k_new.shape != (n_seq, n_head_kv, D) or v_new.shape != k_new.shape):
+        raise ValueError("k_new and v_new must hold one token row per sequence")
+    if out is not None and out.shape != q.shape:
+        raise ValueError("out must be of q's shape")
+    with _on(dev, stream):
+        if out is None:
+            out = torch.empty_like(q)
+        if workspace is None:
+            workspace = decode_batch_workspace(n_head, n_head_kv, D, device=dev)
+        _check("ikv_attn_decode_batch_f32",
+               load().ikv_attn_decode_batch_f32(
+                   _ptr(q), _ptr(k_pool), _ptr(v_pool), ctypes.byref(bt), _ptr(n_kv), _ptr(k_new),
+                   _ptr(v_new), _ptr(out), n_head, n_head_kv, D, scale, _ptr(workspace),
+                   workspace.numel() * 4, _stream()))
     return out
 
 

@@ -85,3 +85,34 @@ def test_packed_prefill_refuses_bad_arguments(call):
         assert call(n_seq=(1 << 20) + 1) == -errno.EOVERFLOW
         assert call(n_seq=1 << 20, n=1, n_head=4096, n_head_kv=4096) == -errno.EOVERFLOW  # 2^32 blocks
         assert call(n_seq=0) == 0
+
+
+def _decode(q=P, kp=P, vp=P, batch="ok", n_kv=P, kn=P, vn=P, out=P, n_head=16, n_head_kv=8, dim=128,
+            ws=P, wsb=1 << 40):
+    b = _batch() if batch == "ok" else batch
+    return ikv.load().ikv_attn_decode_batch_f32(q, kp, vp, b, n_kv, kn, vn, out, n_head, n_head_kv, dim,
+                                                0.0, ws, wsb, None)
+
+
+@pytest.mark.parametrize("batch,code", BAD_BATCHES)
+def test_decode_batch_refuses_a_bad_batch(batch, code):
+    assert _decode(batch=None if batch is None else _batch(**batch)) == -code
+
+
+def test_decode_batch_refuses_bad_arguments():
+    for name in ("q", "kp", "vp", "n_kv", "kn", "vn", "out", "ws"):
+        assert _decode(**{name: None}) == -errno.EINVAL, name
+    assert _decode(n_head=12) == -errno.EINVAL  # not a multiple of n_head_kv
+    assert _decode(n_head=0) == -errno.EINVAL
+    assert _decode(dim=0) == -errno.EINVAL
+    assert _decode(dim=513) == -errno.ENOTSUP
+    assert _decode(ws=P + 4) == -errno.EINVAL
+    need = ikv.load().ikv_attn_decode_batch_workspace_bytes(16, 8, 128)
+    assert need > 0 and _decode(wsb=need - 1) == -errno.EINVAL
+    assert _decode(n_head=1 << 17, n_head_kv=1 << 17) == -errno.EOVERFLOW
+    assert _decode(batch=_batch(n_seq=0)) == 0  # nothing is launched
+
+
+def test_decode_batch_workspace_of_refused_shapes():
+    size = ikv.load().ikv_attn_decode_batch_workspace_bytes
+    assert size(12, 8, 128) == 0 and size(0, 8, 128) == 0 and size(16, 8, 0) == 0 and size(16, 8, 513) == 0
