@@ -122,6 +122,35 @@ int ikv_argmax_ws_f32(const float *logits, int64_t n, int32_t *token, int32_t *t
                       void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------
+ * Sampling of each row of logits [n_rows][n_vocab] from a given uniform number
+ * u[row] in [0, 1) (the reference samples greedily, src/sampler.cpp:42-65).
+ * With y_i = (x_i - max) / temperature and w_i = exp(y_i), tokens in the order
+ * of descending x_i, ties by index:
+ *   top_k   keeps the first top_k tokens (<= 0 or > n_vocab: all);
+ *   top_p   of them the shortest start whose mass is at least top_p times
+ *           theirs (>= 1: all; one token at least);
+ *   min_p   of it the tokens with y_i >= ln(min_p) (<= 0: all; one at least).
+ * token[row] is the first token of the order whose running mass exceeds u times
+ * the kept mass; logprob[row], if logprob is not NULL, is the logarithm of its
+ * share of the kept mass. temperature <= 0 is greedy: the first of the largest
+ * logits, logprob 0. -inf logits are never drawn. A NaN or +inf logit, all
+ * logits -inf, a NaN parameter or an infinite temperature give token -1 and a
+ * NaN logprob. u is brought into [0, 1 - 2^-24]. temperature, top_k, top_p,
+ * min_p [n_rows] may each be NULL: 1, all, 1, 0. Parameters are device memory.
+ * The masses are summed exactly in integers of 2^-45 of the heaviest token's
+ * (n_vocab = 151936; 63 bits less those of n_vocab, 52 at most), so equal calls
+ * give equal results.
+ * workspace: device memory of ikv_sample_workspace_bytes(n_rows, n_vocab)
+ * bytes, 16-byte aligned (else -EINVAL); nothing is expected in it or left in
+ * it. Launches that share it must be ordered. n_vocab up to 2^30 (-EOVERFLOW).
+ * ------------------------------------------------------------------- */
+size_t ikv_sample_workspace_bytes(int64_t n_rows, int64_t n_vocab);
+int ikv_sample_f32(const float *logits, const float *u, const float *temperature,
+                   const int32_t *top_k, const float *top_p, const float *min_p, int64_t n_rows,
+                   int64_t n_vocab, int32_t *token, float *logprob, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------
  * Host helper: the benchmarks' synthetic weights. out_host[i] =
  * std * N(0,1) sample number (offset + i) of the stream `seed`:
  * splitmix64 outputs 2j+1 and 2j+2 of the seed give the uniforms of

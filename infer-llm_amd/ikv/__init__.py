@@ -178,6 +178,12 @@ SIGNATURES = {
     "ikv_argmax_workspace_bytes": (_c_size_t, []),
     "ikv_argmax_ws_f32": (
         _c_int, [_c_void_p, _c_int64, _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "ikv_sample_workspace_bytes": (_c_size_t, [_c_int64, _c_int64]),
+    "ikv_sample_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int64,
+         _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p],
+    ),
     "ikv_synth_normal_f32": (
         _c_int, [ctypes.c_uint64, ctypes.c_uint64, _c_size_t, ctypes.c_double, _c_void_p, _c_int]),
 }
@@ -939,6 +945,44 @@ def argmax_workspace(device=None):
     torch = _torch()
     n = int(load().ikv_argmax_workspace_bytes())
     return torch.zeros(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def sample_workspace(n_rows: int, n_vocab: int, device="cuda"):
+    """Workspace of sample() for up to n_rows rows (reusable across ordered launches)."""
+    torch = _torch()
+    nbytes = int(load().ikv_sample_workspace_bytes(n_rows, n_vocab))
+    return torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device)
+
+
+def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, token=None,
+           logprob=None, workspace=None, stream=None):
+    """The next token of each row of logits [n_rows, n_vocab] from uniform numbers
+    u [n_rows], with each row's temperature (<= 0: greedy), top_k (<= 0: all),
+    top_p and min_p (device tensors [n_rows], or None). Returns (token, logprob),
+    int32 and float32 [n_rows]."""
+    torch = _torch()
+    dev = logits.device
+    _operands(dev, logits=logits, u=u, temperature=temperature, top_k_i=top_k, top_p=top_p, min_p=min_p,
+              token_i=token, logprob=logprob, workspace=workspace)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [n_rows, n_vocab]")
+    n_rows, n_vocab = logits.shape
+    for name, t in (("u", u), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
+                    ("min_p", min_p), ("token", token), ("logprob", logprob)):
+        if t is not None and t.numel() != n_rows:
+            raise ValueError(f"{name} must hold a value per row")
+    with _on(dev, stream):
+        if token is None:
+            token = torch.empty(n_rows, dtype=torch.int32, device=dev)
+        if logprob is None:
+            logprob = torch.empty(n_rows, dtype=torch.float32, device=dev)
+        if workspace is None:
+            workspace = sample_workspace(n_rows, n_vocab, device=dev)
+        _check("ikv_sample_f32",
+               load().ikv_sample_f32(_ptr(logits), _ptr(u), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                     _ptr(min_p), n_rows, n_vocab, _ptr(token), _ptr(logprob),
+                                     _ptr(workspace), workspace.numel() * 4, _stream()))
+    return token, logprob
 
 
 def synth_normal(seed: int, shape, std: float = 1.0, offset: int = 0, threads: int = 8):
