@@ -178,6 +178,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   static_assert(64 % KT == 0, "a unit stays within a block");
   __shared__ float s_m[kWaves][GQ], s_l[kWaves][GQ];
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][GQ][DP];
+  __shared__ float4 s_q[GQ][NV][LPK];  // the query rows, scaled
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = lane % LPK, grp = lane / LPK;
@@ -238,19 +239,24 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     const int heads = min(GQ, a.G - h0);
     const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
     const size_t head0 = static_cast<size_t>(p.seq) * n_head + g * a.G + h0;
-    float4 qv[GQ][NV], o[GQ][NV];
+    float4 o[GQ][NV];
     float m[GQ], sum[GQ];
 #pragma unroll
     for (int h = 0; h < GQ; ++h) {
       m[h] = -INFINITY;
       sum[h] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) o[h][n] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int h = wave; h < GQ; h += kWaves) {
       const auto r = whole_row(a.q + (head0 + min(h, heads - 1)) * a.dim);
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        qv[h][n] = ikv::scale4(a.scale_log2, load(r, 0, n));
-        o[h][n] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 x = ikv::scale4(a.scale_log2, load(r, 0, n));
+        if (grp == 0) s_q[h][n][l] = x;
       }
     }
+    __syncthreads();
     // block table entries, 64 at a time, one per lane, checked as they are read
     const int last_blk = (p.keys - 1) / pg.bt;
     int blk = p.tile * KT / pg.bt, in_blk = p.tile * KT % pg.bt, ent0 = blk, ent = 0;
@@ -277,90 +283,121 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       }
       return row;
     };
-    auto fetch = [&](const float *pool, const float *fresh, long long row, int tile, float4 (&x)[kAhead][NV]) {
-      const int rows = min(KT, p.keys - tile * KT);
+    const int cached = p.keys - (a.k_new ? 1 : 0);  // keys that are read from the pools
+    // (a tile behind the run: no memory is read)
+    auto fetch = [&](const float *pool, long long row, int tile, float4 (&x)[kAhead][NV]) {
+      const int rows = tile < last ? min(KT, cached - tile * KT) : 0;
       const auto r = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<float *>(pool + (row < 0 ? ~row : row) * stride + g * a.dim), 0,
-          ((rows - 1) * stride + a.dim) * 4, ikv::kBufWord3);
+          rows > 0 ? ((rows - 1) * stride + a.dim) * 4 : 0, ikv::kBufWord3);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int key = mine + KPW * i;
+      for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int n = 0; n < NV; ++n) x[i][n] = load(r, static_cast<unsigned>(key) * stride * 4u, n);
+        for (int n = 0; n < NV; ++n)
+          x[i][n] = load(r, static_cast<unsigned>(mine + KPW * i) * stride * 4u, n);
+    };
+    // this lane's scores of N rows of pieces with each head
+    auto scores = [&]<int N>(const float4 (&x)[N][NV], float (&s)[N][GQ]) {
+#pragma unroll
+      for (int h = 0; h < GQ; ++h) {
+        float y[N] = {};
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const float4 w = s_q[h][n][l];
+#pragma unroll
+          for (int i = 0; i < N; ++i) y[i] += ikv::dot4(w, x[i][n]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i][h] = lanes_sum<LPK>(y[i]);
       }
-      if (fresh && tile == p.tiles - 1) {  // the new token's row comes from the caller
-        const auto f = whole_row(fresh + static_cast<size_t>(p.seq) * stride + g * a.dim);
-        float *const to = const_cast<float *>(pool) + (row + rows - 1) * stride + g * a.dim;
+    };
+    auto raise = [&]<int N>(const float (&s)[N][GQ]) {  // the maxima to these scores', if need be
+      bool move = false;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (mine + KPW * i == rows - 1) {
+      for (int h = 0; h < GQ; ++h)
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
-              x[i][n] = load(f, 0, n);
-              if (row >= 0 && h0 == 0) store(to, n, x[i][n]);
-            }
-          }
+        for (int i = 0; i < N; ++i) move |= s[i][h] > m[h] + kRescale;
+      if (__builtin_amdgcn_ballot_w64(move) == 0) return;
+#pragma unroll
+      for (int h = 0; h < GQ; ++h) {
+        float top = m[h];
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, s[i][h]);
+        const float f = weight(m[h], top);
+        m[h] = top;
+        sum[h] *= f;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) o[h][n] = ikv::scale4(f, o[h][n]);
+      }
+    };
+    auto add_values = [&]<int N>(const float (&s)[N][GQ], const float4 (&x)[N][NV]) {
+#pragma unroll
+      for (int h = 0; h < GQ; ++h) {
+        const float ref = m[h] == -INFINITY ? 0.f : m[h];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float w = ikv::fast_exp2(s[i][h] - ref);
+          sum[h] += w;
+#pragma unroll
+          for (int n = 0; n < NV; ++n) o[h][n] = ikv::fma4(w, x[i][n], o[h][n]);
         }
       }
     };
 
     long long row = next_row();
-    fetch(a.k, a.k_new, row, p.tile, kr);
-    fetch(a.v, a.v_new, row, p.tile, vr);
+    fetch(a.k, row, p.tile, kr);
+    fetch(a.v, row, p.tile, vr);
     for (int t = p.tile; t < last; ++t) {
+      asm volatile("" ::: "memory");  // the query rows stay in LDS
       float s[kAhead][GQ];
+      scores(kr, s);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const bool seen = t * KT + mine + KPW * i < p.keys;
+      for (int i = 0; i < kAhead; ++i)
+        if (t * KT + mine + KPW * i >= cached) {
 #pragma unroll
-        for (int h = 0; h < GQ; ++h) {
-          float x = 0.f;
+          for (int h = 0; h < GQ; ++h) s[i][h] = -INFINITY;
+        }
+      const long long here = row;
+      row = next_row();
+      fetch(a.k, row, t + 1, kr);
+      raise(s);
+      add_values(s, vr);
+      fetch(a.v, row, t + 1, vr);
+      if (t + 1 == p.tiles && a.k_new) {
+        // the new token, by the first wave's first lanes, and its place in the pools
+        const size_t from = static_cast<size_t>(p.seq) * stride + g * a.dim;
+        float4 kn[1][NV], vn[1][NV];
 #pragma unroll
-          for (int n = 0; n < NV; ++n) x += ikv::dot4(qv[h][n], kr[i][n]);
-          s[i][h] = lanes_sum<LPK>(x);
-          if (!seen) s[i][h] = -INFINITY;
+        for (int n = 0; n < NV; ++n) {
+          kn[0][n] = load(whole_row(a.k_new + from), 0, n);
+          vn[0][n] = load(whole_row(a.v_new + from), 0, n);
+        }
+        float sn[1][GQ];
+        scores(kn, sn);
+        if (wave != 0 || grp != 0) {
+#pragma unroll
+          for (int h = 0; h < GQ; ++h) sn[0][h] = -INFINITY;
+        }
+        raise(sn);
+        // (a weight of 0 would not silence what is not finite)
+        if (wave == 0 && grp == 0) {
+          add_values(sn, vn);
+          if (here >= 0 && h0 == 0) {
+            const long long to = (here + cached - t * KT) * stride + g * a.dim;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+              store(a.k + to, n, kn[0][n]);
+              store(a.v + to, n, vn[0][n]);
+            }
+          }
         }
       }
-      const bool more = t + 1 < last;
-      if (more) {
-        row = next_row();
-        fetch(a.k, a.k_new, row, t + 1, kr);
-      }
-      bool move = false;
-#pragma unroll
-      for (int h = 0; h < GQ; ++h)
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) move |= s[i][h] > m[h] + kRescale;
-      if (__builtin_amdgcn_ballot_w64(move) != 0) {
-#pragma unroll
-        for (int h = 0; h < GQ; ++h) {
-          float top = m[h];
-#pragma unroll
-          for (int i = 0; i < kAhead; ++i) top = fmaxf(top, s[i][h]);
-          const float f = weight(m[h], top);
-          m[h] = top;
-          sum[h] *= f;
-#pragma unroll
-          for (int n = 0; n < NV; ++n) o[h][n] = ikv::scale4(f, o[h][n]);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < GQ; ++h) {
-        const float ref = m[h] == -INFINITY ? 0.f : m[h];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const float w = ikv::fast_exp2(s[i][h] - ref);
-          sum[h] += w;
-#pragma unroll
-          for (int n = 0; n < NV; ++n) o[h][n] = ikv::fma4(w, vr[i][n], o[h][n]);
-        }
-      }
-      if (more) fetch(a.v, a.v_new, row, t + 1, vr);
     }
 
     // the lane groups and the waves meet
 #pragma unroll
     for (int h = 0; h < GQ; ++h) {
+      __builtin_amdgcn_sched_barrier(0);
       const float top = across_keys<LPK>(m[h], [](float x, float y) { return fmaxf(x, y); });
       const float f = weight(m[h], top);
       auto add = [](float x, float y) { return x + y; };
