@@ -137,12 +137,13 @@ int ikv_argmax_ws_f32(const float *logits, int64_t n, int32_t *token, int32_t *t
  * logits -inf, a NaN parameter or an infinite temperature give token -1 and a
  * NaN logprob. u is brought into [0, 1 - 2^-24]. temperature, top_k, top_p,
  * min_p [n_rows] may each be NULL: 1, all, 1, 0. Parameters are device memory.
- * The masses are summed exactly in integers of 2^-45 of the heaviest token's
- * (n_vocab = 151936; 63 bits less those of n_vocab, 52 at most), so equal calls
+ * The masses are summed exactly in integers of 2^-44 of the heaviest token's
+ * (n_vocab = 151936; 62 bits less those of n_vocab, 51 at most), so equal calls
  * give equal results.
  * workspace: device memory of ikv_sample_workspace_bytes(n_rows, n_vocab)
  * bytes, 16-byte aligned (else -EINVAL); nothing is expected in it or left in
- * it. Launches that share it must be ordered. n_vocab up to 2^30 (-EOVERFLOW).
+ * it, and it is enough for fewer rows. Launches that share it must be ordered.
+ * -EOVERFLOW: n_vocab past 2^30 or n_rows past 2^21.
  * ------------------------------------------------------------------- */
 size_t ikv_sample_workspace_bytes(int64_t n_rows, int64_t n_vocab);
 int ikv_sample_f32(const float *logits, const float *u, const float *temperature,

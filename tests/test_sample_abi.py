@@ -18,7 +18,7 @@ def test_sample_refuses_bad_arguments():
     assert _sample(vocab=0) == -errno.EINVAL
     assert _sample(vocab=-5) == -errno.EINVAL
     assert _sample(vocab=(1 << 30) + 1) == -errno.EOVERFLOW
-    assert _sample(rows=1 << 31) == -errno.EOVERFLOW
+    assert _sample(rows=(1 << 21) + 1) == -errno.EOVERFLOW
     assert _sample(ws=P + 4) == -errno.EINVAL
     need = ikv.load().ikv_sample_workspace_bytes(3, 1000)
     assert need > 0 and _sample(wsb=need - 1) == -errno.EINVAL
@@ -28,3 +28,10 @@ def test_sample_refuses_bad_arguments():
 def test_sample_workspace_of_no_rows():
     size = ikv.load().ikv_sample_workspace_bytes
     assert size(0, 10) == 0 and size(10, 0) == 0 and size(-1, 10) == 0
+
+
+def test_sample_workspace_is_enough_for_fewer_rows():
+    size = ikv.load().ikv_sample_workspace_bytes
+    for vocab in (10, 16384, 16385, 151936):
+        sizes = [size(rows, vocab) for rows in range(1, 1200)]
+        assert sizes == sorted(sizes)
