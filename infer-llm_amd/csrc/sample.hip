@@ -28,7 +28,7 @@
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kBits = 11, kBins = 1 << kBits;  // of a round
 
 struct Args {
@@ -98,7 +98,11 @@ __device__ unsigned long long block_prefix(unsigned long long v, unsigned long l
   __syncthreads();
   if (lane == 63) s_wave[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) v += s_wave[w];
+#pragma unroll
+  for (int w = 0; w < kThreads / 64 - 1; ++w) {  // (all read at once)
+    const unsigned long long y = s_wave[w];
+    if (w < wave) v += y;
+  }
   return v;
 }
 
@@ -320,8 +324,24 @@ struct Window {
   __device__ int bin(float x) const { return static_cast<int>(fminf((top - x) * scale, kBins - 1.0f)); }
 };
 
-constexpr int kList = 4096;  // tokens of a row that are looked at one by one
+constexpr int kList = 2048;  // tokens of a row that are looked at one by one
 constexpr int kMaxChunks = 64;
+
+// The bins that hold the borders (top_k's, top_p's, min_p's, the draw's; hi < lo:
+// none). A border is known to a bin's mass before the ones ahead of it are looked
+// at, so a range of bins may have to be: nearly always one.
+struct Ranges {
+  int lo[4], hi[4];
+  unsigned long long total, before_m;  // all mass, and that before min_p's bins
+  bool has_k;
+
+  __device__ bool holds(int b) const {
+    bool in = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in |= b >= lo[j] && b <= hi[j];
+    return in;
+  }
+};
 
 // What a row's workgroups hand on: the largest and smallest finite logit of
 // each chunk and the first index of the largest, the bins, the list.
@@ -333,8 +353,9 @@ struct RowSpace {
   unsigned long long mass[kBins];
   unsigned long long list[kList];
   unsigned count[kBins];
-  unsigned listed, arrived;
+  unsigned listed, binned, arrived;
   Chunk chunk[kMaxChunks];
+  Ranges ranges;
 };
 
 struct Lists {
@@ -342,10 +363,15 @@ struct Lists {
   unsigned long long list[kList];      // (order, index) of a token
   unsigned count[kBins + 1];
   unsigned long long wave[kThreads / 64];
-  unsigned long long kept_k, kept_p, kept_m, drawn;
+  unsigned long long kept_k, kept_p, kept_m;
+  int spot[5];
+  int n, last;
+};
+
+struct Extremes {
   float top[kThreads / 64], low[kThreads / 64];
   int at[kThreads / 64];
-  int bad, n, last;
+  int bad;
 };
 
 union Space {
@@ -353,30 +379,57 @@ union Space {
   Lists l;
 };
 
-// f(x, index) over x[begin, end) by the workgroup, several loads in flight.
-template <class F>
-__device__ __forceinline__ void each_token(const float *x, int begin, int end, F &&f) {
-  constexpr int kAhead = 4;
-  int i = begin + threadIdx.x;
-  for (; i + (kAhead - 1) * kThreads < end; i += kAhead * kThreads) {
-    float v[kAhead];
+// The tokens of a workgroup: x[begin, end), read anew at each pass, eight loads of
+// a thread in flight.
+struct Chunked {
+  const float *x;
+  int begin, end;
+  template <class F>
+  __device__ __forceinline__ void each(F &&f) const {  // f(logit, index)
+    constexpr int kAhead = 8;
+    for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kAhead * kThreads) {
+      float v[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) v[j] = x[i + j * kThreads];
+      for (int j = 0; j < kAhead; ++j) v[j] = i + j * kThreads < end ? x[i + j * kThreads] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) f(v[j], i + j * kThreads);
+      for (int j = 0; j < kAhead; ++j)
+        if (i + j * kThreads < end) f(v[j], i + j * kThreads);
+    }
   }
-  for (; i < end; i += kThreads) f(x[i], i);
-}
+};
 
-// The largest logit of x[begin, end), its first index, the smallest finite one.
-__device__ Chunk extremes(const float *x, int begin, int end, Lists &l) {
+// Up to N * kThreads tokens, kept in registers.
+template <int N>
+struct Held {
+  float v[N];
+  int n;
+  __device__ Held(const float *x, int n) : n(n) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      v[j] = i < n ? x[i] : 0.0f;
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F &&f) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      if (i < n) f(v[j], i);
+    }
+  }
+};
+
+// The largest logit, its first index, the smallest finite one.
+template <class Tokens>
+__device__ Chunk extremes(const Tokens &tokens, Extremes &l) {
   Chunk c{-INFINITY, INFINITY, INT_MAX, 0};
   auto take = [&](float v, int i) {
     c.bad |= !(v < INFINITY);
     if (v > c.top) c.top = v, c.at = i;
     if (v > -INFINITY) c.low = fminf(c.low, v);
   };
-  each_token(x, begin, end, take);
+  tokens.each(take);
   const float top = ikv::wave_max(c.top);
   int at = c.top == top ? c.at : INT_MAX;
   for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
@@ -398,15 +451,16 @@ __device__ Chunk extremes(const float *x, int begin, int end, Lists &l) {
   return c;
 }
 
-// Masses (and, for top_k, counts) of the tokens of x[begin, end) into l's bins.
-// Tokens that weigh nothing are in none: they come last and move no border.
-__device__ void fill_bins(const Row &row, const Window &win, bool counts, int begin, int end, Lists &l) {
+// Masses (and, for top_k, counts) of the tokens into l's bins. Tokens that weigh
+// nothing are in none: they come last and move no border.
+template <class Tokens>
+__device__ void fill_bins(const Row &row, const Window &win, bool counts, const Tokens &tokens, Lists &l) {
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     l.mass[b] = 0;
     l.count[b] = 0;
   }
   __syncthreads();
-  each_token(row.x, begin, end, [&](float x, int) {
+  tokens.each([&](float x, int) {
     const unsigned long long w = row.weight(x);
     if (w == 0) return;
     const int b = win.bin(x);
@@ -416,102 +470,89 @@ __device__ void fill_bins(const Row &row, const Window &win, bool counts, int be
   __syncthreads();
 }
 
-// l's bins to what comes before each.
-__device__ void sum_bins(Lists &l) {
+// l's bins to what comes before each, and the bins of the borders.
+__device__ Ranges find_ranges(const Row &row, const Window &win, const Cuts &c, Lists &l) {
   constexpr int kPer = kBins / kThreads;
-  unsigned long long m[kPer], ms = 0;
-  unsigned c[kPer], cs = 0;
+  unsigned long long m[kPer + 1], sum_m = 0;  // before this thread's bins, and behind the last
+  unsigned n[kPer + 1], sum_n = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    ms += m[j] = l.mass[threadIdx.x * kPer + j];
-    cs += c[j] = l.count[threadIdx.x * kPer + j];
+    sum_m += m[j + 1] = l.mass[threadIdx.x * kPer + j];
+    sum_n += n[j + 1] = l.count[threadIdx.x * kPer + j];
   }
-  unsigned long long bm = block_prefix(ms, l.wave) - ms;
-  unsigned bc = static_cast<unsigned>(block_prefix(cs, l.wave)) - cs;
+  m[0] = block_prefix(sum_m, l.wave) - sum_m;
+  const bool counts = c.k > 0 && c.k < row.n;
+  n[0] = counts ? static_cast<unsigned>(block_prefix(sum_n, l.wave)) - sum_n : 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    l.mass[threadIdx.x * kPer + j] = bm;
-    l.count[threadIdx.x * kPer + j] = bc;
-    bm += m[j];
-    bc += c[j];
+    l.mass[threadIdx.x * kPer + j] = m[j];
+    l.count[threadIdx.x * kPer + j] = n[j];
+    m[j + 1] += m[j];
+    n[j + 1] += n[j];
   }
   if (threadIdx.x == kThreads - 1) {
-    l.mass[kBins] = bm;
-    l.count[kBins] = bc;
+    l.mass[kBins] = m[kPer];
+    l.count[kBins] = n[kPer];
   }
+  if (threadIdx.x < 5) l.spot[threadIdx.x] = kBins - 1;
   __syncthreads();
+  // the bin in which a running mass or count reaches a border, to l.spot
+  auto find = [&](const auto *before, auto border, int to) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (before[j] < border && before[j + 1] >= border) l.spot[to] = threadIdx.x * kPer + j;
+  };
+  Ranges r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.lo[j] = 1, r.hi[j] = 0;
+  r.total = l.mass[kBins];
+  unsigned long long least = r.total, most = r.total;  // of the kept mass
+  r.has_k = counts && static_cast<unsigned>(c.k) < l.count[kBins];
+  if (r.has_k) {
+    find(n, static_cast<unsigned>(c.k), 0);
+    __syncthreads();
+    r.lo[0] = r.hi[0] = l.spot[0];
+    least = l.mass[r.lo[0]];
+    most = l.mass[r.lo[0] + 1];
+  }
+  if (c.p < 1.0f) {
+    find(m, share_of(least, c.p), 1);
+    find(m, share_of(most, c.p), 2);
+    __syncthreads();
+    r.lo[1] = l.spot[1];
+    r.hi[1] = l.spot[2];
+    least = min(least, l.mass[r.lo[1]]);
+    most = min(most, l.mass[r.hi[1] + 1]);
+  }
+  r.before_m = 0;
+  if (c.low > 0.0f) {
+    const double move = static_cast<double>(c.t) * c.floor, at = row.top + move;
+    const double slack = 1e-12 * (fabs(static_cast<double>(row.top)) + fabs(move));
+    auto edge = [&](double x, float way) {
+      const float f = static_cast<float>(x);
+      return f < INFINITY && f > -INFINITY ? nextafterf(f, way) : f;
+    };
+    r.lo[2] = max(win.bin(edge(at + slack, INFINITY)), 0);
+    r.hi[2] = max(win.bin(edge(at - slack, -INFINITY)), 0);
+    r.before_m = l.mass[r.lo[2]];
+    least = min(least, r.before_m);
+    most = min(most, l.mass[r.hi[2] + 1]);
+  }
+  const unsigned long long heaviest = row.weight(row.top);
+  find(m, drawn_of(max(least, heaviest), c.u), 3);
+  find(m, drawn_of(max(most, heaviest), c.u), 4);
+  __syncthreads();
+  r.lo[3] = l.spot[3];
+  r.hi[3] = l.spot[4];
+  return r;
 }
 
-// The bins that hold the borders. A border is known to a bin's mass before the
-// ones ahead of it are looked at, so a range of bins may have to be: nearly
-// always one.
-struct Ranges {
-  int lo[4], hi[4];  // top_k, top_p, min_p, the draw; hi < lo: none
-  unsigned long long total, before_m;
-  bool has_k;
-
-  template <class T>
-  __device__ static int reaching(const T *before, T border) {  // the first bin at whose end it is reached
-    int lo = 0, hi = kBins - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (before[mid + 1] >= border)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    return lo;
-  }
-
-  __device__ Ranges(const Row &row, const Window &win, const Cuts &c, const Lists &l) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) lo[j] = 1, hi[j] = 0;
-    total = l.mass[kBins];
-    unsigned long long least = total, most = total;  // of the kept mass
-    has_k = c.k > 0 && static_cast<unsigned>(c.k) < l.count[kBins];
-    if (has_k) {
-      lo[0] = hi[0] = reaching(l.count, static_cast<unsigned>(c.k));
-      least = l.mass[lo[0]];
-      most = l.mass[lo[0] + 1];
-    }
-    if (c.p < 1.0f) {
-      lo[1] = reaching(l.mass, share_of(least, c.p));
-      hi[1] = reaching(l.mass, share_of(most, c.p));
-      least = min(least, l.mass[lo[1]]);
-      most = min(most, l.mass[hi[1] + 1]);
-    }
-    before_m = 0;
-    if (c.low > 0.0f) {
-      const double move = static_cast<double>(c.t) * c.floor, at = row.top + move;
-      const double slack = 1e-12 * (fabs(static_cast<double>(row.top)) + fabs(move));
-      auto edge = [&](double x, float way) {
-        const float f = static_cast<float>(x);
-        return f < INFINITY && f > -INFINITY ? nextafterf(f, way) : f;
-      };
-      lo[2] = max(win.bin(edge(at + slack, INFINITY)), 0);
-      hi[2] = max(win.bin(edge(at - slack, -INFINITY)), 0);
-      before_m = l.mass[lo[2]];
-      least = min(least, before_m);
-      most = min(most, l.mass[hi[2] + 1]);
-    }
-    const unsigned long long heaviest = row.weight(row.top);
-    lo[3] = reaching(l.mass, drawn_of(max(least, heaviest), c.u));
-    hi[3] = reaching(l.mass, drawn_of(max(most, heaviest), c.u));
-  }
-
-  __device__ bool holds(int b) const {
-    bool in = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in |= b >= lo[j] && b <= hi[j];
-    return in;
-  }
-};
-
 // The tokens of those bins into l's list (l.n may pass kList: then not all).
-__device__ void gather(const Row &row, const Window &win, const Ranges &rg, int begin, int end, Lists &l) {
+template <class Tokens>
+__device__ void gather(const Row &row, const Window &win, const Ranges &rg, const Tokens &tokens, Lists &l) {
   if (threadIdx.x == 0) l.n = 0;
   __syncthreads();
-  each_token(row.x, begin, end, [&](float x, int i) {
+  tokens.each([&](float x, int i) {
     if (!rg.holds(win.bin(x)) || row.weight(x) == 0) return;
     const int at = atomicAdd(&l.n, 1);
     if (at < kList) l.list[at] = static_cast<unsigned long long>(order_of(x)) << 32 | static_cast<unsigned>(i);
@@ -519,20 +560,26 @@ __device__ void gather(const Row &row, const Window &win, const Ranges &rg, int 
   __syncthreads();
 }
 
-// The token, from the bins' sums and the whole list (n <= kList tokens of it).
-__device__ void resolve(const Args &a, int r, const Row &row, const Window &win, const Cuts &c, const Ranges &rg,
-                        int n, Lists &l) {
+// l's list by order, then index; no two entries are equal.
+__device__ void sort_list(int n, Lists &l) {
   const int tid = threadIdx.x;
-  int size = 64;
+  if (n <= kThreads) {  // each entry's place is the number of smaller ones
+    const unsigned long long mine = tid < n ? l.list[tid] : 0;
+    int at = 0;
+    if ((tid & ~63) < n) {
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) at += l.list[i] < mine;
+    }
+    __syncthreads();
+    if (tid < n) l.list[at] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 2 * kThreads;  // bitonic
   while (size < n) size *= 2;
   for (int i = n + tid; i < size; i += kThreads) l.list[i] = ~0ull;
-  if (tid == 0) {
-    l.kept_k = rg.total;
-    l.kept_p = l.drawn = ~0ull;
-    l.kept_m = rg.before_m;
-  }
   __syncthreads();
-  for (int k = 2; k <= size; k *= 2) {  // bitonic: by order, then index
+  for (int k = 2; k <= size; k *= 2) {
     for (int j = k / 2; j > 0; j /= 2) {
       for (int p = tid; p < size / 2; p += kThreads) {
         const int i = 2 * p - (p & (j - 1)), o = i + j;
@@ -545,35 +592,50 @@ __device__ void resolve(const Args &a, int r, const Row &row, const Window &win,
       __syncthreads();
     }
   }
+}
+
+// The token, from the bins' sums and the whole list (n <= kList tokens of it).
+__device__ void resolve(const Args &a, int r, const Row &row, const Window &win, const Cuts &c, const Ranges &rg,
+                        int n, Lists &l) {
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    l.kept_k = rg.total;
+    l.kept_p = ~0ull;
+    l.kept_m = rg.before_m;
+  }
+  sort_list(n, l);
   // running masses and counts: a bin's tokens are all in the list, one behind
   // the other, so a token's are its bin's and those of the list since the bin's
-  // first one
+  // first one. Each border has one token: no atomics (64-bit ones of a few
+  // hundred lanes on one address took 20 us).
   constexpr int kPer = kList / kThreads;
-  unsigned long long m[kPer], own = 0;
+  unsigned long long w[kPer], m[kPer], own = 0;  // a token's weight, the running mass with it
   float x[kPer];
   int bin[kPer];
+  auto logit = [&](int i) {
+    const unsigned o = static_cast<unsigned>(l.list[i] >> 32);
+    return __uint_as_float((o & 0x80000000u) ? o : ~o & 0x7fffffffu);
+  };
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int i = tid * kPer + j;
-    const unsigned o = i < n ? static_cast<unsigned>(l.list[i] >> 32) : 0u;
-    x[j] = __uint_as_float((o & 0x80000000u) ? o : ~o & 0x7fffffffu);
-    bin[j] = i < n ? win.bin(x[j]) : -1;
-    own += m[j] = i < n ? row.weight(x[j]) : 0;
+    w[j] = 0;
+    if (i < n) {
+      x[j] = logit(i);
+      bin[j] = win.bin(x[j]);
+      w[j] = row.weight(x[j]);
+    }
+    own += w[j];
   }
   unsigned long long run = block_prefix(own, l.wave) - own;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int i = tid * kPer + j;
-    bool first = i < n && i == 0;
-    if (i < n && i > 0) {
-      const unsigned o = static_cast<unsigned>(l.list[i - 1] >> 32);
-      first = win.bin(__uint_as_float((o & 0x80000000u) ? o : ~o & 0x7fffffffu)) != bin[j];
-    }
-    if (first) {  // (one token of the bin: nobody else touches its sums)
+    if (i < n && (i == 0 || win.bin(logit(i - 1)) != bin[j])) {  // the bin's first: nobody else's
       l.mass[bin[j]] -= run;
       l.count[bin[j]] -= static_cast<unsigned>(i);
     }
-    run += m[j];
+    run += w[j];
     m[j] = run;
   }
   __syncthreads();
@@ -583,7 +645,8 @@ __device__ void resolve(const Args &a, int r, const Row &row, const Window &win,
     if (i >= n) continue;
     m[j] += l.mass[bin[j]];
     if (rg.has_k && bin[j] == rg.lo[0] && l.count[bin[j]] + i + 1 == static_cast<unsigned>(c.k)) l.kept_k = m[j];
-    if (c.low > 0.0f && c.passes(x[j], row.top)) atomicMax(&l.kept_m, m[j]);
+    if (c.low > 0.0f && c.passes(x[j], row.top) && (i + 1 == n || !c.passes(logit(i + 1), row.top)))
+      l.kept_m = max(rg.before_m, m[j]);
   }
   __syncthreads();
   unsigned long long kept = l.kept_k;
@@ -591,7 +654,7 @@ __device__ void resolve(const Args &a, int r, const Row &row, const Window &win,
     const unsigned long long need = share_of(kept, c.p);
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (tid * kPer + j < n && m[j] >= need) atomicMin(&l.kept_p, m[j]);
+      if (m[j] >= need && m[j] - w[j] < need && w[j] != 0) l.kept_p = m[j];
     __syncthreads();
     kept = min(kept, l.kept_p);
   }
@@ -599,13 +662,8 @@ __device__ void resolve(const Args &a, int r, const Row &row, const Window &win,
   kept = max(kept, row.weight(row.top));
   const unsigned long long target = drawn_of(kept, c.u);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j)
-    if (tid * kPer + j < n && m[j] >= target) atomicMin(&l.drawn, m[j]);
-  __syncthreads();
-  const unsigned long long drawn = l.drawn;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j)  // (every token of the list weighs something: one has this running mass)
-    if (tid * kPer + j < n && m[j] == drawn)
+  for (int j = 0; j < kPer; ++j)  // (a token that is not in the list weighs nothing)
+    if (m[j] >= target && m[j] - w[j] < target && w[j] != 0)
       answer(a, r, static_cast<int>(static_cast<unsigned>(l.list[tid * kPer + j])), x[j], row, c, kept);
 }
 
@@ -631,18 +689,16 @@ __device__ bool settled(const Args &a, int r, const Cuts &c, const Chunk &e, boo
 }
 
 // A workgroup a row.
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
-  __shared__ Space s;
-  const int r = blockIdx.x;
-  const Cuts c(a, r);
-  const Chunk e = extremes(a.logits + static_cast<size_t>(r) * a.n, 0, a.n, s.l);
+template <class Tokens>
+__device__ void sample_row(const Args &a, int r, const Cuts &c, const Tokens &tokens, Space &s) {
+  __shared__ Extremes x;
+  const Chunk e = extremes(tokens, x);
   if (settled(a, r, c, e, threadIdx.x == 0)) return;
   const Row row = row_of(a, r, c, e.top);
   const Window win(row, e.low, c.t);
-  fill_bins(row, win, c.k > 0 && c.k < a.n, 0, a.n, s.l);
-  sum_bins(s.l);
-  const Ranges rg(row, win, c, s.l);
-  gather(row, win, rg, 0, a.n, s.l);
+  fill_bins(row, win, c.k > 0 && c.k < a.n, tokens, s.l);
+  const Ranges rg = find_ranges(row, win, c, s.l);
+  gather(row, win, rg, tokens, s.l);
   const int n = s.l.n;
   if (n <= kList) {
     resolve(a, r, row, win, c, rg, n, s.l);
@@ -652,26 +708,39 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
   }
 }
 
+constexpr int kHeld = 16;  // tokens of a thread that are kept in registers
+
+__global__ __launch_bounds__(kThreads) void sample_held_kernel(Args a) {
+  __shared__ Space s;
+  const int r = blockIdx.x;
+  const Held<kHeld> tokens(a.logits + static_cast<size_t>(r) * a.n, a.n);
+  sample_row(a, r, Cuts(a, r), tokens, s);
+}
+
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
+  __shared__ Space s;
+  const int r = blockIdx.x;
+  sample_row(a, r, Cuts(a, r), Chunked{a.logits + static_cast<size_t>(r) * a.n, 0, a.n}, s);
+}
+
 // Several workgroups a row, in three launches. The first: each chunk's extremes,
 // and the row's sums cleared.
-__device__ __forceinline__ void chunk_of(const Args &a, int &begin, int &end) {
+__device__ __forceinline__ Chunked chunk_of(const Args &a) {
   const int per = (a.n + gridDim.x - 1) / gridDim.x;
-  begin = min(a.n, static_cast<int>(blockIdx.x) * per);
-  end = min(a.n, begin + per);
+  const int begin = min(a.n, static_cast<int>(blockIdx.x) * per);
+  return Chunked{a.logits + static_cast<size_t>(blockIdx.y) * a.n, begin, min(a.n, begin + per)};
 }
 
 __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(Args a, RowSpace *rows) {
-  __shared__ Lists l;
+  __shared__ Extremes l;
   const int r = blockIdx.y;
   RowSpace &w = rows[r];
   for (int b = blockIdx.x * kThreads + threadIdx.x; b < kBins; b += gridDim.x * kThreads) {
     w.mass[b] = 0;
     w.count[b] = 0;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) w.listed = w.arrived = 0;
-  int begin, end;
-  chunk_of(a, begin, end);
-  const Chunk e = extremes(a.logits + static_cast<size_t>(r) * a.n, begin, end, l);
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.listed = w.binned = w.arrived = 0;
+  const Chunk e = extremes(chunk_of(a), l);
   if (threadIdx.x == 0) w.chunk[blockIdx.x] = e;
 }
 
@@ -687,29 +756,57 @@ __device__ Chunk row_extremes(const RowSpace &w, int chunks) {
   return e;
 }
 
-// The second: the bins.
+// Whether this workgroup is the last of its row's to come here; what the others
+// stored (agent scope) before they came is then there.
+__device__ bool last_of_row(unsigned *counter, int *s_last) {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0);  // this thread's stores and atomics have completed
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *s_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  return *s_last != 0;
+}
+
+template <class T>
+__device__ __forceinline__ T load_agent(const T *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The second: the bins, and by the workgroup that comes last the borders'.
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(Args a, RowSpace *rows) {
   __shared__ Lists l;
   const int r = blockIdx.y;
   RowSpace &w = rows[r];
   const Cuts c(a, r);
   const Chunk e = row_extremes(w, gridDim.x);
-  if (settled(a, r, c, e, false)) return;
+  if (settled(a, r, c, e, blockIdx.x == 0 && threadIdx.x == 0)) return;
   const Row row = row_of(a, r, c, e.top);
   const Window win(row, e.low, c.t);
-  int begin, end;
-  chunk_of(a, begin, end);
   const bool counts = c.k > 0 && c.k < a.n;
-  fill_bins(row, win, counts, begin, end, l);
+  fill_bins(row, win, counts, chunk_of(a), l);
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     if (l.mass[b] == 0) continue;
     atomicAdd(&w.mass[b], l.mass[b]);
     if (counts) atomicAdd(&w.count[b], l.count[b]);
   }
+  if (!last_of_row(&w.binned, &l.last)) return;
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    l.mass[b] = load_agent(&w.mass[b]);
+    l.count[b] = counts ? load_agent(&w.count[b]) : 0;
+  }
+  __syncthreads();
+  const Ranges rg = find_ranges(row, win, c, l);
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    w.mass[b] = l.mass[b];
+    w.count[b] = l.count[b];
+  }
+  if (threadIdx.x == 0) w.ranges = rg;
 }
 
-// The third: the borders' bins, their tokens, and, by the workgroup that comes
-// last, the token.
+// The third: the tokens of those bins, and by the workgroup that comes last the
+// answer.
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Args a, RowSpace *rows) {
   __shared__ Space s;
   Lists &l = s.l;
@@ -717,38 +814,25 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Args a, RowSpace 
   RowSpace &w = rows[r];
   const Cuts c(a, r);
   const Chunk e = row_extremes(w, gridDim.x);
-  if (settled(a, r, c, e, blockIdx.x == 0 && tid == 0)) return;
+  if (settled(a, r, c, e, false)) return;
   const Row row = row_of(a, r, c, e.top);
   const Window win(row, e.low, c.t);
-  for (int b = tid; b < kBins; b += kThreads) {
-    l.mass[b] = w.mass[b];
-    l.count[b] = w.count[b];
-  }
-  __syncthreads();
-  sum_bins(l);
-  const Ranges rg(row, win, c, l);
-  int begin, end;
-  chunk_of(a, begin, end);
-  gather(row, win, rg, begin, end, l);
-  if (tid == 0) l.last = static_cast<int>(atomicAdd(&w.listed, static_cast<unsigned>(l.n)));
+  const Ranges rg = w.ranges;
+  gather(row, win, rg, chunk_of(a), l);
+  if (tid == 0 && l.n > 0) l.last = static_cast<int>(atomicAdd(&w.listed, static_cast<unsigned>(l.n)));
   __syncthreads();
   const unsigned first = static_cast<unsigned>(l.last);
   for (int i = tid; i < min(l.n, kList); i += kThreads)
     if (first + i < kList)
       __hip_atomic_store(&w.list[first + i], l.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // the entries' stores have completed before the arrival
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_waitcnt(0);
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __syncthreads();
-  if (tid == 0)
-    l.last = __hip_atomic_fetch_add(&w.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-  __syncthreads();
-  if (!l.last) return;
-  const unsigned n = __hip_atomic_load(&w.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of_row(&w.arrived, &l.last)) return;
+  const unsigned n = load_agent(&w.listed);
   if (n <= kList) {
-    for (unsigned i = tid; i < n; i += kThreads)
-      l.list[i] = __hip_atomic_load(&w.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (unsigned i = tid; i < n; i += kThreads) l.list[i] = load_agent(&w.list[i]);
+    for (int b = tid; b < kBins; b += kThreads) {
+      l.mass[b] = w.mass[b];
+      l.count[b] = w.count[b];
+    }
     __syncthreads();
     resolve(a, r, row, win, c, rg, static_cast<int>(n), l);
   } else {
@@ -759,7 +843,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Args a, RowSpace 
 
 // Workgroups of a row: one up to kRowTokens tokens, else as many as bring all
 // rows to kGroups, of 2048 tokens at least (one where there are many rows).
-constexpr int kRowTokens = 16384, kGroups = 1024;
+constexpr int kRowTokens = 16384, kGroups = 512;
 int chunks_of(int64_t n_rows, int64_t n_vocab) {
   if (n_vocab <= kRowTokens) return 1;
   const int64_t most = std::max<int64_t>(1, kGroups / n_rows);
@@ -790,7 +874,10 @@ extern "C" int ikv_sample_f32(const float *logits, const float *u, const float *
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int chunks = chunks_of(n_rows, n_vocab);
   if (chunks == 1) {
-    sample_row_kernel<<<static_cast<unsigned>(n_rows), kThreads, 0, s>>>(a);
+    if (n_vocab <= kHeld * kThreads)
+      sample_held_kernel<<<static_cast<unsigned>(n_rows), kThreads, 0, s>>>(a);
+    else
+      sample_row_kernel<<<static_cast<unsigned>(n_rows), kThreads, 0, s>>>(a);
   } else {
     auto *rows = static_cast<RowSpace *>(workspace);
     const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(n_rows));
