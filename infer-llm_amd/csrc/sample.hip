@@ -44,7 +44,7 @@ struct Args {
 
 // 2^f for |f| <= 1/2 by its Taylor series, f ln2 <= 0.3466: the term left out
 // is below 0.3466^13 / 13! = 2^-52.4.
-__device__ __forceinline__ double exp2_series(double f) {
+__device__ double exp2_series(double f) {
   const double z = f * 0.69314718055994530942;
   double r = 1.0 / 479001600.0;
   r = fma(r, z, 1.0 / 39916800.0);
@@ -61,23 +61,49 @@ __device__ __forceinline__ double exp2_series(double f) {
   return fma(r, z, 1.0);
 }
 
+constexpr int kPowers = 64;
+
+// 2^(j / 64) for j < 64, in LDS: 2^t is one of them, a power of two and 2^g with
+// |g| <= 1/128, whose series needs five terms.
+__device__ void fill_powers(double *powers) {
+  const int j = threadIdx.x;
+  if (j < kPowers / 2)
+    powers[j] = exp2_series(j * (1.0 / kPowers));
+  else if (j < kPowers)
+    powers[j] = 2.0 * exp2_series(j * (1.0 / kPowers) - 1.0);
+}
+
 // A row as its workgroup sees it.
 struct Row {
   const float *x;
   int n;
-  float top;         // the largest logit
-  double per_t;      // log2(e) / T
-  double shift;      // S
+  float top;     // the largest logit
+  double per_t;  // log2(e) / T
+  double shift;  // S
+  const double *powers;
 
-  // w in multiples of 2^-S; the largest logit's is 2^S
-  __device__ unsigned long long weight(float v) const {
+  // w in multiples of 2^-S; the largest logit's is 2^S. The same bits wherever it
+  // is inlined (the sums of one launch and the tokens of another have to agree),
+  // so nothing is left to contraction. Without branches: the tokens of a thread
+  // go through it side by side. The series' rest is below (ln2 / 128)^6 / 6! =
+  // 2^-54.6.
+  __device__ __forceinline__ unsigned long long weight(float v) const {
+#pragma clang fp contract(off)
     const double t = (static_cast<double>(v) - static_cast<double>(top)) * per_t;
-    if (!(t > -(shift + 2.0))) return 0;
-    const double whole = rint(t);
-    // times 2^(whole + S), rounded to an integer: the bits of the sum with 2^52
-    const long long power = static_cast<long long>(static_cast<int>(whole + shift) + 1023) << 52;
-    const double sum = fma(exp2_series(t - whole), __builtin_bit_cast(double, power), 0x1p52);
-    return __builtin_bit_cast(unsigned long long, sum) & 0xfffffffffffffull;
+    const double moved = t + 0x1.8p46;  // a multiple of 1/64, its count in the low bits
+    const double g = t - (moved - 0x1.8p46);
+    const int k = static_cast<int>(__builtin_bit_cast(long long, moved));
+    double r = fma(g, 1.3333558146428443e-3, 9.6181291076284772e-3);
+    r = fma(r, g, 5.5504108664821580e-2);
+    r = fma(r, g, 2.4022650695910072e-1);
+    r = fma(r, g, 6.9314718055994531e-1);
+    r = fma(r, g, 1.0);
+    // times 2^(k / 64 + S), rounded to an integer: the bits of the sum with 2^52
+    uint2 power = __builtin_bit_cast(uint2, powers[k & (kPowers - 1)]);
+    power.y += static_cast<unsigned>((k >> 6) + static_cast<int>(shift)) << 20;
+    const uint2 sum = __builtin_bit_cast(uint2, fma(r, __builtin_bit_cast(double, power), 0x1p52));
+    const unsigned long long w = static_cast<unsigned long long>(sum.y & 0xfffffu) << 32 | sum.x;
+    return t > -(shift + 2.0) ? w : 0;
   }
 };
 
@@ -384,16 +410,20 @@ union Space {
 struct Chunked {
   const float *x;
   int begin, end;
-  template <class F>
-  __device__ __forceinline__ void each(F &&f) const {  // f(logit, index)
+  // f(logit, index, g(logit)): g of eight tokens side by side, then f of each
+  template <class G, class F>
+  __device__ __forceinline__ void each(G &&g, F &&f) const {
     constexpr int kAhead = 8;
     for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kAhead * kThreads) {
       float v[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) v[j] = i + j * kThreads < end ? x[i + j * kThreads] : 0.0f;
+      decltype(g(0.0f)) y[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) y[j] = g(v[j]);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
-        if (i + j * kThreads < end) f(v[j], i + j * kThreads);
+        if (i + j * kThreads < end) f(v[j], i + j * kThreads, y[j]);
     }
   }
 };
@@ -410,12 +440,18 @@ struct Held {
       v[j] = i < n ? x[i] : 0.0f;
     }
   }
-  template <class F>
-  __device__ __forceinline__ void each(F &&f) const {
+  template <class G, class F>
+  __device__ __forceinline__ void each(G &&g, F &&f) const {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = threadIdx.x + j * kThreads;
-      if (i < n) f(v[j], i);
+    for (int j0 = 0; j0 < N; j0 += 8) {
+      decltype(g(0.0f)) y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = g(v[j0 + j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = threadIdx.x + (j0 + j) * kThreads;
+        if (i < n) f(v[j0 + j], i, y[j]);
+      }
     }
   }
 };
@@ -424,12 +460,12 @@ struct Held {
 template <class Tokens>
 __device__ Chunk extremes(const Tokens &tokens, Extremes &l) {
   Chunk c{-INFINITY, INFINITY, INT_MAX, 0};
-  auto take = [&](float v, int i) {
+  auto take = [&](float v, int i, int) {
     c.bad |= !(v < INFINITY);
     if (v > c.top) c.top = v, c.at = i;
     if (v > -INFINITY) c.low = fminf(c.low, v);
   };
-  tokens.each(take);
+  tokens.each([](float) { return 0; }, take);
   const float top = ikv::wave_max(c.top);
   int at = c.top == top ? c.at : INT_MAX;
   for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
@@ -460,8 +496,7 @@ __device__ void fill_bins(const Row &row, const Window &win, bool counts, const 
     l.count[b] = 0;
   }
   __syncthreads();
-  tokens.each([&](float x, int) {
-    const unsigned long long w = row.weight(x);
+  tokens.each([&](float x) { return row.weight(x); }, [&](float x, int, unsigned long long w) {
     if (w == 0) return;
     const int b = win.bin(x);
     atomicAdd(&l.mass[b], w);
@@ -552,8 +587,8 @@ template <class Tokens>
 __device__ void gather(const Row &row, const Window &win, const Ranges &rg, const Tokens &tokens, Lists &l) {
   if (threadIdx.x == 0) l.n = 0;
   __syncthreads();
-  tokens.each([&](float x, int i) {
-    if (!rg.holds(win.bin(x)) || row.weight(x) == 0) return;
+  tokens.each([&](float x) { return rg.holds(win.bin(x)); }, [&](float x, int i, bool in) {
+    if (!in || row.weight(x) == 0) return;
     const int at = atomicAdd(&l.n, 1);
     if (at < kList) l.list[at] = static_cast<unsigned long long>(order_of(x)) << 32 | static_cast<unsigned>(i);
   });
@@ -667,9 +702,9 @@ __device__ void resolve(const Args &a, int r, const Row &row, const Window &win,
       answer(a, r, static_cast<int>(static_cast<unsigned>(l.list[tid * kPer + j])), x[j], row, c, kept);
 }
 
-__device__ Row row_of(const Args &a, int r, const Cuts &c, float top) {
+__device__ Row row_of(const Args &a, int r, const Cuts &c, float top, const double *powers) {
   return Row{a.logits + static_cast<size_t>(r) * a.n, a.n, top,
-             1.4426950408889634074 / static_cast<double>(c.t), static_cast<double>(a.shift)};
+             1.4426950408889634074 / static_cast<double>(c.t), static_cast<double>(a.shift), powers};
 }
 
 // Whether a row needs no sums; its answer where `write`.
@@ -692,9 +727,11 @@ __device__ bool settled(const Args &a, int r, const Cuts &c, const Chunk &e, boo
 template <class Tokens>
 __device__ void sample_row(const Args &a, int r, const Cuts &c, const Tokens &tokens, Space &s) {
   __shared__ Extremes x;
+  __shared__ double powers[kPowers];
+  fill_powers(powers);  // (a barrier follows)
   const Chunk e = extremes(tokens, x);
   if (settled(a, r, c, e, threadIdx.x == 0)) return;
-  const Row row = row_of(a, r, c, e.top);
+  const Row row = row_of(a, r, c, e.top, powers);
   const Window win(row, e.low, c.t);
   fill_bins(row, win, c.k > 0 && c.k < a.n, tokens, s.l);
   const Ranges rg = find_ranges(row, win, c, s.l);
@@ -777,12 +814,14 @@ __device__ __forceinline__ T load_agent(const T *p) {
 // The second: the bins, and by the workgroup that comes last the borders'.
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(Args a, RowSpace *rows) {
   __shared__ Lists l;
+  __shared__ double powers[kPowers];
+  fill_powers(powers);  // (a barrier follows)
   const int r = blockIdx.y;
   RowSpace &w = rows[r];
   const Cuts c(a, r);
   const Chunk e = row_extremes(w, gridDim.x);
   if (settled(a, r, c, e, blockIdx.x == 0 && threadIdx.x == 0)) return;
-  const Row row = row_of(a, r, c, e.top);
+  const Row row = row_of(a, r, c, e.top, powers);
   const Window win(row, e.low, c.t);
   const bool counts = c.k > 0 && c.k < a.n;
   fill_bins(row, win, counts, chunk_of(a), l);
@@ -809,13 +848,15 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(Args a, RowSpace 
 // answer.
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Args a, RowSpace *rows) {
   __shared__ Space s;
+  __shared__ double powers[kPowers];
+  fill_powers(powers);  // (a barrier follows)
   Lists &l = s.l;
   const int r = blockIdx.y, tid = threadIdx.x;
   RowSpace &w = rows[r];
   const Cuts c(a, r);
   const Chunk e = row_extremes(w, gridDim.x);
   if (settled(a, r, c, e, false)) return;
-  const Row row = row_of(a, r, c, e.top);
+  const Row row = row_of(a, r, c, e.top, powers);
   const Window win(row, e.low, c.t);
   const Ranges rg = w.ranges;
   gather(row, win, rg, chunk_of(a), l);
