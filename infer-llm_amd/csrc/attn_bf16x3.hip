@@ -125,7 +125,9 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
   const int stride = n_head_kv * dim;  // floats of a token row
   if constexpr (PACKED) {  // one sequence's rows, cache and sizes from here on
     ikv::PackedBlock b;
-    if (!ikv::packed_block<BR>(seqs, G, item, b)) return;
+    if (!(seqs.longest_first ? ikv::packed_block_longest<BR, BN>(seqs, G, item, b)
+                             : ikv::packed_block<BR>(seqs, G, item, b)))
+      return;
     item = b.item;
     n_blocks = b.n_blocks;
     n_rows = b.rows * G;
@@ -662,8 +664,10 @@ void launch(const float *q, const float *k, const float *v, float *out, int n_he
 
 template <int DT, int RW, int KG, int MINW>
 void launch_packed(const float *q, const float *k, const float *v, float *out, int n_head_kv, int G,
-                   int dim, float sl2, const ikv::Pages *pg, const ikv::PackedSeqs &seqs, hipStream_t s) {
+                   int dim, float sl2, const ikv::Pages *pg, ikv::PackedSeqs seqs, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(ikv::packed_blocks(seqs.n_rows, seqs.n_seq, G, 32 * RW) * n_head_kv);
+  // (where all blocks start at once their order does not matter)
+  seqs.longest_first = seqs.n_seq <= ikv::kOrderedSeqs && grid > MINW * kCUs;
   if (pg)
     attn_bf16x3_kernel<DT, RW, KG, MINW, true, true><<<grid, RW * KG * 64, 0, s>>>(
         q, k, v, out, n_head_kv, G, dim, 0, 0, 0, 0, sl2, *pg, seqs);

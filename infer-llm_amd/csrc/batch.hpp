@@ -86,6 +86,7 @@ struct PackedSeqs {
   int capacity = 0;  // tokens that a sequence may have
   int64_t stride = 0;  // block table entries per sequence
   int *status = nullptr;
+  bool longest_first = false;  // the blocks' order (packed_block_longest)
 };
 
 // One block of `block` query rows (row = token * G + query head of the group)
@@ -121,6 +122,77 @@ __device__ __forceinline__ bool packed_block(const PackedSeqs &p, int G, int ite
   }
   b.n_blocks = (b.rows * G + BLOCK - 1) / BLOCK;
   return b.item < b.n_blocks;
+}
+
+// Integer sum over the wave's lanes (DPP and lane swaps), in a scalar register: a
+// workgroup that leaves on it leaves whole, for the compiler, too.
+__device__ __forceinline__ int wave_sum_int(int x) {
+  x += __builtin_amdgcn_mov_dpp(x, kDppXor1, 0xF, 0xF, false);
+  x += __builtin_amdgcn_mov_dpp(x, kDppXor2, 0xF, 0xF, false);
+  x += __builtin_amdgcn_mov_dpp(x, kDppHalfMirror, 0xF, 0xF, false);
+  x += __builtin_amdgcn_mov_dpp(x, kDppMirror, 0xF, 0xF, false);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = static_cast<int>(a[0] + a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __builtin_amdgcn_readfirstlane(static_cast<int>(b[0] + b[1]));
+}
+
+constexpr int kOrderedSeqs = 64;  // packed_block_longest: a sequence a lane
+
+// packed_block with the blocks of all sequences (up to 64) in the order of their
+// tiles of TILE keys, the longest first, so that a launch of more blocks than fit
+// the card does not end on a long one. The number of blocks of at least L tiles
+// is a sum over the sequences, each a division; the L of item's block is found by
+// bisection, about 1 us.
+template <int BLOCK, int TILE>
+__device__ __forceinline__ bool packed_block_longest(const PackedSeqs &p, int G, int item, PackedBlock &b) {
+  check_row_start(p.row_start, p.n_seq, p.n_rows, p.status);
+  const int lane = threadIdx.x & 63;
+  int first = 0, rows = 0, past = 0;
+  if (lane < p.n_seq) {
+    first = p.row_start[lane];
+    const int end = p.row_start[lane + 1];
+    past = p.n_past ? p.n_past[lane] : 0;
+    if (first >= 0 && end >= first && end <= p.n_rows) rows = end - first;
+    if (past < 0 || past > p.capacity - rows) {
+      if (rows > 0 && blockIdx.x == 0 && threadIdx.x < 64) raise_status(p.status, IKV_STATUS_POSITION);
+      rows = past = 0;
+    }
+  }
+  const int blocks = (rows * G + BLOCK - 1) / BLOCK;
+  // this sequence's blocks of L tiles or more: its last ones
+  auto at_least = [&](int L) {
+    const int unseen = TILE * (L - 1) - past;  // tokens before the first that sees so many keys
+    if (unseen <= 0) return blocks;
+    return unseen >= rows ? 0 : (rows * G - unseen * G + BLOCK - 1) / BLOCK;
+  };
+  if (item >= wave_sum_int(blocks)) return false;
+  int lo = 1, hi = 1;  // wave_sum_int(at_least(lo)) > item
+  const int most = rows > 0 ? (past + rows + TILE - 1) / TILE : 0;
+  while (__builtin_amdgcn_ballot_w64(most > hi) != 0) hi *= 2;
+  ++hi;  // more tiles than any block has
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (wave_sum_int(at_least(mid)) > item)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int longer = at_least(lo + 1), here = at_least(lo) - longer;
+  int upto = here;  // blocks of lo tiles of this and the sequences before it
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int y = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += y;
+  }
+  const int rank = item - wave_sum_int(longer);
+  b.seq = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
+  b.first = __builtin_amdgcn_readlane(first, b.seq);
+  b.rows = __builtin_amdgcn_readlane(rows, b.seq);
+  b.past = __builtin_amdgcn_readlane(past, b.seq);
+  b.n_blocks = __builtin_amdgcn_readlane(blocks, b.seq);
+  b.item = __builtin_amdgcn_readlane(longer + rank - (upto - here), b.seq);
+  return true;
 }
 
 }  // namespace ikv
