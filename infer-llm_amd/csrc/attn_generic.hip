@@ -210,24 +210,10 @@ __global__ __launch_bounds__(256) void generic_tile_kernel(
     for (int i = 0; i < RW; ++i)
 #pragma unroll
       for (int t = 0; t < DL; ++t) o[i][t] *= alpha[i];
-    int j_plain = KT;  // keys that are added by their weights alone
-    if constexpr (PACKED) {
-      // the tile of a row's last keys: a masked key weighs 0, but 0 times an
-      // infinite value is NaN, so each row takes the keys that it sees
-      if (kb + KT - 1 > n_past + (r0 + wave * RW) / G) {
-        j_plain = 0;
-        for (int j = 0; j < KT; ++j) {
-#pragma unroll
-          for (int i = 0; i < RW; ++i) {
-            if (kb + j > n_past + tok[i]) continue;
-            const float pj = s_p[wave][i][j];
-#pragma unroll
-            for (int t = 0; t < DL; ++t) o[i][t] = fmaf(pj, s_v[j * DP + lane + 64 * t], o[i][t]);
-          }
-        }
-      }
-    }
-    for (int j4 = 0; j4 < j_plain; j4 += 4) {  // 4 keys: the rows' weights as one 16-byte read
+    // The tile of a row's last keys, in PACKED form: a masked key weighs 0, but 0
+    // times an infinite value is NaN, so its values are taken for zeros
+    const bool last_keys = PACKED && kb + KT - 1 > n_past + (r0 + wave * RW) / G;
+    for (int j4 = 0; j4 < KT; j4 += 4) {  // 4 keys: the rows' weights as one 16-byte read
       float vd[4][DL];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -236,6 +222,18 @@ __global__ __launch_bounds__(256) void generic_tile_kernel(
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
         const float4 pj = *reinterpret_cast<const float4 *>(&s_p[wave][i][j4]);
+        if constexpr (PACKED) {
+          if (last_keys) {
+            const float px[4] = {pj.x, pj.y, pj.z, pj.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const bool sees = kb + j4 + u <= n_past + tok[i];
+#pragma unroll
+              for (int t = 0; t < DL; ++t) o[i][t] = fmaf(px[u], sees ? vd[u][t] : 0.f, o[i][t]);
+            }
+            continue;
+          }
+        }
 #pragma unroll
         for (int t = 0; t < DL; ++t) {
           o[i][t] = fmaf(pj.x, vd[0][t], o[i][t]);
