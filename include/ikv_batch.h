@@ -115,9 +115,12 @@ int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_pool, const
  *            pool is read and not written).
  *   scale    softmax scale; <= 0 selects 1/sqrtf(head_dim)
  *   workspace  device memory of ikv_attn_decode_batch_workspace_bytes() bytes,
- *            16-byte aligned; nothing is expected in it or left in it. It does
- *            not depend on the number of sequences or their lengths. Launches
- *            that share it must be ordered (one stream); concurrent ones race.
+ *            16-byte aligned, for the parts of split contexts and a counter per
+ *            workgroup. It must be zero-filled before its first use; every
+ *            launch leaves the counters at zero again, so it serves every later
+ *            launch of any shape that it is large enough for. Its size does not
+ *            depend on the number of sequences or their lengths. Launches that
+ *            share it must be ordered (one stream); concurrent ones race.
  * Any head_dim up to 512 (else -ENOTSUP) and any n_head that n_head_kv divides;
  * 4-byte aligned operands. A result depends on the other sequences' lengths by
  * the order of its sums, and on nothing else of them; equal calls give equal

@@ -10,8 +10,10 @@
 //     each workgroup adds up the lengths itself.
 //   * A run may end inside a (sequence, head): the workgroup then leaves the
 //     maximum, sum and weighted values of its part in the workspace (at most
-//     two parts a workgroup, so the workspace depends on no length), and a
-//     second launch joins the parts in their order.
+//     two parts a workgroup, so the workspace depends on no length) and counts
+//     itself; the one that comes last joins the parts in their order. Nothing
+//     waits. Up to kWhole units a (sequence, head) stays with the run that holds
+//     its first one: joining takes longer than reading that much.
 //   * LPK lanes hold a key row, NV 16-byte pieces each, so a wave loads 64 / LPK
 //     keys at once; the scores need only the sum over LPK lanes, and each group
 //     of LPK lanes has a running maximum and sums of its own, which meet when
@@ -30,6 +32,7 @@ constexpr int kWaves = 4;       // of a workgroup
 constexpr int kGroups = 2 * kCUs;
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int kMaxDim = 512;
+constexpr int kWhole = 3;  // units of a (sequence, head) that are not split
 constexpr int kAhead = 2;  // keys of a lane group loaded at once
 
 struct Args {
@@ -159,16 +162,28 @@ __device__ __forceinline__ float weight(float m, float top) {  // of sums kept a
   return m == -INFINITY ? 0.f : ikv::fast_exp2(m - top);
 }
 
-// The workspace: (maximum, sum) of each part's heads, then their values. Part
-// 2 w is workgroup w's of a head that began before its run, 2 w + 1 of one that
-// goes on behind it.
+// The workspace: a counter a workgroup (of the parts of the head pass that begins
+// in its run and goes on behind it), then (maximum, sum) of each part's heads and
+// their values. Part 2 w is workgroup w's of a head pass that began before its
+// run, 2 w + 1 of one that goes on behind it. Stored and read at agent scope, as
+// the parts come from several XCDs.
+constexpr size_t kCounterBytes = sizeof(int) * kGroups;
 template <int GQ, int DP>
 struct Parts {
+  int *counters;
   float *ml, *o;
-  __device__ explicit Parts(float *p) : ml(p), o(p + static_cast<size_t>(kGroups) * 2 * GQ * 2) {}
+  __device__ explicit Parts(float *p)
+      : counters(reinterpret_cast<int *>(p)), ml(p + kCounterBytes / sizeof(float)),
+        o(ml + static_cast<size_t>(kGroups) * 2 * GQ * 2) {}
   __device__ float *ml_of(int part, int h) const { return ml + (static_cast<size_t>(part) * GQ + h) * 2; }
   __device__ float *o_of(int part, int h) const { return o + (static_cast<size_t>(part) * GQ + h) * DP; }
 };
+
+__device__ __forceinline__ float2 load2(const float *p) {
+  const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p),
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float(static_cast<unsigned>(x)), __uint_as_float(static_cast<unsigned>(x >> 32)));
+}
 
 template <int LPK, int NV, int GQ, bool VEC>
 __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_kernel(Args a) {
@@ -179,6 +194,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   __shared__ float s_m[kWaves][GQ], s_l[kWaves][GQ];
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][GQ][DP];
   __shared__ float4 s_q[GQ][NV][LPK];  // the query rows, scaled
+  __shared__ int s_last;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = lane % LPK, grp = lane / LPK;
@@ -234,7 +250,13 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
 
   while (u < end) {
     // the run's part of one (sequence, KV head, pass): tiles [p.tile, last)
-    const int last = static_cast<int>(min(static_cast<long long>(p.tiles), p.tile + (end - u)));
+    if (p.tiles <= kWhole && p.tile > 0) {  // (with the run that holds its first unit)
+      u += p.tiles - p.tile;
+      plan.next(a, p);
+      continue;
+    }
+    const int last =
+        p.tiles <= kWhole ? p.tiles : static_cast<int>(min(static_cast<long long>(p.tiles), p.tile + (end - u)));
     const int g = p.item / a.passes, h0 = p.item % a.passes * GQ;
     const int heads = min(GQ, a.G - h0);
     const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
@@ -418,80 +440,94 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     const bool whole = p.tile == 0 && last == p.tiles;
     const Parts<GQ, DP> parts(a.part);
     const int part = 2 * static_cast<int>(blockIdx.x) + (p.tile == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < GQ * DP; i += kWaves * 64) {
-      const int h = i / DP, d = i % DP;
-      if (h >= heads) break;
+    for (int i = threadIdx.x; i < heads * DP / 2; i += kWaves * 64) {
+      const int h = 2 * i / DP, d = 2 * i % DP;
       float top = s_m[0][h];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][h]);
-      float all = 0.f, x = 0.f;
+      float all = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float f = weight(s_m[w][h], top);
         all = fmaf(f, s_l[w][h], all);
         x = fmaf(f, s_o[w][h][d], x);
+        y = fmaf(f, s_o[w][h][d + 1], y);
       }
       if (whole) {
-        if (d < a.dim) a.out[(head0 + h) * a.dim + d] = x / all;
+        float *const o = a.out + (head0 + h) * a.dim + d;
+        if (d < a.dim) o[0] = x / all;
+        if (d + 1 < a.dim) o[1] = y / all;
       } else {
-        parts.o_of(part, h)[d] = x;
-        if (d == 0) {
-          parts.ml_of(part, h)[0] = top;
-          parts.ml_of(part, h)[1] = all;
+        ikv::store2_agent(parts.o_of(part, h) + d, x, y);
+        if (d == 0) ikv::store2_agent(parts.ml_of(part, h), top, all);
+      }
+    }
+    if (!whole) {
+      // this thread's stores have completed before the workgroup is counted
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      __builtin_amdgcn_s_waitcnt(0);
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      __syncthreads();
+      // the head pass's first unit, its workgroups
+      const long long begin = u - p.tile;
+      const int w0 = static_cast<int>(begin / plan.chunk);
+      const int n = static_cast<int>((begin + p.tiles - 1) / plan.chunk) - w0 + 1;
+      if (threadIdx.x == 0) {
+        int *const counter = parts.counters + w0;
+        s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (s_last) {
+        auto at = [&](int i) { return i == 0 ? 2 * w0 + 1 : 2 * (w0 + i); };
+        for (int h = wave; h < heads; h += kWaves) {
+          float top = -INFINITY;
+          for (int i = lane; i < n; i += 64) top = fmaxf(top, load2(parts.ml_of(at(i), h)).x);
+          top = ikv::wave_max(top);
+          float all = 0.f;
+          for (int i = lane; i < n; i += 64) {
+            const float2 ml = load2(parts.ml_of(at(i), h));
+            all = fmaf(weight(ml.x, top), ml.y, all);
+          }
+          all = ikv::wave_sum(all);
+          if (lane == 0) {
+            s_m[0][h] = top;
+            s_l[0][h] = all;
+          }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < heads * DP / 2; i += kWaves * 64) {
+          const int h = 2 * i / DP, d = 2 * i % DP;
+          if (d >= a.dim) continue;
+          const float top = s_m[0][h], all = s_l[0][h];
+          float x = 0.f, y = 0.f;
+          constexpr int kParts = 8;  // loaded at once
+          for (int j = 0; j < n; j += kParts) {
+            float2 ml[kParts], v[kParts];
+#pragma unroll
+            for (int z = 0; z < kParts; ++z) {
+              const int e = at(min(j + z, n - 1));
+              ml[z] = load2(parts.ml_of(e, h));
+              v[z] = load2(parts.o_of(e, h) + d);
+            }
+#pragma unroll
+            for (int z = 0; z < kParts; ++z) {
+              const float f = j + z < n ? weight(ml[z].x, top) : 0.f;
+              if (j + z < n) {
+                x = fmaf(f, v[z].x, x);
+                y = fmaf(f, v[z].y, y);
+              }
+            }
+          }
+          float *const o = a.out + (head0 + h) * a.dim + d;
+          o[0] = x / all;
+          if (d + 1 < a.dim) o[1] = y / all;
         }
       }
     }
     __syncthreads();
     u += last - p.tile;
     plan.next(a, p);
-  }
-}
-
-// Joins the parts of the head pass that begins in workgroup blockIdx.x's run
-// and goes on behind it: that workgroup's, then one of each run it goes through.
-template <int LPK, int NV, int GQ>
-__global__ __launch_bounds__(256) void decode_batch_join_kernel(Args a) {
-  constexpr int KT = kWaves * kAhead * (64 / LPK);
-  constexpr int DP = LPK * NV * 4;
-  __shared__ float s_top[GQ], s_all[GQ];
-  const Plan<KT> plan(a);
-  const long long begin = plan.chunk * blockIdx.x, end = min(plan.total, begin + plan.chunk);
-  if (begin >= end || end == plan.total) return;
-  const Place p = plan.at(a, end - 1);
-  if (p.tile + 1 == p.tiles) return;            // it ends with the run
-  if (end - 1 - p.tile < begin) return;         // it began before the run
-  const int w0 = blockIdx.x;
-  const int n = static_cast<int>((end - 1 - p.tile + p.tiles - 1) / plan.chunk) - w0 + 1;  // parts
-  const int h0 = p.item % a.passes * GQ, g = p.item / a.passes;
-  const int heads = min(GQ, a.G - h0);
-  const Parts<GQ, DP> parts(a.part);
-  auto part = [&](int i) { return i == 0 ? 2 * w0 + 1 : 2 * (w0 + i); };
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int h = wave; h < heads; h += 4) {
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, parts.ml_of(part(i), h)[0]);
-    top = ikv::wave_max(top);
-    float all = 0.f;
-    for (int i = lane; i < n; i += 64) {
-      const float *ml = parts.ml_of(part(i), h);
-      all = fmaf(weight(ml[0], top), ml[1], all);
-    }
-    all = ikv::wave_sum(all);
-    if (lane == 0) {
-      s_top[h] = top;
-      s_all[h] = all;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * DP; i += 256) {
-    const int h = i / DP, d = i % DP;
-    if (d >= a.dim) continue;
-    const float top = s_top[h];
-    float x = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j)
-      x = fmaf(weight(parts.ml_of(part(j), h)[0], top), parts.o_of(part(j), h)[d], x);
-    a.out[((static_cast<size_t>(p.seq) * a.n_head_kv + g) * a.G + h0 + h) * a.dim + d] = x / s_all[h];
   }
 }
 
@@ -514,7 +550,6 @@ int launch(const Args &a, bool vec, hipStream_t s) {
     decode_batch_kernel<LPK, NV, GQ, true><<<kGroups, kWaves * 64, 0, s>>>(a);
   else
     decode_batch_kernel<LPK, NV, GQ, false><<<kGroups, kWaves * 64, 0, s>>>(a);
-  decode_batch_join_kernel<LPK, NV, GQ><<<kGroups, 256, 0, s>>>(a);
   return ikv::launch_status();
 }
 
@@ -523,7 +558,7 @@ int launch(const Args &a, bool vec, hipStream_t s) {
 extern "C" size_t ikv_attn_decode_batch_workspace_bytes(int n_head, int n_head_kv, int head_dim) {
   if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || head_dim > kMaxDim) return 0;
   const Form f = form_of(n_head / n_head_kv, head_dim);
-  return static_cast<size_t>(kGroups) * 2 * f.gq * (f.lpk * f.nv * 4 + 2) * sizeof(float);
+  return kCounterBytes + static_cast<size_t>(kGroups) * 2 * f.gq * (f.lpk * f.nv * 4 + 2) * sizeof(float);
 }
 
 extern "C" int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,

@@ -733,11 +733,11 @@ def attn_prefill_packed_paged(q, k_pool, v_pool, tables, block_tokens: int, row_
 
 
 def decode_batch_workspace(n_head: int, n_head_kv: int, head_dim: int, device="cuda"):
-    """Workspace of attn_decode_batch for these heads: any number of sequences,
-    any lengths (reusable across ordered launches)."""
+    """Zero-filled workspace of attn_decode_batch for these heads: any number of
+    sequences, any lengths (reusable across ordered launches)."""
     torch = _torch()
     nbytes = int(load().ikv_attn_decode_batch_workspace_bytes(n_head, n_head_kv, head_dim))
-    return torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device)
+    return torch.zeros((nbytes + 3) // 4, dtype=torch.float32, device=device)
 
 
 def attn_decode_batch(q, k_pool, v_pool, tables, block_tokens: int, n_kv, *, k_new=None, v_new=None,

@@ -155,13 +155,31 @@ def test_decode_batch_flags_blocks_outside_the_pool(dev):
 def test_decode_batch_equal_calls_give_equal_bits(dev):
     n_kv = [1000, 0, 37, 5000, 64]
     q, pools, tables, fresh, _ = _setup(dev, 31, n_kv, 64, 32, 8, 128)
-    ws = ikv.decode_batch_workspace(32, 8, 128)
+    ws = ikv.decode_batch_workspace(64, 1, 128)  # (larger than it need be)
     args = (q, *pools, _dev32(tables, dev), 64, _dev32(n_kv, dev))
     first = ikv.attn_decode_batch(*args, k_new=fresh[0], v_new=fresh[1], workspace=ws)
-    for fill in (float("nan"), 1e30, 0.0):  # what is in the workspace does not matter
-        ws.fill_(fill)
+    for other in ((16, 2, 128), (3, 1, 65), (32, 8, 128)):  # also after other shapes
+        need = ikv.load().ikv_attn_decode_batch_workspace_bytes(*other)
+        assert need <= ws.numel() * 4
+        n2 = [900, 3, 2100]
+        q2, pools2, tables2, fresh2, own2 = _setup(dev, 32, n2, 64, *other)
+        out2 = ikv.attn_decode_batch(q2, *pools2, _dev32(tables2, dev), 64, _dev32(n2, dev), k_new=fresh2[0],
+                                     v_new=fresh2[1], workspace=ws)
+        _check_rows(out2, q2, own2)
         again = ikv.attn_decode_batch(*args, k_new=fresh[0], v_new=fresh[1], workspace=ws)
         assert torch.equal(first, again)
+
+
+def test_decode_batch_of_every_split(dev):
+    """Contexts around the units and the runs: whole, cut once, through several
+    workgroups, next to short ones that are not split."""
+    heads, kv, dim = 4, 2, 128
+    for n_kv in ([64 * i + j for i in range(6) for j in (-1, 0, 1) if 64 * i + j > 0],
+                 [193] * 40, [30000] + [1] * 70 + [129, 257] * 9, [700 + 61 * i for i in range(90)]):
+        q, pools, tables, fresh, own = _setup(dev, len(n_kv), n_kv, 64, heads, kv, dim)
+        out = ikv.attn_decode_batch(q, *pools, _dev32(tables, dev), 64, _dev32(n_kv, dev), k_new=fresh[0],
+                                    v_new=fresh[1])
+        _check_rows(out, q, own)
 
 
 def test_decode_batch_replays_with_new_lengths(dev):
