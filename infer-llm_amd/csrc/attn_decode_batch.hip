@@ -54,11 +54,11 @@ __device__ __forceinline__ int keys_of(const Args &a, int seq) {
   return n > 0 && n <= a.b.capacity ? n : 0;
 }
 
-__device__ __forceinline__ long long wave_prefix(long long x) {  // inclusive
+__device__ __forceinline__ unsigned long long wave_prefix(unsigned long long x) {  // inclusive
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) {
-    const long long y = __shfl_up(x, o, 64);
+    const unsigned long long y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
   return x;
@@ -71,58 +71,74 @@ struct Place {
 
 template <int KT>
 struct Plan {
-  long long total, chunk;
+  using Units = unsigned long long;
+  Units total, chunk;
+  unsigned items;  // head passes of a sequence
+  // the sequence s0 + lane of 64: its keys, and the units up to its end
+  int s0, keys;
+  Units upto;
 
   __device__ static int tiles_of(int keys) { return (keys + KT - 1) / KT; }
 
-  __device__ Plan(const Args &a) {
-    const int lane = threadIdx.x & 63;
-    long long t = 0;
-    for (int s = lane; s < a.b.n_seq; s += 64) t += tiles_of(keys_of(a, s));
-    total = __shfl(wave_prefix(t), 63, 64) * (static_cast<long long>(a.n_head_kv) * a.passes);
+  __device__ void look(const Args &a, int first, Units before) {
+    const int s = first + static_cast<int>(threadIdx.x & 63);
+    s0 = first;
+    keys = s < a.b.n_seq ? keys_of(a, s) : 0;
+    upto = before + wave_prefix(static_cast<Units>(tiles_of(keys)) * items);
+  }
+
+  __device__ Plan(const Args &a) : items(a.n_head_kv * a.passes) {
+    total = 0;
+    for (int s = 0; s < a.b.n_seq; s += 64) {
+      look(a, s, total);
+      total = __shfl(upto, 63, 64);
+    }
     chunk = (total + kGroups - 1) / kGroups;
   }
 
   // where unit u (< total) is
-  __device__ Place at(const Args &a, long long u) const {
-    const int lane = threadIdx.x & 63;
-    const long long items = static_cast<long long>(a.n_head_kv) * a.passes;
-    long long base = 0;
-    Place p{};
-    for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-      const int keys = s0 + lane < a.b.n_seq ? keys_of(a, s0 + lane) : 0;
-      const long long mine = tiles_of(keys) * items;
-      const long long upto = base + wave_prefix(mine);
-      const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > u);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        p.seq = s0 + l;
-        p.keys = __builtin_amdgcn_readlane(keys, l);
-        p.tiles = tiles_of(p.keys);
-        const long long r = u - __shfl(upto - mine, l, 64);
-        p.item = static_cast<int>(r / p.tiles);
-        p.tile = static_cast<int>(r - static_cast<long long>(p.item) * p.tiles);
-        p.item = __builtin_amdgcn_readfirstlane(p.item);
-        p.tile = __builtin_amdgcn_readfirstlane(p.tile);
-        return p;
+  __device__ Place at(const Args &a, Units u) {
+    if (a.b.n_seq > 64) {
+      Units before = 0;
+      for (int s = 0; s < a.b.n_seq; s += 64) {
+        look(a, s, before);
+        before = __shfl(upto, 63, 64);
+        if (before > u) break;
       }
-      base = __shfl(upto, 63, 64);
     }
-    return p;  // (not reached for u < total)
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > u));
+    Place p;
+    p.seq = s0 + l;
+    p.keys = __builtin_amdgcn_readlane(keys, l);
+    p.tiles = tiles_of(p.keys);
+    const Units r = u - (__shfl(upto, l, 64) - static_cast<Units>(p.tiles) * items);
+    if (r >> 32) {
+      p.item = static_cast<int>(r / p.tiles);
+      p.tile = static_cast<int>(r % p.tiles);
+    } else {
+      p.item = static_cast<int>(static_cast<unsigned>(r) / p.tiles);
+      p.tile = static_cast<int>(static_cast<unsigned>(r) % p.tiles);
+    }
+    p.item = __builtin_amdgcn_readfirstlane(p.item);
+    p.tile = __builtin_amdgcn_readfirstlane(p.tile);
+    return p;
   }
 
   // the first unit of the next head pass
-  __device__ void next(const Args &a, Place &p) const {
+  __device__ void next(const Args &a, Place &p) {
     p.tile = 0;
-    if (++p.item < a.n_head_kv * a.passes) return;
+    if (++p.item < static_cast<int>(items)) return;
     p.item = 0;
     const int lane = threadIdx.x & 63;
-    for (int s0 = p.seq + 1; s0 < a.b.n_seq; s0 += 64) {
-      const int keys = s0 + lane < a.b.n_seq ? keys_of(a, s0 + lane) : 0;
-      const unsigned long long some = __builtin_amdgcn_ballot_w64(keys > 0);
+    for (int first = s0;; first += 64) {
+      if (first != s0) {
+        if (first >= a.b.n_seq) return;  // (behind the last sequence: nobody goes on)
+        look(a, first, 0);               // (upto is not asked again)
+      }
+      const unsigned long long some = __builtin_amdgcn_ballot_w64(keys > 0 && first + lane > p.seq);
       if (some) {
         const int l = __builtin_ctzll(some);
-        p.seq = s0 + l;
+        p.seq = first + l;
         p.keys = __builtin_amdgcn_readlane(keys, l);
         p.tiles = tiles_of(p.keys);
         return;
@@ -202,16 +218,17 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   const int stride = a.n_head_kv * a.dim;  // floats of a token row
 
   // slots without keys: a zero row, and the flag where the length is no length
-  for (int s = blockIdx.x; s < a.b.n_seq; s += gridDim.x) {
+  // (from the last workgroups on: in a small call they have nothing else to do)
+  for (int s = gridDim.x - 1 - blockIdx.x; s < a.b.n_seq; s += gridDim.x) {
     if (keys_of(a, s) > 0) continue;
     if (a.n_kv[s] != 0 && threadIdx.x == 0) ikv::raise_status(a.b.status, IKV_STATUS_POSITION);
     float *o = a.out + static_cast<size_t>(s) * n_head * a.dim;
     for (int d = threadIdx.x; d < n_head * a.dim; d += kWaves * 64) o[d] = 0.f;
   }
 
-  const Plan<KT> plan(a);
-  long long u = plan.chunk * blockIdx.x;
-  const long long end = min(plan.total, u + plan.chunk);
+  Plan<KT> plan(a);
+  unsigned long long u = plan.chunk * blockIdx.x;
+  const unsigned long long end = min(plan.total, u + plan.chunk);
   if (u >= end) return;
   Place p = plan.at(a, u);
   unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
@@ -256,7 +273,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       continue;
     }
     const int last =
-        p.tiles <= kWhole ? p.tiles : static_cast<int>(min(static_cast<long long>(p.tiles), p.tile + (end - u)));
+        p.tiles <= kWhole ? p.tiles : static_cast<int>(min<unsigned long long>(p.tiles, p.tile + (end - u)));
     const int g = p.item / a.passes, h0 = p.item % a.passes * GQ;
     const int heads = min(GQ, a.G - h0);
     const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
@@ -270,15 +287,15 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
 #pragma unroll
       for (int n = 0; n < NV; ++n) o[h][n] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    for (int h = wave; h < GQ; h += kWaves) {
-      const auto r = whole_row(a.q + (head0 + min(h, heads - 1)) * a.dim);
+    // the query rows, a head a wave (to LDS once the first keys are on their way)
+    constexpr int kHeads = (GQ + kWaves - 1) / kWaves;
+    float4 qr[kHeads][NV];
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const float4 x = ikv::scale4(a.scale_log2, load(r, 0, n));
-        if (grp == 0) s_q[h][n][l] = x;
-      }
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = min(wave + kWaves * i, heads - 1);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) qr[i][n] = load(whole_row(a.q + (head0 + h) * a.dim), 0, n);
     }
-    __syncthreads();
     // block table entries, 64 at a time, one per lane, checked as they are read
     const int last_blk = (p.keys - 1) / pg.bt;
     int blk = p.tile * KT / pg.bt, in_blk = p.tile * KT % pg.bt, ent0 = blk, ent = 0;
@@ -369,6 +386,13 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     long long row = next_row();
     fetch(a.k, row, p.tile, kr);
     fetch(a.v, row, p.tile, vr);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if (wave + kWaves * i < GQ && grp == 0) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) s_q[wave + kWaves * i][n][l] = ikv::scale4(a.scale_log2, qr[i][n]);
+      }
+    __syncthreads();
     for (int t = p.tile; t < last; ++t) {
       asm volatile("" ::: "memory");  // the query rows stay in LDS
       float s[kAhead][GQ];
@@ -469,7 +493,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
       __syncthreads();
       // the head pass's first unit, its workgroups
-      const long long begin = u - p.tile;
+      const unsigned long long begin = u - p.tile;
       const int w0 = static_cast<int>(begin / plan.chunk);
       const int n = static_cast<int>((begin + p.tiles - 1) / plan.chunk) - w0 + 1;
       if (threadIdx.x == 0) {
