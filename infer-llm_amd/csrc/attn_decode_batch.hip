@@ -5,12 +5,15 @@
 // HBM bounds it: every K and V row is read once and takes 4 G flops a float.
 //
 //   * The work is cut into units of KT keys of one KV head of one sequence, in
-//     the order (sequence, KV head, keys). The workgroups take equal runs of
-//     units, however the lengths differ, from n_kv as it stands on the device:
-//     each workgroup adds up the lengths itself.
+//     the order (sequence, KV head, keys), and these into runs of equal length,
+//     from n_kv as it stands on the device: each workgroup adds up the lengths
+//     itself. There are as many runs as workgroups, or, where that makes them
+//     longer than 16 units, up to four times as many: a workgroup that has done
+//     its own takes the next one that is left (with equal shares the last
+//     workgroup was done 13 % after the average one).
 //   * A run may end inside a (sequence, head): the workgroup then leaves the
 //     maximum, sum and weighted values of its part in the workspace (at most
-//     two parts a workgroup, so the workspace depends on no length) and counts
+//     two parts a run, so the workspace depends on no length) and counts
 //     itself; the one that comes last joins the parts in their order. Nothing
 //     waits. Up to kWhole units a (sequence, head) stays with the run that holds
 //     its first one: joining takes longer than reading that much.
@@ -29,7 +32,9 @@ namespace {
 
 constexpr int kCUs = 256;       // MI355X compute units
 constexpr int kWaves = 4;       // of a workgroup
-constexpr int kGroups = 2 * kCUs;
+constexpr int kGroups = 2 * kCUs;    // workgroups of a launch
+constexpr int kRuns = 4 * kGroups;   // most runs of units
+constexpr int kRunUnits = 16;        // units of a run where there are more runs than workgroups
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int kMaxDim = 512;
 constexpr int kWhole = 3;  // units of a (sequence, head) that are not split
@@ -64,6 +69,13 @@ __device__ __forceinline__ unsigned long long wave_prefix(unsigned long long x) 
   return x;
 }
 
+// x of lane l (the same for the whole wave), in scalar registers.
+__device__ __forceinline__ unsigned long long lane_value(unsigned long long x, int l) {
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(x), l);
+  const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(x >> 32), l);
+  return static_cast<unsigned long long>(hi) << 32 | lo;
+}
+
 // A place in the list of units: unit `tile` of `tiles` of head pass `item`.
 struct Place {
   int seq, keys, tiles, item, tile;
@@ -72,7 +84,8 @@ struct Place {
 template <int KT>
 struct Plan {
   using Units = unsigned long long;
-  Units total, chunk;
+  Units total, chunk;  // all units, those of a run
+  int runs;
   unsigned items;  // head passes of a sequence
   // the sequence s0 + lane of 64: its keys, and the units up to its end
   int s0, keys;
@@ -91,9 +104,11 @@ struct Plan {
     total = 0;
     for (int s = 0; s < a.b.n_seq; s += 64) {
       look(a, s, total);
-      total = __shfl(upto, 63, 64);
+      total = lane_value(upto, 63);
     }
-    chunk = (total + kGroups - 1) / kGroups;
+    runs = static_cast<int>(min(max(total / kRunUnits, static_cast<Units>(kGroups)), static_cast<Units>(kRuns)));
+    chunk = (total + runs - 1) / runs;
+    if (chunk == 0) chunk = 1;
   }
 
   // where unit u (< total) is
@@ -102,7 +117,7 @@ struct Plan {
       Units before = 0;
       for (int s = 0; s < a.b.n_seq; s += 64) {
         look(a, s, before);
-        before = __shfl(upto, 63, 64);
+        before = lane_value(upto, 63);
         if (before > u) break;
       }
     }
@@ -111,7 +126,7 @@ struct Plan {
     p.seq = s0 + l;
     p.keys = __builtin_amdgcn_readlane(keys, l);
     p.tiles = tiles_of(p.keys);
-    const Units r = u - (__shfl(upto, l, 64) - static_cast<Units>(p.tiles) * items);
+    const Units r = u - (lane_value(upto, l) - static_cast<Units>(p.tiles) * items);
     if (r >> 32) {
       p.item = static_cast<int>(r / p.tiles);
       p.tile = static_cast<int>(r % p.tiles);
@@ -178,19 +193,19 @@ __device__ __forceinline__ float weight(float m, float top) {  // of sums kept a
   return m == -INFINITY ? 0.f : ikv::fast_exp2(m - top);
 }
 
-// The workspace: a counter a workgroup (of the parts of the head pass that begins
-// in its run and goes on behind it), then (maximum, sum) of each part's heads and
-// their values. Part 2 w is workgroup w's of a head pass that began before its
-// run, 2 w + 1 of one that goes on behind it. Stored and read at agent scope, as
+// The workspace: a counter a run (of the parts of the head pass that begins in it
+// and goes on behind it) and one of the runs that were fetched, then (maximum,
+// sum) of each part's heads and their values. Part 2 r is run r's of a head pass
+// that began before it, 2 r + 1 of one that goes on behind it. Stored and read at agent scope, as
 // the parts come from several XCDs.
-constexpr size_t kCounterBytes = sizeof(int) * kGroups;
+constexpr size_t kCounterBytes = sizeof(int) * (kRuns + 64);
 template <int GQ, int DP>
 struct Parts {
-  int *counters;
+  int *counters;  // [kRuns], then the fetched runs'
   float *ml, *o;
   __device__ explicit Parts(float *p)
       : counters(reinterpret_cast<int *>(p)), ml(p + kCounterBytes / sizeof(float)),
-        o(ml + static_cast<size_t>(kGroups) * 2 * GQ * 2) {}
+        o(ml + static_cast<size_t>(kRuns) * 2 * GQ * 2) {}
   __device__ float *ml_of(int part, int h) const { return ml + (static_cast<size_t>(part) * GQ + h) * 2; }
   __device__ float *o_of(int part, int h) const { return o + (static_cast<size_t>(part) * GQ + h) * DP; }
 };
@@ -210,6 +225,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   __shared__ float s_m[kWaves][GQ], s_l[kWaves][GQ];
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][GQ][DP];
   __shared__ float4 s_q[GQ][NV][LPK];  // the query rows, scaled
+  __shared__ float4 s_new[2][NV][LPK];  // the new token's K and V row
   __shared__ int s_last;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -227,10 +243,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   }
 
   Plan<KT> plan(a);
-  unsigned long long u = plan.chunk * blockIdx.x;
-  const unsigned long long end = min(plan.total, u + plan.chunk);
-  if (u >= end) return;
-  Place p = plan.at(a, u);
+  const Parts<GQ, DP> parts(a.part);
   unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
@@ -265,7 +278,31 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     }
   };
 
-  while (u < end) {
+  int run = blockIdx.x;
+  unsigned long long u = plan.chunk * run, end = min(plan.total, u + plan.chunk);
+  Place p{};
+  if (u < end) p = plan.at(a, u);
+  for (;;) {
+    if (u >= end) {
+      // the next run that nobody has: the first come, first served, so that no
+      // workgroup is left with more than a run at the end. Every workgroup fetches
+      // until there is none, runs times in all; the last fetch clears the counter.
+      if (plan.runs <= kGroups) return;
+      if (threadIdx.x == 0) {
+        int *const fetched = parts.counters + kRuns;
+        const int before = __hip_atomic_fetch_add(fetched, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == plan.runs - 1) __hip_atomic_store(fetched, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = before;
+      }
+      __syncthreads();
+      run = kGroups + __builtin_amdgcn_readfirstlane(s_last);
+      __syncthreads();
+      if (run >= plan.runs) return;
+      u = plan.chunk * run;
+      end = min(plan.total, u + plan.chunk);
+      if (u < end) p = plan.at(a, u);
+      continue;
+    }
     // the run's part of one (sequence, KV head, pass): tiles [p.tile, last)
     if (p.tiles <= kWhole && p.tile > 0) {  // (with the run that holds its first unit)
       u += p.tiles - p.tile;
@@ -295,6 +332,14 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       const int h = min(wave + kWaves * i, heads - 1);
 #pragma unroll
       for (int n = 0; n < NV; ++n) qr[i][n] = load(whole_row(a.q + (head0 + h) * a.dim), 0, n);
+    }
+    // and, where the run has the last keys, the new rows by the last two waves
+    const bool has_new = a.k_new != nullptr && last == p.tiles;
+    float4 fresh[NV];
+    if (has_new && wave >= kWaves - 2) {
+      const float *row = (wave == kWaves - 2 ? a.k_new : a.v_new) + static_cast<size_t>(p.seq) * stride + g * a.dim;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) fresh[n] = load(whole_row(row), 0, n);
     }
     // block table entries, 64 at a time, one per lane, checked as they are read
     const int last_blk = (p.keys - 1) / pg.bt;
@@ -392,6 +437,10 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
 #pragma unroll
         for (int n = 0; n < NV; ++n) s_q[wave + kWaves * i][n][l] = ikv::scale4(a.scale_log2, qr[i][n]);
       }
+    if (has_new && wave >= kWaves - 2 && grp == 0) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) s_new[wave - (kWaves - 2)][n][l] = fresh[n];
+    }
     __syncthreads();
     for (int t = p.tile; t < last; ++t) {
       asm volatile("" ::: "memory");  // the query rows stay in LDS
@@ -409,14 +458,13 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       raise(s);
       add_values(s, vr);
       fetch(a.v, row, t + 1, vr);
-      if (t + 1 == p.tiles && a.k_new) {
+      if (has_new && t + 1 == p.tiles) {
         // the new token, by the first wave's first lanes, and its place in the pools
-        const size_t from = static_cast<size_t>(p.seq) * stride + g * a.dim;
         float4 kn[1][NV], vn[1][NV];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-          kn[0][n] = load(whole_row(a.k_new + from), 0, n);
-          vn[0][n] = load(whole_row(a.v_new + from), 0, n);
+          kn[0][n] = s_new[0][n][l];
+          vn[0][n] = s_new[1][n][l];
         }
         float sn[1][GQ];
         scores(kn, sn);
@@ -462,8 +510,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     }
     __syncthreads();
     const bool whole = p.tile == 0 && last == p.tiles;
-    const Parts<GQ, DP> parts(a.part);
-    const int part = 2 * static_cast<int>(blockIdx.x) + (p.tile == 0 ? 1 : 0);
+    const int part = 2 * run + (p.tile == 0 ? 1 : 0);
     for (int i = threadIdx.x; i < heads * DP / 2; i += kWaves * 64) {
       const int h = 2 * i / DP, d = 2 * i % DP;
       float top = s_m[0][h];
@@ -492,7 +539,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       __builtin_amdgcn_s_waitcnt(0);
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
       __syncthreads();
-      // the head pass's first unit, its workgroups
+      // the head pass's first unit, its first run, its runs
       const unsigned long long begin = u - p.tile;
       const int w0 = static_cast<int>(begin / plan.chunk);
       const int n = static_cast<int>((begin + p.tiles - 1) / plan.chunk) - w0 + 1;
@@ -582,7 +629,7 @@ int launch(const Args &a, bool vec, hipStream_t s) {
 extern "C" size_t ikv_attn_decode_batch_workspace_bytes(int n_head, int n_head_kv, int head_dim) {
   if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || head_dim > kMaxDim) return 0;
   const Form f = form_of(n_head / n_head_kv, head_dim);
-  return kCounterBytes + static_cast<size_t>(kGroups) * 2 * f.gq * (f.lpk * f.nv * 4 + 2) * sizeof(float);
+  return kCounterBytes + static_cast<size_t>(kRuns) * 2 * f.gq * (f.lpk * f.nv * 4 + 2) * sizeof(float);
 }
 
 extern "C" int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,
