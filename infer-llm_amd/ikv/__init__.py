@@ -595,20 +595,19 @@ def attn_prefill_paged(q, k_pool, v_pool, table, block_tokens: int, n_past: int 
 # device int32 tensors, which a captured call reads anew at every replay
 # ----------------------------------------------------------------------------
 
-def _operands(device, **tensors):
-    """Contiguous tensors on `device`: float32 ones, or int32 where the name
-    ends in _i. None is left out."""
+def _operands(device, floats, float_names, ints, int_names):
+    """Contiguous float32 and int32 tensors on `device`, a device; None is left out."""
     torch = _torch()
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        want = torch.int32 if name.endswith("_i") else torch.float32
-        if t.dtype is not want:
-            raise TypeError(f"{name.removesuffix('_i')} must be {want}, got {t.dtype}")
-        if t.device != device or not t.is_cuda:
-            raise ValueError(f"{name.removesuffix('_i')} must be on the device of the others")
-        if not t.is_contiguous():
-            raise ValueError(f"{name.removesuffix('_i')} must be contiguous")
+    for want, tensors, names in ((torch.float32, floats, float_names), (torch.int32, ints, int_names)):
+        for i, t in enumerate(tensors):
+            if t is None or (t.dtype is want and t.device == device and t.is_cuda and t.is_contiguous()):
+                continue
+            name = names.split()[i]
+            if t.dtype is not want:
+                raise TypeError(f"{name} must be {want}, got {t.dtype}")
+            if t.device != device or not t.is_cuda:
+                raise ValueError(f"{name} must be on the device of the others")
+            raise ValueError(f"{name} must be contiguous")
 
 
 class _Here:
@@ -661,8 +660,8 @@ def append_packed(k_pool, v_pool, k_rows, v_rows, tables, block_tokens: int, row
     """Rows [row_start[s], row_start[s + 1]) of k_rows and v_rows [n, n_head_kv, D]
     become sequence s's tokens first_token[s].. (0.. without it) in the pools."""
     dev = k_pool.device
-    _operands(dev, k_pool=k_pool, v_pool=v_pool, k_rows=k_rows, v_rows=v_rows, tables_i=tables,
-              row_start_i=row_start, first_token_i=first_token, status_i=status)
+    _operands(dev, (k_pool, v_pool, k_rows, v_rows), "k_pool v_pool k_rows v_rows",
+              (tables, row_start, first_token, status), "tables row_start first_token status")
     if k_rows.dim() != 3 or k_rows.shape != v_rows.shape:
         raise ValueError("k_rows and v_rows must be of one shape [rows, n_head_kv, head_dim]")
     n_rows, n_head_kv, D = k_rows.shape
@@ -687,7 +686,7 @@ def attn_prefill_packed(q, k, v, row_start, *, out=None, scale: float = 0.0, sta
     that is allocated here: undefined)."""
     torch = _torch()
     dev = q.device
-    _operands(dev, q=q, k=k, v=v, out=out, row_start_i=row_start, status_i=status)
+    _operands(dev, (q, k, v, out), "q k v out", (row_start, status), "row_start status")
     n_rows, n_head, D = q.shape
     if k.dim() != 3 or k.shape != v.shape or k.shape[0] != n_rows or k.shape[2] != D:
         raise ValueError("k and v must be [rows of q, n_head_kv, head_dim]")
@@ -711,8 +710,8 @@ def attn_prefill_packed_paged(q, k_pool, v_pool, tables, block_tokens: int, row_
     sequence's queries behind n_past[s] cached tokens (none without it)."""
     torch = _torch()
     dev = q.device
-    _operands(dev, q=q, k_pool=k_pool, v_pool=v_pool, out=out, tables_i=tables,
-              row_start_i=row_start, n_past_i=n_past, status_i=status)
+    _operands(dev, (q, k_pool, v_pool, out), "q k_pool v_pool out",
+              (tables, row_start, n_past, status), "tables row_start n_past status")
     n_rows, n_head, D = q.shape
     _need_pools(k_pool, v_pool, k_pool.shape[-2], D)
     bt = kv_batch(tables, block_tokens, k_pool, status)
@@ -748,8 +747,8 @@ def attn_decode_batch(q, k_pool, v_pool, tables, block_tokens: int, n_kv, *, k_n
     appended."""
     torch = _torch()
     dev = q.device
-    _operands(dev, q=q, k_pool=k_pool, v_pool=v_pool, k_new=k_new, v_new=v_new, out=out,
-              workspace=workspace, tables_i=tables, n_kv_i=n_kv, status_i=status)
+    _operands(dev, (q, k_pool, v_pool, k_new, v_new, out, workspace),
+              "q k_pool v_pool k_new v_new out workspace", (tables, n_kv, status), "tables n_kv status")
     n_seq, n_head, D = q.shape
     n_head_kv = k_pool.shape[-2]
     _need_pools(k_pool, v_pool, n_head_kv, D)
@@ -962,15 +961,14 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, t
     int32 and float32 [n_rows]."""
     torch = _torch()
     dev = logits.device
-    _operands(dev, logits=logits, u=u, temperature=temperature, top_k_i=top_k, top_p=top_p, min_p=min_p,
-              token_i=token, logprob=logprob, workspace=workspace)
+    _operands(dev, (logits, u, temperature, top_p, min_p, logprob, workspace),
+              "logits u temperature top_p min_p logprob workspace", (top_k, token), "top_k token")
     if logits.dim() != 2:
         raise ValueError("logits must be [n_rows, n_vocab]")
     n_rows, n_vocab = logits.shape
-    for name, t in (("u", u), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
-                    ("min_p", min_p), ("token", token), ("logprob", logprob)):
+    for t in (u, temperature, top_k, top_p, min_p, token, logprob):
         if t is not None and t.numel() != n_rows:
-            raise ValueError(f"{name} must hold a value per row")
+            raise ValueError("u, the parameters and the results must hold a value per row")
     with _on(dev, stream):
         if token is None:
             token = torch.empty(n_rows, dtype=torch.int32, device=dev)
