@@ -667,7 +667,7 @@ void launch_packed(const float *q, const float *k, const float *v, float *out, i
                    int dim, float sl2, const ikv::Pages *pg, ikv::PackedSeqs seqs, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(ikv::packed_blocks(seqs.n_rows, seqs.n_seq, G, 32 * RW) * n_head_kv);
   // (where all blocks start at once their order does not matter)
-  seqs.longest_first = seqs.n_seq <= ikv::kOrderedSeqs && grid > MINW * kCUs;
+  seqs.longest_first = seqs.n_seq <= ikv::kLaneSeqs && grid > MINW * kCUs;
   if (pg)
     attn_bf16x3_kernel<DT, RW, KG, MINW, true, true><<<grid, RW * KG * 64, 0, s>>>(
         q, k, v, out, n_head_kv, G, dim, 0, 0, 0, 0, sl2, *pg, seqs);

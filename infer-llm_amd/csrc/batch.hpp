@@ -101,24 +101,59 @@ __host__ __device__ inline int64_t packed_blocks(int64_t n_rows, int64_t n_seq, 
   return n_rows * G / block + n_seq;
 }
 
+constexpr int kLaneSeqs = 64;  // up to so many, a sequence a lane
+
+// One sequence of each lane: its first row, its rows and its history; no rows
+// where its sizes are out of range (flagged).
+struct LaneSeq {
+  int first = 0, rows = 0, past = 0;
+  __device__ explicit LaneSeq(const PackedSeqs &p) {
+    const int lane = threadIdx.x & 63;
+    if (lane >= p.n_seq) return;
+    const int at = p.row_start[lane], end = p.row_start[lane + 1], before = p.n_past ? p.n_past[lane] : 0;
+    if (at < 0 || end < at || end > p.n_rows) return;  // (check_row_start raises)
+    first = at;
+    if (before < 0 || before > p.capacity - (end - at)) {
+      if (end > at && blockIdx.x == 0 && threadIdx.x < 64) raise_status(p.status, IKV_STATUS_POSITION);
+      return;
+    }
+    rows = end - at;
+    past = before;
+  }
+};
+
 // The block that workgroup `item` takes, or false where there is none. Sequence
 // s may take items from row_start[s] * G / block + s on: that leaves it at least
 // the blocks that it has, whatever the lengths, so no list of blocks is needed.
 template <int BLOCK>
 __device__ __forceinline__ bool packed_block(const PackedSeqs &p, int G, int item, PackedBlock &b) {
   check_row_start(p.row_start, p.n_seq, p.n_rows, p.status);
-  auto base = [&](int s) { return min(max(p.row_start[s], 0), p.n_rows) * G / BLOCK + s; };
-  b.seq = wave_find_last(p.n_seq, [&](int s) { return base(s) <= item; });
-  if (b.seq < 0) return false;
-  b.first = p.row_start[b.seq];
-  const int end = p.row_start[b.seq + 1];
-  b.past = p.n_past ? p.n_past[b.seq] : 0;
-  b.item = item - base(b.seq);
-  if (b.first < 0 || end < b.first || end > p.n_rows) return false;  // (check_row_start raises)
-  b.rows = end - b.first;
-  if (b.past < 0 || b.past > p.capacity - b.rows) {
-    if (b.rows > 0 && threadIdx.x == 0) raise_status(p.status, IKV_STATUS_POSITION);
-    return false;
+  auto base = [&](int start, int s) { return min(max(start, 0), p.n_rows) * G / BLOCK + s; };
+  if (p.n_seq <= kLaneSeqs) {
+    // (one round of loads where the search and its result take two)
+    const int lane = threadIdx.x & 63;
+    const LaneSeq mine(p);
+    const int from = lane < p.n_seq ? base(p.row_start[lane], lane) : INT_MAX;
+    const unsigned long long upto = __builtin_amdgcn_ballot_w64(from <= item);
+    if (upto == 0) return false;
+    b.seq = 63 - __builtin_clzll(upto);
+    b.first = __builtin_amdgcn_readlane(mine.first, b.seq);
+    b.rows = __builtin_amdgcn_readlane(mine.rows, b.seq);
+    b.past = __builtin_amdgcn_readlane(mine.past, b.seq);
+    b.item = item - __builtin_amdgcn_readlane(from, b.seq);
+  } else {
+    b.seq = wave_find_last(p.n_seq, [&](int s) { return base(p.row_start[s], s) <= item; });
+    if (b.seq < 0) return false;
+    b.first = p.row_start[b.seq];
+    const int end = p.row_start[b.seq + 1];
+    b.past = p.n_past ? p.n_past[b.seq] : 0;
+    b.item = item - base(b.first, b.seq);
+    if (b.first < 0 || end < b.first || end > p.n_rows) return false;
+    b.rows = end - b.first;
+    if (b.past < 0 || b.past > p.capacity - b.rows) {
+      if (b.rows > 0 && threadIdx.x == 0) raise_status(p.status, IKV_STATUS_POSITION);
+      return false;
+    }
   }
   b.n_blocks = (b.rows * G + BLOCK - 1) / BLOCK;
   return b.item < b.n_blocks;
@@ -137,28 +172,17 @@ __device__ __forceinline__ int wave_sum_int(int x) {
   return __builtin_amdgcn_readfirstlane(static_cast<int>(b[0] + b[1]));
 }
 
-constexpr int kOrderedSeqs = 64;  // packed_block_longest: a sequence a lane
-
-// packed_block with the blocks of all sequences (up to 64) in the order of their
-// tiles of TILE keys, the longest first, so that a launch of more blocks than fit
-// the card does not end on a long one. The number of blocks of at least L tiles
-// is a sum over the sequences, each a division; the L of item's block is found by
-// bisection, about 1 us.
+// packed_block with the blocks of all sequences (up to kLaneSeqs) in the order of
+// their tiles of TILE keys, the longest first, so that a launch of more blocks
+// than fit the card does not end on a long one. The number of blocks of at least
+// L tiles is a sum over the sequences, each a division; the L of item's block is
+// found by bisection, about 1 us.
 template <int BLOCK, int TILE>
 __device__ __forceinline__ bool packed_block_longest(const PackedSeqs &p, int G, int item, PackedBlock &b) {
   check_row_start(p.row_start, p.n_seq, p.n_rows, p.status);
   const int lane = threadIdx.x & 63;
-  int first = 0, rows = 0, past = 0;
-  if (lane < p.n_seq) {
-    first = p.row_start[lane];
-    const int end = p.row_start[lane + 1];
-    past = p.n_past ? p.n_past[lane] : 0;
-    if (first >= 0 && end >= first && end <= p.n_rows) rows = end - first;
-    if (past < 0 || past > p.capacity - rows) {
-      if (rows > 0 && blockIdx.x == 0 && threadIdx.x < 64) raise_status(p.status, IKV_STATUS_POSITION);
-      rows = past = 0;
-    }
-  }
+  const LaneSeq mine(p);
+  const int first = mine.first, rows = mine.rows, past = mine.past;
   const int blocks = (rows * G + BLOCK - 1) / BLOCK;
   // this sequence's blocks of L tiles or more: its last ones
   auto at_least = [&](int L) {
