@@ -94,11 +94,23 @@ int ikv_attn_prefill_packed_f32(const float *q, const float *k, const float *v,
  * keys 0 .. n_past[s] + t. The pools already hold the new tokens' rows
  * (ikv_append_packed_f32); rows behind a sequence's last token are not read. A
  * sequence that does not fit its table, or of a negative n_past, raises
- * IKV_STATUS_POSITION and its rows are not written. */
+ * IKV_STATUS_POSITION and its rows are not written.
+ *   workspace  NULL, or device memory, 16-byte aligned (else -EINVAL), for the
+ *            parts of sequences of few rows behind long histories, whose keys
+ *            are then split over several workgroups (a second launch joins the
+ *            parts). ikv_attn_prefill_packed_paged_workspace_bytes() says how
+ *            much is used for these sizes (max_tokens: table_stride *
+ *            block_tokens); 0, or less memory than that: nothing is split.
+ *            Nothing is expected in it or left in it. Launches that share it
+ *            must be ordered. */
+size_t ikv_attn_prefill_packed_paged_workspace_bytes(int64_t n_seq, int64_t n_rows,
+                                                     int64_t max_tokens, int n_head, int n_head_kv,
+                                                     int head_dim);
 int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_pool, const float *v_pool,
                                       const ikv_kv_batch *batch, const int32_t *row_start,
                                       const int32_t *n_past, int64_t n_rows, float *out, int n_head,
-                                      int n_head_kv, int head_dim, float scale, void *stream);
+                                      int n_head_kv, int head_dim, float scale, void *workspace,
+                                      size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------
  * Decode attention of one new token of each sequence over a paged cache, the

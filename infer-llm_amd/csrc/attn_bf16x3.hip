@@ -98,6 +98,35 @@ __device__ __forceinline__ void load_dims(__amdgpu_buffer_rsrc_t r, unsigned off
   }
 }
 
+// Packed prompts of few rows behind long histories: the keys of a block of rows in
+// up to seqs.parts parts, each a workgroup's. A part leaves its rows' sums and
+// maxima in the workspace, as the lanes hold them, and attn_join_kernel adds them
+// up. A block has as many parts as it holds times the load of a slot of the card
+// if all were equal, and kPartTiles: where the blocks fill the card, long ones are
+// split and the others are not.
+constexpr int kPartTiles = 8;
+constexpr int kMaxParts = 16;
+static_assert(kPartTiles % 4 == 0, "tiles of every key group");
+// (by the whole wave; up to kLaneSeqs sequences)
+template <int BLOCK>
+__device__ __forceinline__ int part_tiles(const ikv::PackedSeqs &seqs, int G, int n_head_kv, int tiles) {
+  if (seqs.parts == 1) return max(tiles, 1);
+  const ikv::LaneSeq mine(seqs);
+  const int blocks = (mine.rows * G + BLOCK - 1) / BLOCK;
+  const float all = ikv::wave_sum(blocks * ((mine.past + 0.5f * mine.rows) / BN + 0.5f));
+  const float load = fmaxf(all * n_head_kv / seqs.part_slots, kPartTiles);
+  // (whole times that only: a rest would start another round)
+  const int parts = min(max(static_cast<int>(tiles / load + 0.1f), 1), seqs.parts);
+  const int per = (tiles + parts - 1) / parts;
+  return __builtin_amdgcn_readfirstlane((per + 3) / 4 * 4);
+}
+template <int DT>
+constexpr int kPartFloats = (16 * DT + 3) * 64;  // of a wave: values, maximum, sum, whether on F32
+template <int DT, int RW>
+__device__ __forceinline__ float *part_of(float *space, int part, int slot) {
+  return space + (static_cast<size_t>(part) * RW + slot) * kPartFloats<DT>;
+}
+
 template <int DT, int RW, int KG, int MINW, bool PAGED, bool PACKED>
 __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
     const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
@@ -123,8 +152,16 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
   const int r32 = lane & 31, c2 = lane >> 5;
   const int n_head = n_head_kv * G;
   const int stride = n_head_kv * dim;  // floats of a token row
+  int part = 0, part_at = 0;  // PACKED: the part of the keys, and where its sums go
   if constexpr (PACKED) {  // one sequence's rows, cache and sizes from here on
     ikv::PackedBlock b;
+    // (all first parts before the second ones: workgroups go to the compute units
+    // in turn, and with a block's parts next to each other, of which only the first
+    // ones are there, some units had none: 341 us against 204)
+    const int blocks = gridDim.x / n_head_kv / seqs.parts;
+    part = item / blocks;
+    item %= blocks;
+    part_at = item * n_head_kv + g;
     if (!(seqs.longest_first ? ikv::packed_block_longest<BR, BN>(seqs, G, item, b)
                              : ikv::packed_block<BR>(seqs, G, item, b)))
       return;
@@ -223,17 +260,26 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
   const int tok = min(row, n_rows - 1) / G;
   const int head = g * G + min(row, n_rows - 1) % G;
   const int first_tok = min(row0, n_rows - 1) / G;
-  const int n_tiles =
-      (min(n_kv, n_past + (min((blk + 1) * BR, n_rows) - 1) / G + 1) + BN - 1) / BN;
-  const int n_it = (n_tiles + KG - 1) / KG;  // tiles kg, kg + KG, ... of each group
-  // (a tile past the end is masked whole; what is staged for it is the last one)
-  auto staged = [&](int i) { return min(kg + KG * i, n_tiles - 1); };
+  int n_tiles = (min(n_kv, n_past + (min((blk + 1) * BR, n_rows) - 1) / G + 1) + BN - 1) / BN;
+  int tile0 = 0;  // the first of this workgroup's tiles
+  bool whole = true;
+  if constexpr (PACKED) {
+    const int per = part_tiles<BR>(seqs, G, n_head_kv, n_tiles);
+    tile0 = part * per;
+    if (tile0 >= n_tiles) return;
+    whole = per >= n_tiles;
+    n_tiles = min(n_tiles, tile0 + per);
+  }
+  const int n_it = (n_tiles - tile0 + KG - 1) / KG;  // tiles kg, kg + KG, ... of each group
+  // (a tile past the end is masked whole; what is staged for it is the last one.
+  // Parts of the keys are multiples of KG tiles: none is past a part's end.)
+  auto staged = [&](int i) { return min(tile0 + kg + KG * i, n_tiles - 1); };
   // The staged tiles' rows, one after the other. A paged cache's next 64 block
   // table entries are held one per lane, checked as they are read, and tiles
   // and blocks are counted along: a look into the table, its check and a
   // division at every load cost 8 % (777 tokens behind 3319 of 32 heads over 8:
   // 319 us, here 298, contiguous 293).
-  int next = kg, blk_of = 0, in_blk = 0, last_blk = 0, last_in = 0, ent = 0, ent0 = 0;
+  int next = tile0 + kg, blk_of = 0, in_blk = 0, last_blk = 0, last_in = 0, ent = 0, ent0 = 0;
   const int per_blk = PAGED ? pages.bt / BN : 1;  // at least 2
   auto entries = [&](int b) {
     ent0 = b;
@@ -244,7 +290,7 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
     }
   };
   if constexpr (PAGED) {
-    blk_of = kg / per_blk, in_blk = kg % per_blk;
+    blk_of = next / per_blk, in_blk = next % per_blk;
     last_blk = (n_tiles - 1) / per_blk, last_in = (n_tiles - 1) % per_blk;
     entries(min(blk_of, last_blk));
   }
@@ -329,7 +375,7 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
     constexpr int P = decltype(par)::value;  // i & 1: the V buffers
     // S of tile i is in s0 + s1, K of tile i + 1 and V of tile i are staged,
     // K of tile i + 2 is on its way
-    const int kbase = (kg + KG * i) * BN;
+    const int kbase = (tile0 + kg + KG * i) * BN;
     float p[16];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -542,21 +588,28 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
   // the tiles that all its rows see whole and key by key over the rest, where
   // a row takes only the keys it sees (a masked key weighs 0, but 0 times an
   // infinite value is NaN)
+  // (a row may see no key of a part of them: its sums are then zeros)
+  if (!whole) inv = fabsf(l_part) < INFINITY ? 1.0f : NAN;
   bool odd = s_lost != 0 || !(fabsf(inv) < INFINITY);
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd |= !(fabsf(o[t][e] * inv) < INFINITY);
-  if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+  const bool redone = __builtin_amdgcn_ballot_w64(odd) != 0;
+  if (redone) {
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = floatx16{};
     m_row = -INFINITY;
     l_part = 0.f;
     const float *qr = q + (static_cast<size_t>(tok) * n_head + head) * dim;
     const int last_tok = min(row0 + 31, n_rows - 1) / G;
-    const int my_end = min(n_kv, n_past + last_tok + 1);
-    const int full = min(n_kv, n_past + first_tok + 1) / BN;  // tiles that every row sees whole
-    for (int tile = 0; tile < full; ++tile) {
+    int my_end = min(n_kv, n_past + last_tok + 1);
+    int full = min(n_kv, n_past + first_tok + 1) / BN;  // tiles that every row sees whole
+    if constexpr (PACKED) {
+      my_end = min(my_end, n_tiles * BN);
+      full = max(min(full, n_tiles), tile0);
+    }
+    for (int tile = tile0; tile < full; ++tile) {
       int first = tile * BN;
       if constexpr (PAGED) first += static_cast<int>(ikv::page_shift(pages, first));
       const auto rk = tile_rsrc(k, tile, first);
@@ -634,6 +687,19 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
     }
     inv = 1.0f / pair_sum(l_part);
   }
+  if constexpr (PACKED) {
+    if (!whole) {
+      float *const x = part_of<DT, RW>(seqs.space, part_at * seqs.parts + part, slot) + lane;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[(16 * t + e) * 64] = o[t][e];
+      x[16 * DT * 64] = m_row;
+      x[(16 * DT + 1) * 64] = l_part;
+      x[(16 * DT + 2) * 64] = redone ? 1.f : 0.f;
+      return;
+    }
+  }
   if (row_ok) {
     float *orow = out + (static_cast<size_t>(tok) * n_head + head) * dim;
 #pragma unroll
@@ -645,6 +711,80 @@ __global__ __launch_bounds__(RW * KG * 64, MINW) void attn_bf16x3_kernel(
           *reinterpret_cast<floatx4 *>(orow + d) =
               floatx4{o[t][4 * z], o[t][4 * z + 1], o[t][4 * z + 2], o[t][4 * z + 3]} * inv;
       }
+  }
+}
+
+// Joins the parts of each block of rows that has more than one. A wave takes 32
+// dims of the rows that a wave holds above, a lane the values that it holds there;
+// all parts' maxima, then four parts' values are loaded at once.
+template <int DT, int RW>
+__global__ __launch_bounds__(RW *DT * 64) void attn_join_kernel(float *__restrict__ out, int n_head_kv, int G,
+                                                                int dim, ikv::PackedSeqs seqs) {
+  constexpr int BR = 32 * RW;
+  const int g = blockIdx.x % n_head_kv, item = blockIdx.x / n_head_kv;
+  const int lane = threadIdx.x & 63, t = (threadIdx.x >> 6) % DT, slot = threadIdx.x / (64 * DT);
+  const int r32 = lane & 31, c2 = lane >> 5;
+  ikv::PackedBlock b;
+  if (!(seqs.longest_first ? ikv::packed_block_longest<BR, BN>(seqs, G, item, b)
+                           : ikv::packed_block<BR>(seqs, G, item, b)))
+    return;
+  const int n_rows = b.rows * G, blk = b.n_blocks - 1 - b.item;
+  const int n_tiles = (b.past + (min((blk + 1) * BR, n_rows) - 1) / G + 1 + BN - 1) / BN;
+  const int per = part_tiles<BR>(seqs, G, n_head_kv, n_tiles), n = (n_tiles + per - 1) / per;
+  if (n == 1) return;
+  constexpr int kNext = RW * kPartFloats<DT>;
+  const float *const x = part_of<DT, RW>(seqs.space, blockIdx.x * seqs.parts, slot) + lane;
+  float m[kMaxParts], l[kMaxParts], on_f32[kMaxParts], f[kMaxParts];
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) {
+    m[i] = -INFINITY;
+    l[i] = on_f32[i] = 0.f;
+    if (i < n) {
+      m[i] = x[i * kNext + 16 * DT * 64];
+      l[i] = x[i * kNext + (16 * DT + 1) * 64];
+      on_f32[i] = x[i * kNext + (16 * DT + 2) * 64];
+    }
+  }
+  float top = -INFINITY, any = 0.f, all = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) {
+    top = fmaxf(top, m[i]);
+    any = fmaxf(any, on_f32[i]);
+  }
+  // the pieces' sums have a factor of kProbScale, those that were redone on F32
+  // have not: where there are both, the former lose it
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) {
+    f[i] = m[i] == -INFINITY ? 0.f : ikv::fast_exp2(m[i] - top);
+    if (any != on_f32[i]) f[i] *= 1.0f / kProbScale;
+    if (i < n) all = fmaf(f[i], l[i], all);
+  }
+  floatx16 o{};
+#pragma unroll
+  for (int i0 = 0; i0 < kMaxParts; i0 += 4) {
+    if (i0 >= n) break;
+    floatx16 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[i][e] = x[min(i0 + i, n - 1) * kNext + (16 * t + e) * 64];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i0 + i >= n) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = fmaf(f[i0 + i], v[i][e], o[e]);
+    }
+  }
+  const int row = blk * BR + slot * 32 + r32;
+  const float inv = 1.0f / pair_sum(all);
+  if (row >= n_rows) return;
+  const int n_head = n_head_kv * G;
+  float *orow = out + (static_cast<size_t>(b.first + row / G) * n_head + g * G + row % G) * dim;
+#pragma unroll
+  for (int z = 0; z < 4; ++z) {
+    const int d = 32 * t + 8 * z + 4 * c2;
+    if (d < dim)
+      *reinterpret_cast<floatx4 *>(orow + d) = floatx4{o[4 * z], o[4 * z + 1], o[4 * z + 2], o[4 * z + 3]} * inv;
   }
 }
 
@@ -665,7 +805,8 @@ void launch(const float *q, const float *k, const float *v, float *out, int n_he
 template <int DT, int RW, int KG, int MINW>
 void launch_packed(const float *q, const float *k, const float *v, float *out, int n_head_kv, int G,
                    int dim, float sl2, const ikv::Pages *pg, ikv::PackedSeqs seqs, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(ikv::packed_blocks(seqs.n_rows, seqs.n_seq, G, 32 * RW) * n_head_kv);
+  const unsigned blocks = static_cast<unsigned>(ikv::packed_blocks(seqs.n_rows, seqs.n_seq, G, 32 * RW) * n_head_kv);
+  const unsigned grid = blocks * seqs.parts;
   // (where all blocks start at once their order does not matter)
   seqs.longest_first = seqs.n_seq <= ikv::kLaneSeqs && grid > MINW * kCUs;
   if (pg)
@@ -674,6 +815,7 @@ void launch_packed(const float *q, const float *k, const float *v, float *out, i
   else
     attn_bf16x3_kernel<DT, RW, KG, MINW, false, true><<<grid, RW * KG * 64, 0, s>>>(
         q, k, v, out, n_head_kv, G, dim, 0, 0, 0, 0, sl2, ikv::Pages{}, seqs);
+  if (seqs.parts > 1) attn_join_kernel<DT, RW><<<blocks, RW * DT * 64, 0, s>>>(out, n_head_kv, G, dim, seqs);
 }
 
 }  // namespace
@@ -713,12 +855,25 @@ double time_of(const Form &f, int64_t rows, int G, int64_t n_kv, int64_t n_past,
 // 24-fold, half of them behind 0 to 4000 keys, that is on average 4% (5% with
 // histories) from the better form of two; the larger form always, 11% (15%) with
 // heads of 128 and 5% (9%) with heads of 64.
-double time_of_packed(const Form &f, double rows, double n_seq, bool histories, int G, int heads) {
+// With parts, they share the longest one's steps, down to kPartTiles, and each has
+// its own ends.
+double time_of_packed(const Form &f, double rows, double n_seq, bool histories, int G, int heads, int parts) {
   const double mean = rows / n_seq, seen = histories ? 256 : 0;
   const double steps = ((std::ceil(mean / BN) + 1) / 2 + seen / BN) / f.groups + f.ends;
-  const double longest = std::ceil((std::min(rows, 1.5 * mean) + seen) / BN / f.groups) + f.ends;
-  const double load = n_seq * heads * std::ceil(mean * G / f.rows) * steps;
-  return f.fixed + std::max(f.alone * longest, f.busy * load / f.slots);
+  double longest = std::ceil((std::min(rows, 1.5 * mean) + seen) / BN / f.groups / parts);
+  if (parts > 1) longest = std::max<double>(longest, kPartTiles / f.groups);
+  const double load = n_seq * heads * std::ceil(mean * G / f.rows) * (steps + (parts - 1) * f.ends);
+  return f.fixed + std::max(f.alone * (longest + f.ends), f.busy * load / f.slots);
+}
+
+// Parts of a block's keys, at most: twice the workgroups that fit the card; one
+// where all blocks of sequences of equal lengths would not fit it, or a sequence
+// cannot have kPartTiles twice. A workgroup whose part is empty leaves at once.
+int parts_of(const Form &f, int64_t n_rows, int64_t n_seq, int64_t capacity, int G, int heads) {
+  if (capacity <= 2 * kPartTiles * BN || n_seq > ikv::kLaneSeqs) return 1;
+  const double mean = static_cast<double>(n_rows) / n_seq;
+  const double blocks = n_seq * heads * std::ceil(mean * G / f.rows);
+  return blocks > f.slots ? 1 : static_cast<int>(std::min<double>(std::ceil(2.0 * f.slots / blocks), kMaxParts));
 }
 
 // heads of 128: 128 rows and one key group, or 64 and two; heads of 64: 64 rows
@@ -771,25 +926,58 @@ int attn_bf16x3(const float *q, const float *k, const float *v, const Pages *pag
   return launch_status();
 }
 
+namespace {
+
+// The form of a launch, its parts, and the workspace that these need.
+struct PackedPlan {
+  int form, parts;
+  size_t bytes;
+};
+PackedPlan packed_plan(int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, bool split) {
+  const int G = n_head / n_head_kv;
+  PackedPlan best{};
+  double least = 0;
+  for (int i = 0; i < 2; ++i) {
+    const Form &f = head_dim > 64 ? kForms128[i] : kForms64[i];
+    const int parts = split ? parts_of(f, seqs.n_rows, seqs.n_seq, seqs.capacity, G, n_head_kv) : 1;
+    const double us = time_of_packed(f, seqs.n_rows, seqs.n_seq, seqs.n_past != nullptr, G, n_head_kv, parts);
+    if (i > 0 && us >= least) continue;
+    least = us;
+    const size_t lanes = sizeof(float) * (head_dim > 64 ? kPartFloats<4> : kPartFloats<2>);
+    best = {i, parts,
+            parts > 1 ? packed_blocks(seqs.n_rows, seqs.n_seq, G, f.rows) * n_head_kv * parts * (f.rows / 32) * lanes : 0};
+  }
+  return best;
+}
+
+}  // namespace
+
+size_t attn_bf16x3_packed_bytes(int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs) {
+  return packed_plan(n_head, n_head_kv, head_dim, seqs, true).bytes;
+}
+
 int attn_bf16x3_packed(const float *q, const float *k, const float *v, const Pages *pages, float *out,
-                       int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, float scale,
-                       hipStream_t s) {
+                       int n_head, int n_head_kv, int head_dim, PackedSeqs seqs, float scale,
+                       size_t space_bytes, hipStream_t s) {
   const int G = n_head / n_head_kv;
   if (!attn_bf16x3_supported(q, k, v, out, n_head, n_head_kv, head_dim, seqs.n_rows + seqs.n_seq,
                              seqs.capacity, 0))
     return -ENOTSUP;
-  if (packed_blocks(seqs.n_rows, seqs.n_seq, G, 32) * n_head_kv > INT_MAX) return -EOVERFLOW;
+  if (packed_blocks(seqs.n_rows, seqs.n_seq, G, 32) * n_head_kv > INT_MAX / kMaxParts) return -EOVERFLOW;
   if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   const float sl2 = scale * kLog2e;
-  auto us = [&](const Form &f) { return time_of_packed(f, seqs.n_rows, seqs.n_seq, seqs.n_past != nullptr, G, n_head_kv); };
+  PackedPlan plan = packed_plan(n_head, n_head_kv, head_dim, seqs, seqs.space != nullptr);
+  if (plan.bytes > space_bytes) plan = packed_plan(n_head, n_head_kv, head_dim, seqs, false);
+  seqs.parts = plan.parts;
+  seqs.part_slots = (head_dim > 64 ? kForms128[plan.form] : kForms64[plan.form]).slots;
 #define IKV_A3(...) launch_packed<__VA_ARGS__>(q, k, v, out, n_head_kv, G, head_dim, sl2, pages, seqs, s)
   if (head_dim > 64) {
-    if (us(kForms128[0]) <= us(kForms128[1]))
+    if (plan.form == 0)
       IKV_A3(4, 4, 1, 1);
     else
       IKV_A3(4, 2, 2, 1);
   } else {
-    if (us(kForms64[0]) <= us(kForms64[1]))
+    if (plan.form == 0)
       IKV_A3(2, 2, 2, 2);
     else
       IKV_A3(2, 1, 4, 1);

@@ -24,9 +24,13 @@ int attn_bf16x3(const float *q, const float *k, const float *v, const Pages *pag
 
 // Packed prompts (batch.hpp): k and v packed as q is, or, with pages, pools
 // read through the table of each sequence (pages->table: the first one's).
-// n_rows > 0 and n_seq > 0. -ENOTSUP for what attn_bf16x3_supported refuses.
+// n_rows > 0 and n_seq > 0. seqs.space: NULL, or space_bytes of 16-byte aligned
+// workspace for the parts of blocks whose keys are split (they are not where it
+// is too small). -ENOTSUP for what attn_bf16x3_supported refuses.
 int attn_bf16x3_packed(const float *q, const float *k, const float *v, const Pages *pages, float *out,
-                       int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs, float scale,
-                       hipStream_t s);
+                       int n_head, int n_head_kv, int head_dim, PackedSeqs seqs, float scale,
+                       size_t space_bytes, hipStream_t s);
+// The workspace with which it splits as it would; 0: it does not.
+size_t attn_bf16x3_packed_bytes(int n_head, int n_head_kv, int head_dim, const PackedSeqs &seqs);
 
 }  // namespace ikv

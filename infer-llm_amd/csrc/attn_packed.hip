@@ -13,7 +13,7 @@ namespace {
 
 int prefill_packed(const float *q, const float *k, const float *v, const ikv::Pages *pages,
                    ikv::PackedSeqs seqs, int64_t n_rows, float *out, int n_head, int n_head_kv,
-                   int head_dim, float scale, void *stream) {
+                   int head_dim, float scale, size_t space_bytes, void *stream) {
   if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || n_rows < 0) return -EINVAL;
   if (!ikv::generic_attn_shape(n_head, n_head_kv, head_dim)) return -ENOTSUP;
   if (n_rows == 0 || seqs.n_seq == 0) return 0;
@@ -21,7 +21,8 @@ int prefill_packed(const float *q, const float *k, const float *v, const ikv::Pa
   if (n_rows > INT_MAX / 8 / n_head) return -EOVERFLOW;
   seqs.n_rows = static_cast<int>(n_rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rc = ikv::attn_bf16x3_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale, s);
+  const int rc = ikv::attn_bf16x3_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale,
+                                          space_bytes, s);
   if (rc != -ENOTSUP) return rc;
   return ikv::attn_generic_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale, s);
 }
@@ -39,14 +40,14 @@ extern "C" int ikv_attn_prefill_packed_f32(const float *q, const float *k, const
   seqs.n_seq = static_cast<int>(n_seq);
   seqs.capacity = static_cast<int>(ikv::kMaxSeqTokens) - 1;
   seqs.status = status;
-  return prefill_packed(q, k, v, nullptr, seqs, n_rows, out, n_head, n_head_kv, head_dim, scale, stream);
+  return prefill_packed(q, k, v, nullptr, seqs, n_rows, out, n_head, n_head_kv, head_dim, scale, 0, stream);
 }
 
 extern "C" int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_pool, const float *v_pool,
                                                  const ikv_kv_batch *batch, const int32_t *row_start,
                                                  const int32_t *n_past, int64_t n_rows, float *out,
                                                  int n_head, int n_head_kv, int head_dim, float scale,
-                                                 void *stream) {
+                                                 void *workspace, size_t workspace_bytes, void *stream) {
   ikv::BatchPages b;
   if (const int rc = ikv::batch_arg(batch, b)) return rc;
   ikv::PackedSeqs seqs;
@@ -56,7 +57,23 @@ extern "C" int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_
   seqs.capacity = b.capacity;
   seqs.stride = b.stride;
   seqs.status = b.status;
+  if (workspace && !ikv::aligned16(workspace)) return -EINVAL;
+  seqs.space = static_cast<float *>(workspace);
   const ikv::Pages pages{b.tables, b.bt, b.n_blocks, b.status};
   return prefill_packed(q, k_pool, v_pool, &pages, seqs, n_rows, out, n_head, n_head_kv, head_dim, scale,
-                        stream);
+                        workspace ? workspace_bytes : 0, stream);
+}
+
+extern "C" size_t ikv_attn_prefill_packed_paged_workspace_bytes(int64_t n_seq, int64_t n_rows, int64_t max_tokens,
+                                                                int n_head, int n_head_kv, int head_dim) {
+  if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || n_seq <= 0 || n_seq > ikv::kMaxSeqs ||
+      n_rows <= 0 || n_rows > INT_MAX / 8 / n_head || max_tokens <= 0 || max_tokens > ikv::kMaxSeqTokens ||
+      head_dim <= 0 || head_dim > 128 || head_dim % 4 != 0)
+    return 0;
+  ikv::PackedSeqs seqs;
+  seqs.n_past = reinterpret_cast<const int32_t *>(16);  // (histories; not read)
+  seqs.n_seq = static_cast<int>(n_seq);
+  seqs.n_rows = static_cast<int>(n_rows);
+  seqs.capacity = static_cast<int>(max_tokens);
+  return ikv::attn_bf16x3_packed_bytes(n_head, n_head_kv, head_dim, seqs);
 }

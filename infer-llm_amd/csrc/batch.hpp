@@ -87,6 +87,9 @@ struct PackedSeqs {
   int64_t stride = 0;  // block table entries per sequence
   int *status = nullptr;
   bool longest_first = false;  // the blocks' order (packed_block_longest)
+  int parts = 1;               // of a block's keys, at most (attn_bf16x3.hip),
+  int part_slots = 0;          // and the workgroups that fit the card
+  float *space = nullptr;      // the parts' sums
 };
 
 // One block of `block` query rows (row = token * G + query head of the group)

@@ -146,8 +146,10 @@ SIGNATURES = {
     "ikv_attn_prefill_packed_paged_f32": (
         _c_int,
         [_c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_int64, _c_void_p,
-         _c_int, _c_int, _c_int, _c_float, _c_void_p],
+         _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_size_t, _c_void_p],
     ),
+    "ikv_attn_prefill_packed_paged_workspace_bytes": (
+        _c_size_t, [_c_int64, _c_int64, _c_int64, _c_int, _c_int, _c_int]),
     "ikv_attn_decode_batch_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
     "ikv_attn_decode_batch_f32": (
         _c_int,
@@ -704,16 +706,28 @@ def attn_prefill_packed(q, k, v, row_start, *, out=None, scale: float = 0.0, sta
     return out
 
 
+def prefill_packed_workspace(n_seq: int, n_rows: int, max_tokens: int, n_head: int, n_head_kv: int,
+                             head_dim: int, device="cuda"):
+    """Workspace of attn_prefill_packed_paged for these sizes (max_tokens: what a
+    table covers), or None where it uses none."""
+    torch = _torch()
+    nbytes = int(load().ikv_attn_prefill_packed_paged_workspace_bytes(n_seq, n_rows, max_tokens, n_head,
+                                                                      n_head_kv, head_dim))
+    return torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device) if nbytes else None
+
+
 def attn_prefill_packed_paged(q, k_pool, v_pool, tables, block_tokens: int, row_start, n_past=None,
-                              *, out=None, scale: float = 0.0, status=None, stream=None):
+                              *, out=None, scale: float = 0.0, status=None, workspace=None, stream=None):
     """attn_prefill_packed over paged pools that hold the new rows already, each
-    sequence's queries behind n_past[s] cached tokens (none without it)."""
+    sequence's queries behind n_past[s] cached tokens (none without it). Without
+    `workspace` (prefill_packed_workspace) one is allocated where it is used."""
     torch = _torch()
     dev = q.device
-    _operands(dev, (q, k_pool, v_pool, out), "q k_pool v_pool out",
+    _operands(dev, (q, k_pool, v_pool, out, workspace), "q k_pool v_pool out workspace",
               (tables, row_start, n_past, status), "tables row_start n_past status")
     n_rows, n_head, D = q.shape
-    _need_pools(k_pool, v_pool, k_pool.shape[-2], D)
+    n_head_kv = k_pool.shape[-2]
+    _need_pools(k_pool, v_pool, n_head_kv, D)
     bt = kv_batch(tables, block_tokens, k_pool, status)
     if row_start.numel() != bt.n_seq + 1:
         raise ValueError("row_start must hold n_seq + 1 rows")
@@ -724,10 +738,14 @@ def attn_prefill_packed_paged(q, k_pool, v_pool, tables, block_tokens: int, row_
     with _on(dev, stream):
         if out is None:
             out = torch.empty_like(q)
+        if workspace is None and n_past is not None:
+            workspace = prefill_packed_workspace(bt.n_seq, n_rows, bt.table_stride * block_tokens, n_head,
+                                                 n_head_kv, D, device=dev)
         _check("ikv_attn_prefill_packed_paged_f32",
                load().ikv_attn_prefill_packed_paged_f32(
                    _ptr(q), _ptr(k_pool), _ptr(v_pool), ctypes.byref(bt), _ptr(row_start),
-                   _ptr(n_past), n_rows, _ptr(out), n_head, k_pool.shape[1], D, scale, _stream()))
+                   _ptr(n_past), n_rows, _ptr(out), n_head, n_head_kv, D, scale, _ptr(workspace),
+                   0 if workspace is None else workspace.numel() * 4, _stream()))
     return out
 
 

@@ -57,10 +57,10 @@ def _packed(q=P, k=P, v=P, start=P, n_seq=3, n=10, out=P, n_head=16, n_head_kv=8
 
 
 def _packed_paged(q=P, k=P, v=P, batch="ok", start=P, past=None, n=10, out=P, n_head=16, n_head_kv=8,
-                  dim=128):
+                  dim=128, ws=None, wsb=0):
     b = _batch() if batch == "ok" else batch
     return ikv.load().ikv_attn_prefill_packed_paged_f32(q, k, v, b, start, past, n, out, n_head,
-                                                        n_head_kv, dim, 0.0, None)
+                                                        n_head_kv, dim, 0.0, ws, wsb, None)
 
 
 @pytest.mark.parametrize("batch,code", BAD_BATCHES)
@@ -85,6 +85,19 @@ def test_packed_prefill_refuses_bad_arguments(call):
         assert call(n_seq=(1 << 20) + 1) == -errno.EOVERFLOW
         assert call(n_seq=1 << 20, n=1, n_head=4096, n_head_kv=4096) == -errno.EOVERFLOW  # 2^32 blocks
         assert call(n_seq=0) == 0
+    else:
+        assert call(ws=P + 4, wsb=1 << 30) == -errno.EINVAL
+        assert call(n=1, batch=_batch(n_seq=1 << 20, stride=1), n_head=4096, n_head_kv=4096) == -errno.EOVERFLOW
+
+
+def test_packed_prefill_workspace():
+    size = ikv.load().ikv_attn_prefill_packed_paged_workspace_bytes
+    assert size(1, 16, 4096, 16, 8, 128) > 0            # few rows, perhaps behind many keys
+    assert size(1, 16, 512, 16, 8, 128) == 0            # a table of two parts' keys
+    assert size(8, 1 << 16, 1 << 16, 32, 8, 128) == 0   # blocks enough for the card
+    assert size(1, 16, 4096, 16, 8, 200) == 0           # the generic kernel's
+    assert size(0, 16, 4096, 16, 8, 128) == 0 and size(1, 0, 4096, 16, 8, 128) == 0
+    assert size(1, 16, 4096, 12, 8, 128) == 0 and size(1, 16, 1 << 29, 16, 8, 128) == 0
 
 
 def _decode(q=P, kp=P, vp=P, batch="ok", n_kv=P, kn=P, vn=P, out=P, n_head=16, n_head_kv=8, dim=128,

@@ -83,6 +83,61 @@ def test_packed_prompts_on_pages(dev, heads, kv, dim, rows, past, bt):
         at += r
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(16, 8, 128), (2, 1, 128), (12, 4, 64), (8, 1, 80), (1, 1, 32)])
+@pytest.mark.parametrize("rows,past", [([1], [3000]), ([64], [1000]), ([5, 1, 0, 33], [2000, 10, 5, 511]),
+                                       ([70, 300], [257, 0]), ([2] * 9, [700 + 31 * i for i in range(9)])])
+def test_few_rows_behind_long_histories(dev, heads, kv, dim, rows, past):
+    """Keys split over workgroups, joined; and the same without a workspace."""
+    bt = 64
+    q, pools, tables, own = _paged(dev, 9 + sum(past) + dim, rows, past, bt, heads, kv, dim)
+    args = (q, *pools, _dev32(tables, dev), bt, _dev32(starts(rows), dev), _dev32(past, dev))
+    need = ikv.load().ikv_attn_prefill_packed_paged_workspace_bytes(
+        len(rows), sum(rows), tables.shape[1] * bt, heads, kv, dim)
+    assert (need > 0) == (tables.shape[1] * bt > 512)  # a table of less than two parts' keys: none
+    ws = torch.full(((need + 3) // 4,), float("nan"), device=dev)
+    split = ikv.attn_prefill_packed_paged(*args, workspace=ws)
+    again = ikv.attn_prefill_packed_paged(*args)
+    assert torch.equal(split, again)
+    small = ikv.attn_prefill_packed_paged(*args, workspace=ws[:4].contiguous())
+    for out in (split, small):
+        at = 0
+        for r, p, (k, v) in zip(rows, past, own):
+            if r:
+                qs = q[at:at + r]
+                assert_near(out[at:at + r], attention64(qs, k, v, p), attention_bound(qs, k, v))
+            at += r
+
+
+def test_split_keys_that_the_pieces_do_not_carry(dev):
+    """Infinite, NaN and tiny values in one part of the keys: only the rows that
+    see them have them, and the tiny ones keep their bits."""
+    heads, kv, dim, rows, past = 2, 1, 128, [40], [1500]
+    q, pools, tables, own = _paged(dev, 83, rows, past, 64, heads, kv, dim)
+    k, v = own[0]
+    args = (q, *pools, _dev32(tables, dev), 64, _dev32([0, 40], dev), _dev32(past, dev))
+    clean = ikv.attn_prefill_packed_paged(*args)
+
+    def put(pool, token, value, d=slice(None)):
+        pool[rows_of(tables, 0, 64, [token])[0], :, d] = value
+
+    put(pools[1], 1520, float("inf"), 3)  # seen from row 20 on
+    out = ikv.attn_prefill_packed_paged(*args)
+    assert_near(out[:20], clean[:20].cpu().double(), 2 * attention_bound(q, k, v), 2 * NORMAL_REL)
+    assert torch.isinf(out[20:, :, 3]).all() and torch.isfinite(out[20:, :, 4:]).all()
+    put(pools[1], 1520, 0.0, 3)
+    put(pools[0], 700, float("nan"))      # an early part: seen by all
+    assert torch.isnan(ikv.attn_prefill_packed_paged(*args)).all()
+    put(pools[0], 700, 0.0)
+    k[700] = 0
+    pools[1][:, :, 7] = pools[1][:, :, 7] * 1e-36  # a dim of tiny values
+    v[:, :, 7] *= 1e-36
+    v[1520, :, 3] = 0
+    out = ikv.attn_prefill_packed_paged(*args)
+    want = attention64(q, k, v, 1500)
+    assert_near(out, want, attention_bound(q, k, v))
+    assert_near(out[:, :, 7] * 1e36, want[:, :, 7] * 1e36, attention_bound(q, k, v[:, :, 7:8] * 1e36))
+
+
 def test_packed_prompts_of_every_size_class(dev):
     """Few rows and many take different forms of the kernel."""
     for heads, kv, dim, n in ((16, 8, 128, 500), (16, 8, 128, 4200), (32, 8, 64, 400), (32, 8, 64, 3000)):
