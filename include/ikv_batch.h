@@ -82,7 +82,7 @@ int ikv_append_packed_f32(void *k_pool, void *v_pool, const void *k_rows, const 
  * grouping, scale and results as for ikv_attn_prefill_f32 (any head_dim up to
  * 512, any n_head that n_head_kv divides; else -ENOTSUP / -EINVAL; no
  * workspace), any alignment of 4 bytes. status: device int, or NULL.
- * -EOVERFLOW: n_rows * n_head past 2^28, or too many blocks for one launch.
+ * -EOVERFLOW: n_rows * n_head past 2^27, or too many blocks for one launch.
  * ------------------------------------------------------------------- */
 int ikv_attn_prefill_packed_f32(const float *q, const float *k, const float *v,
                                 const int32_t *row_start, int64_t n_seq, int64_t n_rows, float *out,

@@ -110,6 +110,7 @@ static_assert(kPartTiles % 4 == 0, "tiles of every key group");
 // (by the whole wave; up to kLaneSeqs sequences)
 template <int BLOCK>
 __device__ __forceinline__ int part_tiles(const ikv::PackedSeqs &seqs, int G, int n_head_kv, int tiles) {
+#pragma clang fp contract(off)  // (the same number in both kernels)
   if (seqs.parts == 1) return max(tiles, 1);
   const ikv::LaneSeq mine(seqs);
   const int blocks = (mine.rows * G + BLOCK - 1) / BLOCK;
@@ -963,7 +964,7 @@ int attn_bf16x3_packed(const float *q, const float *k, const float *v, const Pag
   if (!attn_bf16x3_supported(q, k, v, out, n_head, n_head_kv, head_dim, seqs.n_rows + seqs.n_seq,
                              seqs.capacity, 0))
     return -ENOTSUP;
-  if (packed_blocks(seqs.n_rows, seqs.n_seq, G, 32) * n_head_kv > INT_MAX / kMaxParts) return -EOVERFLOW;
+  if (packed_blocks(seqs.n_rows, seqs.n_seq, G, 32) * n_head_kv > kMaxWorkgroups) return -EOVERFLOW;
   if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   const float sl2 = scale * kLog2e;
   PackedPlan plan = packed_plan(n_head, n_head_kv, head_dim, seqs, seqs.space != nullptr);

@@ -751,9 +751,8 @@ int attn_generic_packed(const float *q, const float *k, const float *v, const Pa
                         hipStream_t s) {
   if (!generic_attn_shape(n_head, n_head_kv, head_dim)) return -ENOTSUP;
   const int G = n_head / n_head_kv;
-  if (seqs.n_rows > INT_MAX / 4 / n_head) return -EOVERFLOW;
   const int64_t blocks = packed_blocks(seqs.n_rows, seqs.n_seq, G, kTileRows);
-  if (blocks * n_head_kv > INT_MAX) return -EOVERFLOW;
+  if (blocks * n_head_kv > kMaxWorkgroups) return -EOVERFLOW;
   if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   const unsigned grid = static_cast<unsigned>(blocks * n_head_kv);
   const float sl2 = scale * kLog2e;

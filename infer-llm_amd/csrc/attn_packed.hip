@@ -18,7 +18,7 @@ int prefill_packed(const float *q, const float *k, const float *v, const ikv::Pa
   if (!ikv::generic_attn_shape(n_head, n_head_kv, head_dim)) return -ENOTSUP;
   if (n_rows == 0 || seqs.n_seq == 0) return 0;
   if (!q || !k || !v || !out || !seqs.row_start) return -EINVAL;
-  if (n_rows > INT_MAX / 8 / n_head) return -EOVERFLOW;
+  if (n_rows > INT_MAX / 16 / n_head) return -EOVERFLOW;
   seqs.n_rows = static_cast<int>(n_rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rc = ikv::attn_bf16x3_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale,
@@ -67,7 +67,7 @@ extern "C" int ikv_attn_prefill_packed_paged_f32(const float *q, const float *k_
 extern "C" size_t ikv_attn_prefill_packed_paged_workspace_bytes(int64_t n_seq, int64_t n_rows, int64_t max_tokens,
                                                                 int n_head, int n_head_kv, int head_dim) {
   if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || n_seq <= 0 || n_seq > ikv::kMaxSeqs ||
-      n_rows <= 0 || n_rows > INT_MAX / 8 / n_head || max_tokens <= 0 || max_tokens > ikv::kMaxSeqTokens ||
+      n_rows <= 0 || n_rows > INT_MAX / 16 / n_head || max_tokens <= 0 || max_tokens > ikv::kMaxSeqTokens ||
       head_dim <= 0 || head_dim > 128 || head_dim % 4 != 0)
     return 0;
   ikv::PackedSeqs seqs;

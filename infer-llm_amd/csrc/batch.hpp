@@ -13,6 +13,7 @@
 namespace ikv {
 
 constexpr int64_t kMaxSeqs = 1 << 20;       // n_seq
+constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;  // of 256 threads: 2^32 in a launch
 constexpr int64_t kMaxSeqTokens = 1 << 28;  // tokens of one sequence
 
 // Block tables of several sequences (ikv_kv_batch).
