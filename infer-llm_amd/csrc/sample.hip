@@ -21,6 +21,13 @@
 // selection in one workgroup instead: 11 bits of a value's place in the order a
 // round, three rounds to one value, whose tokens weigh the same, so that what is
 // left is a division.
+//
+// Measured (MI355X, us): one row of 151936 25 (three launches of 4, 13 and 10: each
+// a chain of loads, sums over the workgroup and atomics of 1 us; the row itself is
+// read in 0.1), 48 rows 50 (8, 22, 18: the weights in double, LDS atomics at 25
+// cycles a wave, and the last workgroup's sums), 200 rows of 8191, each held in one
+// workgroup's registers, 17. All logits equal, 151936 of them, with top_p: 425 (one
+// workgroup goes over the row nine times), 48 such rows 650.
 #include "../../include/ikv_model.h"
 #include "ikv_common.hpp"
 
@@ -132,6 +139,96 @@ __device__ unsigned long long block_prefix(unsigned long long v, unsigned long l
   return v;
 }
 
+// The tokens of a workgroup: x[begin, end), read anew at each pass, eight loads of
+// a thread in flight.
+struct Chunked {
+  const float *x;
+  int begin, end;
+  // f(logit, index, g(logit)): g of eight tokens side by side, then f of each
+  template <class G, class F>
+  __device__ __forceinline__ void each(G &&g, F &&f) const {
+    constexpr int kAhead = 8;
+    for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kAhead * kThreads) {
+      float v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) v[j] = i + j * kThreads < end ? x[i + j * kThreads] : 0.0f;
+      decltype(g(0.0f)) y[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) y[j] = g(v[j]);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i + j * kThreads < end) f(v[j], i + j * kThreads, y[j]);
+    }
+  }
+};
+
+// Up to N * kThreads tokens, kept in registers.
+template <int N>
+struct Held {
+  float v[N];
+  int n;
+  __device__ Held(const float *x, int n) : n(n) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      v[j] = i < n ? x[i] : 0.0f;
+    }
+  }
+  template <class G, class F>
+  __device__ __forceinline__ void each(G &&g, F &&f) const {
+#pragma unroll
+    for (int j0 = 0; j0 < N; j0 += 8) {
+      decltype(g(0.0f)) y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = g(v[j0 + j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = threadIdx.x + (j0 + j) * kThreads;
+        if (i < n) f(v[j0 + j], i, y[j]);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ Chunked tokens_of(const Row &row) { return {row.x, 0, row.n}; }
+
+// Tokens one by one for rows of equal logits by the thousand: a weight is computed
+// where a logit differs from the thread's last one, and a thread's tokens of one
+// bin that come one behind the other go there together (an atomic of 64 lanes at
+// one address takes 64 turns). One row of 151936 equal ones 1650 to 425 us; for
+// other rows it costs more than it gives (48 of them 49 to 59 us in fill_bins).
+struct Run {
+  unsigned long long *mass;
+  unsigned *count;
+  float x = NAN;
+  unsigned long long each = 0;  // x's weight
+  int bin = 0;
+  unsigned n = 0;
+  unsigned long long w = 0;
+  __device__ __forceinline__ unsigned long long weight(const Row &row, float v) {
+    if (v != x) {
+      x = v;
+      each = row.weight(v);
+    }
+    return each;
+  }
+  __device__ __forceinline__ void flush() {
+    if (n == 0) return;
+    atomicAdd(&mass[bin], w);
+    atomicAdd(&count[bin], n);
+  }
+  __device__ __forceinline__ void add(const Row &row, int b, float v) {
+    if (b != bin) {
+      flush();
+      bin = b;
+      n = 0;
+      w = 0;
+    }
+    ++n;
+    w += weight(row, v);
+  }
+};
+
 struct Shared {
   unsigned count[kBins];
   unsigned long long mass[kBins];
@@ -167,14 +264,13 @@ __device__ Spot select(const Row &row, Shared &s, unsigned long long border) {
     }
     if (tid == 0) s.found[0] = kBins;
     __syncthreads();
-    for (int i = tid; i < row.n; i += kThreads) {
-      const unsigned o = order_of(row.x[i]);
-      if (round > 0 && (o >> left) != r.order) continue;
-      const unsigned b = (o >> (left - bits)) & ((1u << bits) - 1);
-      atomicAdd(&s.count[b], 1u);
-      const unsigned long long w = row.weight(row.x[i]);
-      if (w) atomicAdd(&s.mass[b], w);
-    }
+    Run run{s.mass, s.count};
+    tokens_of(row).each([](float) { return 0; }, [&](float x, int, int) {
+      const unsigned o = order_of(x);
+      if (round > 0 && (o >> left) != r.order) return;
+      run.add(row, static_cast<int>((o >> (left - bits)) & ((1u << bits) - 1)), x);
+    });
+    run.flush();
     __syncthreads();
     constexpr int kPer = kBins / kThreads;
     unsigned long long c = 0, m = 0;
@@ -238,8 +334,10 @@ __device__ __forceinline__ unsigned long long tokens_to(const Spot &b, unsigned 
 template <class F>
 __device__ unsigned long long mass_of(const Row &row, Shared &s, F &&f) {
   unsigned long long m = 0;
-  for (int i = threadIdx.x; i < row.n; i += kThreads)
-    if (f(row.x[i])) m += row.weight(row.x[i]);
+  Run run{};
+  tokens_of(row).each([](float) { return 0; }, [&](float x, int, int) {
+    if (f(x)) m += run.weight(row, x);
+  });
   m = block_prefix(m, s.wave);
   __syncthreads();
   if (threadIdx.x == kThreads - 1) s.found[0] = m;
@@ -249,21 +347,48 @@ __device__ unsigned long long mass_of(const Row &row, Shared &s, F &&f) {
   return m;
 }
 
-// Index of the rank-th (from 1) token of a value, in index order.
+// Index of the rank-th (from 1) token of a value, in index order: each wave counts
+// those of its part of the row, and the wave that has it goes over its part again.
 __device__ int index_of(const Row &row, Shared &s, unsigned order, unsigned long long rank) {
-  unsigned long long before = 0;
+  constexpr int kWaves = kThreads / 64, kAhead = 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = (row.n + kWaves - 1) / kWaves, begin = min(row.n, wave * per), end = min(row.n, begin + per);
+  // f(index of lane 0's token, the lanes whose token it is) until it returns true
+  auto scan = [&](auto &&f) {
+    for (int i0 = begin; i0 < end; i0 += 64 * kAhead) {
+      float v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) v[j] = i0 + j * 64 + lane < end ? row.x[i0 + j * 64 + lane] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const bool is = i0 + j * 64 + lane < end && order_of(v[j]) == order;
+        if (f(i0 + j * 64, __builtin_amdgcn_ballot_w64(is))) return;
+      }
+    }
+  };
+  unsigned long long own = 0;
+  scan([&](int, unsigned long long is) {
+    own += __popcll(is);
+    return false;
+  });
+  if (lane == 0) s.wave[wave] = own;
   if (threadIdx.x == 0) s.found[0] = row.n - 1;
-  for (int i0 = 0; i0 < row.n; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const bool is = i < row.n && order_of(row.x[i]) == order;
-    const unsigned long long upto = before + block_prefix(is ? 1 : 0, s.wave);
-    if (is && upto == rank) s.found[0] = i;
-    __syncthreads();
-    if (threadIdx.x == kThreads - 1) s.found[1] = upto;
-    __syncthreads();
-    before = s.found[1];
-    if (before >= rank) break;
+  __syncthreads();
+  unsigned long long before = 0;
+  for (int w = 0; w < wave; ++w) before += s.wave[w];
+  if (before < rank && before + own >= rank) {
+    scan([&](int i, unsigned long long is) {
+      const unsigned long long upto = before + __popcll(is);
+      if (upto < rank) {
+        before = upto;
+        return false;
+      }
+      const bool mine = (is >> lane & 1) && before + __popcll(is & ((2ull << lane) - 1)) == rank;
+      if (mine) s.found[0] = i + lane;
+      return true;
+    });
   }
+  __syncthreads();
   const int at = static_cast<int>(s.found[0]);
   __syncthreads();
   return at;
@@ -403,57 +528,6 @@ struct Extremes {
 union Space {
   Shared select;
   Lists l;
-};
-
-// The tokens of a workgroup: x[begin, end), read anew at each pass, eight loads of
-// a thread in flight.
-struct Chunked {
-  const float *x;
-  int begin, end;
-  // f(logit, index, g(logit)): g of eight tokens side by side, then f of each
-  template <class G, class F>
-  __device__ __forceinline__ void each(G &&g, F &&f) const {
-    constexpr int kAhead = 8;
-    for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kAhead * kThreads) {
-      float v[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j] = i + j * kThreads < end ? x[i + j * kThreads] : 0.0f;
-      decltype(g(0.0f)) y[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) y[j] = g(v[j]);
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (i + j * kThreads < end) f(v[j], i + j * kThreads, y[j]);
-    }
-  }
-};
-
-// Up to N * kThreads tokens, kept in registers.
-template <int N>
-struct Held {
-  float v[N];
-  int n;
-  __device__ Held(const float *x, int n) : n(n) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = threadIdx.x + j * kThreads;
-      v[j] = i < n ? x[i] : 0.0f;
-    }
-  }
-  template <class G, class F>
-  __device__ __forceinline__ void each(G &&g, F &&f) const {
-#pragma unroll
-    for (int j0 = 0; j0 < N; j0 += 8) {
-      decltype(g(0.0f)) y[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = g(v[j0 + j]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = threadIdx.x + (j0 + j) * kThreads;
-        if (i < n) f(v[j0 + j], i, y[j]);
-      }
-    }
-  }
 };
 
 // The largest logit, its first index, the smallest finite one.
