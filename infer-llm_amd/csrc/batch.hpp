@@ -160,7 +160,7 @@ __device__ __forceinline__ bool packed_block(const PackedSeqs &p, int G, int ite
     }
   }
   b.n_blocks = (b.rows * G + BLOCK - 1) / BLOCK;
-  return b.item < b.n_blocks;
+  return b.item >= 0 && b.item < b.n_blocks;  // (below 0: where row_start descends, if at all)
 }
 
 // Integer sum over the wave's lanes (DPP and lane swaps), in a scalar register: a

@@ -251,3 +251,17 @@ def test_packed_prompts_refuse_mixed_operands(dev):
                           (dict(out=q[:3].clone()), ValueError), (dict(row_start=start[:0]), ValueError)):
         with pytest.raises(error):
             ikv.attn_prefill_packed(**{**dict(q=q, k=k, v=v, row_start=start), **change})
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (4, 2, 33)])
+def test_many_sequences_whose_rows_descend(dev, heads, kv, dim):
+    """Over 64 sequences of which some begin behind the next ones: flagged, and
+    nothing outside of the operands is written."""
+    n = 400
+    bad = [0] * 10 + [200] * 10 + [300] * 10 + [40] * 70 + [400]
+    q, k, v = _inputs(dev, 5, n, heads, kv, dim)
+    wide = torch.full((3 * n, heads, dim), FILL, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    ikv.attn_prefill_packed(q, k, v, _dev32(bad, dev), out=wide[n:2 * n], status=status)
+    assert status.item() == ikv.STATUS_POSITION
+    assert (wide[:n] == FILL).all() and (wide[2 * n:] == FILL).all()
