@@ -254,3 +254,32 @@ def test_decode_batch_refuses_mixed_operands(dev):
                           (dict(workspace=torch.zeros(4, device=dev)), ikv.IkvError)):
         with pytest.raises(error):
             ikv.attn_decode_batch(**{**ok, **change})
+
+
+def test_two_captured_calls_share_a_workspace(dev):
+    """Of different heads and lengths (one's runs are dealt out as workgroups are
+    done), replayed one after the other, with eager calls between them."""
+    calls, graphs = [], []
+    ws = max((ikv.decode_batch_workspace(*h) for h in ((32, 8, 128), (10, 1, 80))), key=torch.Tensor.numel)
+    for n_kv, (heads, kv, dim) in (([4096] * 20 + [1, 0], (32, 8, 128)), ([9, 1500, 70], (10, 1, 80))):
+        n, width = len(n_kv), 64
+        tables = torch.randperm(n * width, dtype=torch.int32, device=dev).view(n, width)
+        pools = [torch.randn(n * width * 64, kv, dim, device=dev) for _ in range(2)]
+        q = torch.randn(n, heads, dim, device=dev)
+        calls.append(((q, *pools, tables, 64, _dev32(n_kv, dev)), torch.empty_like(q)))
+        ikv.attn_decode_batch(*calls[-1][0], out=calls[-1][1], workspace=ws)
+    torch.cuda.synchronize()
+    for args, out in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ikv.attn_decode_batch(*args, out=out, workspace=ws)
+    want = [ikv.attn_decode_batch(*args) for args, _ in calls]  # (a workspace of its own)
+    for i in range(4):
+        for _, out in calls:
+            out.fill_(FILL)
+        for j in (0, 1, 1, 0)[i:] + (0, 1):
+            graphs[j].replay()
+        ikv.attn_decode_batch(*calls[i % 2][0], workspace=ws)
+        torch.cuda.synchronize()
+        for (_, out), w in zip(calls, want):
+            assert torch.equal(out, w)
