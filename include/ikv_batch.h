@@ -99,10 +99,13 @@ int ikv_attn_prefill_packed_f32(const float *q, const float *k, const float *v,
  *            parts of sequences of few rows behind long histories, whose keys
  *            are then split over several workgroups (a second launch joins the
  *            parts). ikv_attn_prefill_packed_paged_workspace_bytes() says how
- *            much is used for these sizes (max_tokens: table_stride *
+ *            much is used at most for these sizes (max_tokens: table_stride *
  *            block_tokens); 0, or less memory than that: nothing is split.
  *            Nothing is expected in it or left in it. Launches that share it
- *            must be ordered. */
+ *            must be ordered.
+ * The histories' lengths are device data: that no sequence is longer than a few
+ * hundred tokens, for which the call has a faster kernel, shows only in tables
+ * that cover no more (768), or in n_past NULL with so few rows. */
 size_t ikv_attn_prefill_packed_paged_workspace_bytes(int64_t n_seq, int64_t n_rows,
                                                      int64_t max_tokens, int n_head, int n_head_kv,
                                                      int head_dim);

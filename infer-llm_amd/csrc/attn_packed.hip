@@ -1,20 +1,21 @@
 // attn_packed.hip — causal attention over several prompts, packed one behind
 // the other (ikv_attn_prefill_packed_f32 and its paged form): the checks, and
-// the choice between the two kernels that run them, the bf16-piece one
-// (attn_bf16x3.hip) and, for head sizes and alignments that it does not take,
-// the generic one (attn_generic.hip). Each workgroup finds its sequence from
-// row_start (packed_block in batch.hpp) and then works as on a prompt alone.
-// Where the blocks are more than fit the card, those with the most keys start
-// first; where they are fewer, the keys of the long ones are split (attn_bf16x3.
-// hip). The bf16-piece kernel takes prompts of every length here: one token of 16
-// heads of 128 10.2 us against 13.0 in the generic one, 16 prompts of 64 tokens 17
-// against 33.
+// the choice among the three kernels that run them: short prompts with heads of
+// 128 that leave each block a CU take the F32 MFMA one (attn_prefill.hip), others
+// the bf16-piece one (attn_bf16x3.hip) and, for head sizes and alignments that it
+// does not take, the generic one (attn_generic.hip). Each workgroup finds its
+// sequence from row_start (packed_block in batch.hpp) and then works as on a
+// prompt alone. In the bf16-piece kernel, where the blocks are more than fit the
+// card, those with the most keys start first; where they are fewer, the keys of
+// the long ones are split. It takes prompts of every length: 16 of 64 tokens, 16
+// heads of 128, 17 us against 33 in the generic one, one token 10.2 against 13.0.
 // Measured (MI355X, us): 5 prompts of 8192 tokens together, 32 heads of 128 over
 // 8, behind up to 2000: 1620-1700, 178-187 TFLOP/s, 1.1 PFLOP/s of pieces; 16
 // prompts of 7001 tokens, 16 heads of 128: 162-169; 9 chunks of 1999 tokens, 12
-// heads of 64, behind up to 1500: 63 (in two launches); 6 prompts of 160: 17.
+// heads of 64, behind up to 1500: 63 (in two launches).
 #include "attn_bf16x3.hpp"
 #include "attn_generic.hpp"
+#include "attn_prefill.hpp"
 #include "batch.hpp"
 
 namespace {
@@ -29,8 +30,10 @@ int prefill_packed(const float *q, const float *k, const float *v, const ikv::Pa
   if (n_rows > INT_MAX / 16 / n_head) return -EOVERFLOW;
   seqs.n_rows = static_cast<int>(n_rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rc = ikv::attn_bf16x3_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale,
-                                          space_bytes, s);
+  int rc = ikv::attn_prefill_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale, s);
+  if (rc != -ENOTSUP) return rc;
+  rc = ikv::attn_bf16x3_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale,
+                               space_bytes, s);
   if (rc != -ENOTSUP) return rc;
   return ikv::attn_generic_packed(q, k, v, pages, out, n_head, n_head_kv, head_dim, seqs, scale, s);
 }

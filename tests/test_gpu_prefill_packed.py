@@ -265,3 +265,29 @@ def test_many_sequences_whose_rows_descend(dev, heads, kv, dim):
     ikv.attn_prefill_packed(q, k, v, _dev32(bad, dev), out=wide[n:2 * n], status=status)
     assert status.item() == ikv.STATUS_POSITION
     assert (wide[:n] == FILL).all() and (wide[2 * n:] == FILL).all()
+
+
+@pytest.mark.parametrize("rows,past", [([700, 60], 0), ([900, 60], 0), ([90, 30, 1], 500), ([90, 30, 1], 900)],
+                         ids=["768keys", "more", "behind500", "behind900"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (2, 2, 128), (8, 1, 128), (4, 2, 64)])
+def test_infinity_and_nan_on_either_side_of_the_key_limit(dev, heads, kv, dim, rows, past):
+    """An infinite value and a NaN key in the middle of the first sequence: the rows
+    before them and the other sequences have none of it."""
+    q, pools, tables, own = _paged(dev, sum(rows) + past, rows, [past] * len(rows), 64, heads, kv, dim)
+    bad_v, bad_k = past + rows[0] // 2, past + rows[0] * 2 // 3
+    at_v, at_k = rows_of(tables, 0, 64, [bad_v, bad_k])
+    pools[1][at_v, :, 0], pools[0][at_k] = float("inf"), float("nan")
+    out = ikv.attn_prefill_packed_paged(q, *pools, _dev32(tables, dev), 64, _dev32(starts(rows), dev),
+                                        _dev32([past] * len(rows), dev))
+    first, second = bad_v - past, bad_k - past
+    assert_near(out[:first], attention64(q[:first], *own[0], past), attention_bound(q[:first], *own[0]))
+    mid = out[first:second]
+    assert torch.isinf(mid[:, :, 0]).all()
+    assert_near(mid[:, :, 1:], attention64(q[first:second], *own[0], past + first)[:, :, 1:],
+                attention_bound(q[first:second], *own[0]))
+    assert torch.isnan(out[second:rows[0]]).all()
+    at = rows[0]
+    for s in range(1, len(rows)):
+        mine = slice(at, at + rows[s])
+        assert_near(out[mine], attention64(q[mine], *own[s], past), attention_bound(q[mine], *own[s]))
+        at += rows[s]
