@@ -10,9 +10,10 @@
 // the long ones are split. It takes prompts of every length: 16 of 64 tokens, 16
 // heads of 128, 17 us against 33 in the generic one, one token 10.2 against 13.0.
 // Measured (MI355X, us): 5 prompts of 8192 tokens together, 32 heads of 128 over
-// 8, behind up to 2000: 1620-1700, 178-187 TFLOP/s, 1.1 PFLOP/s of pieces; 16
-// prompts of 7001 tokens, 16 heads of 128: 162-169; 9 chunks of 1999 tokens, 12
-// heads of 64, behind up to 1500: 63 (in two launches).
+// 8, behind up to 2000: 1620-1750, 173-187 TFLOP/s, 1.1 PFLOP/s of pieces; 16
+// prompts of 7001 tokens, 16 heads of 128: 162-173; 9 chunks of 1999 tokens, 12
+// heads of 64, behind up to 1500: 61-64 (in two launches); 6 prompts of 160, 16
+// heads of 128: 11 (the call; the kernel 9.7).
 #include "attn_bf16x3.hpp"
 #include "attn_generic.hpp"
 #include "attn_prefill.hpp"

@@ -22,12 +22,12 @@
 // round, three rounds to one value, whose tokens weigh the same, so that what is
 // left is a division.
 //
-// Measured (MI355X, us): one row of 151936 25 (three launches of 4, 13 and 10: each
+// Measured (MI355X, us): one row of 151936 22-24 (three launches of 4, 7 and 13: each
 // a chain of loads, sums over the workgroup and atomics of 1 us; the row itself is
-// read in 0.1), 48 rows 50 (8, 22, 18: the weights in double, LDS atomics at 25
+// read in 0.1), 48 rows 46 (8, 16, 23: the weights in double, LDS atomics at 25
 // cycles a wave, and the last workgroup's sums), 200 rows of 8191, each held in one
-// workgroup's registers, 17. All logits equal, 151936 of them, with top_p: 425 (one
-// workgroup goes over the row nine times), 48 such rows 650.
+// workgroup's registers, 17. All logits equal, 151936 of them, with top_p: 410 (one
+// workgroup goes over the row nine times), 48 such rows 640.
 #include "../../include/ikv_model.h"
 #include "ikv_common.hpp"
 
@@ -195,7 +195,7 @@ __device__ __forceinline__ Chunked tokens_of(const Row &row) { return {row.x, 0,
 // Tokens one by one for rows of equal logits by the thousand: a weight is computed
 // where a logit differs from the thread's last one, and a thread's tokens of one
 // bin that come one behind the other go there together (an atomic of 64 lanes at
-// one address takes 64 turns). One row of 151936 equal ones 1650 to 425 us; for
+// one address takes 64 turns). One row of 151936 equal ones 1650 to 410 us; for
 // other rows it costs more than it gives (48 of them 49 to 59 us in fill_bins).
 struct Run {
   unsigned long long *mass;
