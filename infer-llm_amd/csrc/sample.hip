@@ -22,7 +22,7 @@
 // round, three rounds to one value, whose tokens weigh the same, so that what is
 // left is a division.
 //
-// Measured (MI355X, us): one row of 151936 22-24 (three launches of 4, 7 and 13: each
+// Measured (MI355X, us): one row of 151936 18-24 (three launches of 4, 7 and 13: each
 // a chain of loads, sums over the workgroup and atomics of 1 us; the row itself is
 // read in 0.1), 48 rows 46 (8, 16, 23: the weights in double, LDS atomics at 25
 // cycles a wave, and the last workgroup's sums), 200 rows of 8191, each held in one

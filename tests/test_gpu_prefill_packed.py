@@ -291,3 +291,31 @@ def test_infinity_and_nan_on_either_side_of_the_key_limit(dev, heads, kv, dim, r
         mine = slice(at, at + rows[s])
         assert_near(out[mine], attention64(q[mine], *own[s], past), attention_bound(q[mine], *own[s]))
         at += rows[s]
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (2, 1), (4, 1), (8, 1), (16, 2), (3, 3), (3, 1)])
+@pytest.mark.parametrize("rows", [[2] * 70 + [90], [33, 0, 1, 64], [1], [0, 17]], ids=lambda r: f"{len(r)}seqs")
+def test_short_prompts_with_heads_of_128(dev, heads, kv, rows):
+    """Every grouping, with and without pages and histories."""
+    past = [(7 * i) % 130 for i in range(len(rows))]
+    q, pools, tables, own = _paged(dev, sum(rows) + heads, rows, past, 64, heads, kv, 128)
+    start = _dev32(starts(rows), dev)
+    q = torch.cat([q, torch.full((3, heads, 128), float("nan"), device=dev)])  # rows of no sequence
+    out = torch.full_like(q, FILL)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    ikv.attn_prefill_packed_paged(q, *pools, _dev32(tables, dev), 64, start, _dev32(past, dev), out=out,
+                                  status=status)
+    new = [torch.cat([t[p:] for t, p in zip(kind, past)] + [torch.full((3, kv, 128), float("nan"), device=dev)])
+           for kind in zip(*own)]
+    alone = ikv.attn_prefill_packed(q, *new, start, out=torch.full_like(q, FILL), status=status)
+    assert status.item() == 0
+    assert (out[sum(rows):] == FILL).all() and (alone[sum(rows):] == FILL).all()
+    at = 0
+    for s, r in enumerate(rows):
+        if r == 0:
+            continue
+        mine, (k, v) = slice(at, at + r), own[s]
+        at += r
+        assert_near(out[mine], attention64(q[mine], k, v, past[s]), attention_bound(q[mine], k, v))
+        k, v = k[past[s]:], v[past[s]:]
+        assert_near(alone[mine], attention64(q[mine], k, v, 0), attention_bound(q[mine], k, v))
