@@ -4,7 +4,7 @@
  * prompts, the decode attention of one new token of each sequence, and the
  * sampler of every row of logits. The single-sequence forms are in ikv.h and
  * ikv_model.h; the reference runs one sequence at a time (src/model.cpp:
- * 164-311) and samples greedily (src/sampler.cpp:5-35), so these entry points
+ * 164-311) and samples greedily (src/sampler.cpp:42-65), so these entry points
  * have no counterpart there. Conventions as in ikv.h: device pointers, stream
  * as void*, 0 / negative errno / positive hipError_t, nothing allocates, frees
  * or synchronises, F32 row-major.
