@@ -945,11 +945,16 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Args a, RowSpace 
   }
 }
 
-// Workgroups of a row: one up to kRowTokens tokens, else as many as bring all
-// rows to kGroups, of 2048 tokens at least (one where there are many rows).
-constexpr int kRowTokens = 16384, kGroups = 512;
+// Workgroups of a row: one up to 16384 tokens, or 32768 where there are 64 rows or
+// more; else as many as bring all rows to kGroups, of 2048 tokens at least (one
+// where there are many rows). One against several, in three launches (us): 1 row of
+// 16385 22.5, 20.5, of 32768 33.5, 19.8; 16 rows of 16385 23.2, 22.7, of 24576 28.6,
+// 23.7; 64 rows of 16385 23.3, 32.7, of 32768 34.7, 33.6, of 49152 47.0, 36.9; 200
+// rows of 32768 35.6, 44.1, of 65536 67.9, 64.4. kGroups 256 and 1024: 48 rows of
+// 151936 56.9 and 58.7 against 49.4; at most 32 workgroups: one row 29.8 against 28.0.
+constexpr int kRowTokens = 16384, kRowsTokens = 32768, kManyRows = 64, kGroups = 512;
 int chunks_of(int64_t n_rows, int64_t n_vocab) {
-  if (n_vocab <= kRowTokens) return 1;
+  if (n_vocab <= (n_rows < kManyRows ? kRowTokens : kRowsTokens)) return 1;
   const int64_t most = std::max<int64_t>(1, kGroups / n_rows);
   return static_cast<int>(std::min<int64_t>({most, (n_vocab + 2047) / 2048, kMaxChunks}));
 }
@@ -978,7 +983,9 @@ extern "C" int ikv_sample_f32(const float *logits, const float *u, const float *
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int chunks = chunks_of(n_rows, n_vocab);
   if (chunks == 1) {
-    if (n_vocab <= kHeld * kThreads)
+    // tokens in registers where they are many and each row has a CU: 200 rows of 8192
+    // 15.8 us against 17.0, of 4096 15.0 against 13.7, 300 rows of 8192 28.9 against 21.1
+    if (n_vocab > 4096 && n_vocab <= kHeld * kThreads && n_rows <= 256)
       sample_held_kernel<<<static_cast<unsigned>(n_rows), kThreads, 0, s>>>(a);
     else
       sample_row_kernel<<<static_cast<unsigned>(n_rows), kThreads, 0, s>>>(a);

@@ -222,3 +222,21 @@ def test_sample_refuses_mixed_operands(dev):
                           (dict(workspace=torch.zeros(1, device=dev)), ikv.IkvError)):
         with pytest.raises(error):
             ikv.sample(**{**dict(logits=x, u=u), **change})
+
+
+@pytest.mark.parametrize("rows,n,few", [(300, 5000, 90), (70, 20000, 9), (64, 32768, 63), (64, 32769, 3),
+                                        (256, 4097, 1), (257, 4096, 200)])
+def test_rows_are_sampled_as_in_smaller_calls(dev, rows, n, few):
+    """One workgroup a row or several, tokens in registers or not: the same results."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(rows + n)
+    x = torch.randn(rows, n, generator=g, device=dev) * 2
+    u = torch.rand(rows, generator=g, device=dev)
+    k = torch.randint(0, 200, (rows,), generator=g, device=dev, dtype=torch.int32)
+    p = 0.5 + 0.6 * torch.rand(rows, generator=g, device=dev)
+    token, logprob = ikv.sample(x, u, top_k=k, top_p=p)
+    for at in range(0, rows, few):
+        s = slice(at, min(at + few, rows))
+        some, some_logprob = ikv.sample(x[s], u[s], top_k=k[s], top_p=p[s])
+        assert torch.equal(token[s], some) and torch.equal(logprob[s], some_logprob)
+    check(x[-3:].cpu().numpy(), u[-3:].tolist(), None, k[-3:].tolist(), p[-3:].tolist())
