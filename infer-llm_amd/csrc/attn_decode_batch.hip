@@ -15,8 +15,8 @@
 //     maximum, sum and weighted values of its part in the workspace (at most
 //     two parts a run, so the workspace depends on no length) and counts
 //     itself; the one that comes last joins the parts in their order. Nothing
-//     waits. Up to kWhole units a (sequence, head) stays with the run that holds
-//     its first one: joining takes longer than reading that much.
+//     waits. A (sequence, head) of few units stays with the run that holds its first
+//     one (Plan::kept): joining takes longer than reading that much.
 //   * LPK lanes hold a key row, NV 16-byte pieces each, so a wave loads 64 / LPK
 //     keys at once; the scores need only the sum over LPK lanes, and each group
 //     of LPK lanes has a running maximum and sums of its own, which meet when
@@ -40,12 +40,16 @@ namespace {
 
 constexpr int kCUs = 256;       // MI355X compute units
 constexpr int kWaves = 4;       // of a workgroup
-constexpr int kGroups = 2 * kCUs;    // workgroups of a launch
-constexpr int kRuns = 4 * kGroups;   // most runs of units
+// Workgroups of a launch: as many as are on the card at once. With 8 query heads
+// and more than 64 dims, whose registers leave room for one on a CU, 512 were two
+// rounds: 16 heads of 80 over 1, 64 contexts of 380 tokens 33 us, with 256 20; 32 of
+// up to 5448 59 and 53.
+constexpr int groups_of(int nv, int gq) { return gq > 4 && nv > 2 ? kCUs : 2 * kCUs; }
+constexpr int kRuns = 8 * kCUs;  // most runs of units
 constexpr int kRunUnits = 16;        // units of a run where there are more runs than workgroups
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int kMaxDim = 512;
-constexpr int kWhole = 3;  // units of a (sequence, head) that are not split
+constexpr int kWhole = 3;  // units of a (sequence, head) that are not split anywhere
 // Cache policy of a load: rows of the pools are read once (non-temporal: 48 long
 // contexts of the 8B heads 410 -> 373 us).
 constexpr std::integral_constant<int, 0> kKept{};
@@ -93,11 +97,11 @@ struct Place {
   int seq, keys, tiles, item, tile;
 };
 
-template <int KT>
+template <int KT, int GROUPS>
 struct Plan {
   using Units = unsigned long long;
   Units total, chunk;  // all units, those of a run
-  int runs;
+  int runs, whole;
   unsigned items;  // head passes of a sequence
   // the sequence s0 + lane of 64: its keys, and the units up to its end
   int s0, keys;
@@ -118,9 +122,20 @@ struct Plan {
       look(a, s, total);
       total = lane_value(upto, 63);
     }
-    runs = static_cast<int>(min(max(total / kRunUnits, static_cast<Units>(kGroups)), static_cast<Units>(kRuns)));
+    runs = static_cast<int>(min(max(total / kRunUnits, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
     chunk = (total + runs - 1) / runs;
     if (chunk == 0) chunk = 1;
+    whole = chunk > 1 ? static_cast<int>(min(chunk, static_cast<Units>(4))) + 3 : kWhole;
+  }
+
+  // whether a (sequence, head) of so many units stays with one run: up to kWhole, and
+  // up to three more than a run has where those are two or more and it is no whole
+  // number of them (a run of two parts then has two starts and two joins): 16 heads
+  // of 128 over 8, 16 contexts of 300 tokens 18.2 -> 13.0 us, 24 of 380, two whole
+  // runs each, 18.8 split and 22.5 not; of 200, runs of one unit, 9.8 and 11.3; over
+  // ragged lengths between 10 % more and as much less.
+  __device__ bool kept(int tiles) const {
+    return tiles <= kWhole || (tiles <= whole && static_cast<unsigned>(tiles) % static_cast<unsigned>(chunk) != 0);
   }
 
   // where unit u (< total) is
@@ -254,7 +269,8 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     for (int d = threadIdx.x; d < n_head * a.dim; d += kWaves * 64) o[d] = 0.f;
   }
 
-  Plan<KT> plan(a);
+  constexpr int kGroups = groups_of(NV, GQ);
+  Plan<KT, kGroups> plan(a);
   const Parts<GQ, DP> parts(a.part);
   unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
 #pragma unroll
@@ -317,13 +333,13 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       continue;
     }
     // the run's part of one (sequence, KV head, pass): tiles [p.tile, last)
-    if (p.tiles <= kWhole && p.tile > 0) {  // (with the run that holds its first unit)
+    if (plan.kept(p.tiles) && p.tile > 0) {  // (with the run that holds its first unit)
       u += p.tiles - p.tile;
       plan.next(a, p);
       continue;
     }
     const int last =
-        p.tiles <= kWhole ? p.tiles : static_cast<int>(min<unsigned long long>(p.tiles, p.tile + (end - u)));
+        plan.kept(p.tiles) ? p.tiles : static_cast<int>(min<unsigned long long>(p.tiles, p.tile + (end - u)));
     const int g = p.item / a.passes, h0 = p.item % a.passes * GQ;
     const int heads = min(GQ, a.G - h0);
     const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
@@ -631,9 +647,9 @@ Form form_of(int G, int dim) {
 template <int LPK, int NV, int GQ>
 int launch(const Args &a, bool vec, hipStream_t s) {
   if (vec)
-    decode_batch_kernel<LPK, NV, GQ, true><<<kGroups, kWaves * 64, 0, s>>>(a);
+    decode_batch_kernel<LPK, NV, GQ, true><<<groups_of(NV, GQ), kWaves * 64, 0, s>>>(a);
   else
-    decode_batch_kernel<LPK, NV, GQ, false><<<kGroups, kWaves * 64, 0, s>>>(a);
+    decode_batch_kernel<LPK, NV, GQ, false><<<groups_of(NV, GQ), kWaves * 64, 0, s>>>(a);
   return ikv::launch_status();
 }
 
