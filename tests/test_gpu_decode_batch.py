@@ -283,3 +283,19 @@ def test_two_captured_calls_share_a_workspace(dev):
         torch.cuda.synchronize()
         for (_, out), w in zip(calls, want):
             assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("heads,kv,dim,n_kv", [
+    (16, 8, 128, [300] * 16), (16, 8, 128, [380] * 24 + [1]), (16, 8, 128, [440] * 30 + [0, 64, 130]),
+    (16, 1, 80, [300] * 40), (16, 1, 80, [440] * 100), (16, 1, 80, [4000 - 61 * i for i in range(44)]),
+    (10, 1, 200, [2000 + 100 * i for i in range(24)])],
+    ids=["16of300", "24of380", "30of440", "g8_40of300", "g8_100of440", "g8_long", "g8_200dims"])
+def test_decode_batch_of_equal_contexts(dev, heads, kv, dim, n_kv):
+    """Contexts of a few units across the runs, and heads in groups of 8 with fewer
+    and with more runs than workgroups; twice on one workspace."""
+    q, pools, tables, fresh, own = _setup(dev, len(n_kv), n_kv, 64, heads, kv, dim)
+    ws = ikv.decode_batch_workspace(heads, kv, dim)
+    args = (q, *pools, _dev32(tables, dev), 64, _dev32(n_kv, dev))
+    out = ikv.attn_decode_batch(*args, k_new=fresh[0], v_new=fresh[1], workspace=ws)
+    _check_rows(out, q, own)
+    assert torch.equal(out, ikv.attn_decode_batch(*args, k_new=fresh[0], v_new=fresh[1], workspace=ws))
