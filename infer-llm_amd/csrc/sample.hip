@@ -640,8 +640,10 @@ __device__ Ranges find_ranges(const Row &row, const Window &win, const Cuts &c, 
       const float f = static_cast<float>(x);
       return f < INFINITY && f > -INFINITY ? nextafterf(f, way) : f;
     };
-    r.lo[2] = max(win.bin(edge(at + slack, INFINITY)), 0);
-    r.hi[2] = max(win.bin(edge(at - slack, -INFINITY)), 0);
+    // (a min_p of more than 1 is past the largest logit, perhaps past all floats: a
+    // window of no width would put that into its last bin)
+    r.lo[2] = win.bin(fminf(edge(at + slack, INFINITY), row.top));
+    r.hi[2] = win.bin(fminf(edge(at - slack, -INFINITY), row.top));
     r.before_m = l.mass[r.lo[2]];
     least = min(least, r.before_m);
     most = min(most, l.mass[r.hi[2] + 1]);

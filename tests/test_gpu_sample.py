@@ -240,3 +240,14 @@ def test_rows_are_sampled_as_in_smaller_calls(dev, rows, n, few):
         some, some_logprob = ikv.sample(x[s], u[s], top_k=k[s], top_p=p[s])
         assert torch.equal(token[s], some) and torch.equal(logprob[s], some_logprob)
     check(x[-3:].cpu().numpy(), u[-3:].tolist(), None, k[-3:].tolist(), p[-3:].tolist())
+
+
+def test_sample_min_p_past_one_at_the_largest_temperatures(dev):
+    """No token passes, so the first one is kept, also where temperature times
+    ln(min_p) is past the largest float."""
+    rng = np.random.default_rng(11)
+    for n in (5, 300, 9000, 20000):
+        x = np.full((4, n), 1.5, np.float32)
+        x[2] = _normal(rng, 1, n)[0]
+        x[3] = 3.4e38
+        check(x, [0.9] * 4, [3e38, 1.0, 3e38, 3e38], None, None, [1e10, 2.0, 1e10, 1e30])
