@@ -760,6 +760,11 @@ __global__ __launch_bounds__(RW *DT * 64) void attn_join_kernel(float *__restric
     if (any != on_f32[i]) f[i] *= 1.0f / kProbScale;
     if (i < n) all = fmaf(f[i], l[i], all);
   }
+  // (divided before they are added: with the factor, the parts' sums together may
+  // be past what F32 holds where each of them and the result are not)
+  const float inv = 1.0f / pair_sum(all);
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) f[i] *= inv;
   floatx16 o{};
 #pragma unroll
   for (int i0 = 0; i0 < kMaxParts; i0 += 4) {
@@ -777,7 +782,6 @@ __global__ __launch_bounds__(RW *DT * 64) void attn_join_kernel(float *__restric
     }
   }
   const int row = blk * BR + slot * 32 + r32;
-  const float inv = 1.0f / pair_sum(all);
   if (row >= n_rows) return;
   const int n_head = n_head_kv * G;
   float *orow = out + (static_cast<size_t>(b.first + row / G) * n_head + g * G + row % G) * dim;
@@ -785,7 +789,7 @@ __global__ __launch_bounds__(RW *DT * 64) void attn_join_kernel(float *__restric
   for (int z = 0; z < 4; ++z) {
     const int d = 32 * t + 8 * z + 4 * c2;
     if (d < dim)
-      *reinterpret_cast<floatx4 *>(orow + d) = floatx4{o[4 * z], o[4 * z + 1], o[4 * z + 2], o[4 * z + 3]} * inv;
+      *reinterpret_cast<floatx4 *>(orow + d) = floatx4{o[4 * z], o[4 * z + 1], o[4 * z + 2], o[4 * z + 3]};
   }
 }
 

@@ -319,3 +319,19 @@ def test_short_prompts_with_heads_of_128(dev, heads, kv, rows):
         assert_near(out[mine], attention64(q[mine], k, v, past[s]), attention_bound(q[mine], k, v))
         k, v = k[past[s]:], v[past[s]:]
         assert_near(alone[mine], attention64(q[mine], k, v, 0), attention_bound(q[mine], k, v))
+
+
+def test_split_keys_of_large_values(dev):
+    """Each part's sums are finite where all parts' together would not be: 4040 keys
+    of values about 2e30, whose sum is kept times 2^17."""
+    heads, kv, dim, rows, past = 2, 1, 128, [40], [4000]
+    q, pools, tables, own = _paged(dev, 87, rows, past, 64, heads, kv, dim)
+    q *= 1e-3  # weights of about one
+    at = torch.tensor(rows_of(tables, 0, 64, range(4040)), dtype=torch.long, device=dev)
+    v = (1 + 0.1 * own[0][1]) * 2e30
+    pools[1][at] = v
+    args = (q, *pools, _dev32(tables, dev), 64, _dev32([0, 40], dev), _dev32(past, dev))
+    want = attention64(q, own[0][0], v, 4000)
+    for ws in (None, torch.empty(4, device=dev)):  # split, and in one piece
+        out = ikv.attn_prefill_packed_paged(*args, workspace=ws)
+        assert_near(out, want, attention_bound(q, own[0][0], v), rel=None)
