@@ -42,10 +42,11 @@ extern "C" {
  * [0, n_pool_blocks) is treated as by ikv_kv_pages: reads take block 0's rows,
  * writes are dropped, IKV_STATUS_BLOCK is raised in *status. Sequences may
  * share blocks that none of them writes in the call.
- * Checked before any launch (-EINVAL): block_tables not NULL, table_stride and
- * n_pool_blocks positive, block_tokens a positive multiple of 64, n_seq not
- * negative; -EOVERFLOW: pool rows past 2^31, n_seq past 2^20, a table_stride *
- * block_tokens past 2^28 (0 sequences: nothing is launched).
+ * Checked before any launch (-EINVAL): n_pool_blocks positive, block_tokens a
+ * positive multiple of 64, table_stride and n_seq not negative, and where there
+ * are sequences block_tables not NULL and table_stride positive; -EOVERFLOW:
+ * pool rows past 2^31, n_seq past 2^20, a table_stride * block_tokens past 2^28.
+ * 0 sequences: nothing is launched, and 0 is returned where the rest is right.
  * ------------------------------------------------------------------- */
 typedef struct ikv_kv_batch {
     const int32_t *block_tables; /* [n_seq][table_stride] */

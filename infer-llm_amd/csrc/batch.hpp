@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "../../include/ikv_batch.h"
@@ -28,11 +29,13 @@ struct BatchPages {
 };
 
 inline int batch_arg(const ikv_kv_batch *b, BatchPages &out) {
-  if (!b || !b->block_tables || b->table_stride <= 0 || b->block_tokens <= 0 ||
-      b->block_tokens % 64 != 0 || b->n_pool_blocks <= 0 || b->n_seq < 0)
+  if (!b || b->table_stride < 0 || b->block_tokens <= 0 || b->block_tokens % 64 != 0 || b->n_pool_blocks <= 0 ||
+      b->n_seq < 0)
     return -EINVAL;
+  // (no sequences: an empty table has no address, and perhaps no columns)
+  if (b->n_seq > 0 && (!b->block_tables || b->table_stride == 0)) return -EINVAL;
   if (b->block_tokens > INT_MAX / b->n_pool_blocks || b->n_seq > kMaxSeqs ||
-      b->block_tokens > kMaxSeqTokens / b->table_stride)
+      b->block_tokens > kMaxSeqTokens / std::max<int64_t>(b->table_stride, 1))
     return -EOVERFLOW;
   out.tables = b->block_tables;
   out.stride = b->table_stride;

@@ -129,3 +129,21 @@ def test_decode_batch_refuses_bad_arguments():
 def test_decode_batch_workspace_of_refused_shapes():
     size = ikv.load().ikv_attn_decode_batch_workspace_bytes
     assert size(12, 8, 128) == 0 and size(0, 8, 128) == 0 and size(16, 8, 0) == 0 and size(16, 8, 513) == 0
+
+
+@pytest.mark.parametrize("empty", [dict(tables=None), dict(tables=None, stride=0), dict(stride=0)],
+                         ids=lambda e: "+".join(e))
+def test_no_sequences_need_no_tables(empty):
+    """A step in which nobody is active: an empty table has no address and may have
+    no columns."""
+    b = _batch(n_seq=0, **empty)
+    assert _append(batch=b) == 0
+    assert _packed_paged(batch=b) == 0 and _packed_paged(batch=b, past=P) == 0
+    assert _decode(batch=b) == 0
+
+
+def test_no_sequences_are_no_excuse():
+    """What else is wrong with a call is refused all the same."""
+    for bad in (dict(stride=-1), dict(bt=32), dict(bt=0), dict(pool=0)):
+        b = _batch(n_seq=0, **bad)
+        assert _append(batch=b) == _packed_paged(batch=b) == _decode(batch=b) == -errno.EINVAL, bad

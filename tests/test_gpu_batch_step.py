@@ -229,3 +229,23 @@ def test_a_decode_step_captured_and_replayed(dev):
         tokens = dict(enumerate(token.tolist()))
     for a, b in zip(eager.pools, graphed.pools):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("width", [0, 5])
+def test_a_step_without_sequences(dev, width):
+    """Nobody is active: nothing is written, nothing is refused."""
+    kv, D = 2, 64
+    pools = [torch.full((256, kv, D), 7.0, device=dev) for _ in range(2)]
+    tables = torch.zeros((0, width), dtype=torch.int32, device=dev)
+    none, start = torch.zeros(0, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    for rows in (0, 3):  # (rows of no sequence)
+        q, k = torch.randn(rows, 4, D, device=dev), torch.randn(rows, kv, D, device=dev)
+        out = torch.full_like(q, 3.0)
+        ikv.append_packed(*pools, k, k, tables, 64, start, none)
+        assert ikv.attn_prefill_packed(q, k, k, start, out=out) is out
+        for past in (none, None):
+            assert ikv.attn_prefill_packed_paged(q, *pools, tables, 64, start, past, out=out) is out
+        assert (out == 3.0).all()
+    q, k = torch.randn(0, 4, D, device=dev), torch.randn(0, kv, D, device=dev)
+    assert ikv.attn_decode_batch(q, *pools, tables, 64, none, k_new=k, v_new=k).shape == (0, 4, D)
+    assert all((p == 7.0).all() for p in pools)
