@@ -179,6 +179,15 @@ __device__ __forceinline__ int wave_sum_int(int x) {
   return __builtin_amdgcn_readfirstlane(static_cast<int>(b[0] + b[1]));
 }
 
+// Of a sequence's blocks, those whose last row sees at least L tiles of `tile` keys:
+// its last ones.
+__host__ __device__ constexpr int blocks_of_tiles(int rows, int past, int G, int block, int tile, int L) {
+  const int blocks = (rows * G + block - 1) / block;
+  const int unseen = tile * (L - 1) - past;  // tokens before the first that sees so many keys
+  if (unseen <= 0) return blocks;
+  return unseen >= rows ? 0 : blocks - unseen * G / block;
+}
+
 // packed_block with the blocks of all sequences (up to kLaneSeqs) in the order of
 // their tiles of TILE keys, the longest first, so that a launch of more blocks
 // than fit the card does not end on a long one. The number of blocks of at least
@@ -191,12 +200,7 @@ __device__ __forceinline__ bool packed_block_longest(const PackedSeqs &p, int G,
   const LaneSeq mine(p);
   const int first = mine.first, rows = mine.rows, past = mine.past;
   const int blocks = (rows * G + BLOCK - 1) / BLOCK;
-  // this sequence's blocks of L tiles or more: its last ones
-  auto at_least = [&](int L) {
-    const int unseen = TILE * (L - 1) - past;  // tokens before the first that sees so many keys
-    if (unseen <= 0) return blocks;
-    return unseen >= rows ? 0 : (rows * G - unseen * G + BLOCK - 1) / BLOCK;
-  };
+  auto at_least = [&](int L) { return blocks_of_tiles(rows, past, G, BLOCK, TILE, L); };
   if (item >= wave_sum_int(blocks)) return false;
   int lo = 1, hi = 1;  // wave_sum_int(at_least(lo)) > item
   const int most = rows > 0 ? (past + rows + TILE - 1) / TILE : 0;
