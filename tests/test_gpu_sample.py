@@ -251,3 +251,28 @@ def test_sample_min_p_past_one_at_the_largest_temperatures(dev):
         x[2] = _normal(rng, 1, n)[0]
         x[3] = 3.4e38
         check(x, [0.9] * 4, [3e38, 1.0, 3e38, 3e38], None, None, [1e10, 2.0, 1e10, 1e30])
+
+
+@pytest.mark.parametrize("n", [300, 6000, 9000, 40001, 151936])
+def test_sample_min_p_among_ties(dev, n):
+    """Few different values: min_p falls between them, just below or above one, or
+    at the largest, alone and with cuts by top_k and top_p inside a tie."""
+    rng = np.random.default_rng(n + 1)
+    grid = []
+    for t in (1.0, 0.5, 2.5):
+        at = np.float32(math.exp(-1.0 / t))  # of the values one below the largest
+        lows = [float(np.nextafter(at, np.float32(0))), float(np.nextafter(at, np.float32(1))),
+                math.exp(-1.5 / t), math.exp(-0.5 / t), math.exp(-2.5 / t), 1.0, 1.5]
+        cuts = [(0, 1.0), (n // 3, 1.0), (n // 2 + 1, 0.63), (0, 0.37), (0, 0.991)]
+        grid += [(t, low, *cut) for low in lows for cut in cuts]
+    rows = 12
+    for i in range(0, len(grid), rows):
+        some = [grid[(i + j) % len(grid)] for j in range(rows)]
+        few = rng.integers(0, 3, (rows, n)).astype(np.float32)
+        few[0] = 1.5
+        few[1, n // 5:] = 0.0
+        few[2] = np.where(rng.random(n) < 0.5, np.float32(0.0), np.float32(-0.0))
+        few[3, : n // 2] = -np.inf
+        u = rng.random(rows).tolist()
+        u[4], u[5] = 0.0, LAST_U
+        check(few, u, [s[0] for s in some], [s[2] for s in some], [s[3] for s in some], [s[1] for s in some])
