@@ -335,3 +335,51 @@ def test_split_keys_of_large_values(dev):
     for ws in (None, torch.empty(4, device=dev)):  # split, and in one piece
         out = ikv.attn_prefill_packed_paged(*args, workspace=ws)
         assert_near(out, want, attention_bound(q, own[0][0], v), rel=None)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 8, 128), (2, 1, 128), (12, 4, 64), (8, 1, 80)])
+def test_captured_prompts_on_pages_with_new_histories(dev, heads, kv, dim):
+    """One capture with a workspace serves histories from none to long ones, so keys
+    in one part and in many; what the workspace holds does not matter."""
+    bt, blocks, n_seq, n = 64, 64, 4, 48
+    g = torch.Generator(device=dev)
+    g.manual_seed(heads + dim)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    pools = [rnd(n_seq * blocks * bt, kv, dim) for _ in range(2)]
+    order = torch.randperm(n_seq * blocks, generator=g, device=dev).view(n_seq, blocks)
+    tables = order.to(torch.int32)
+    keys = [(order[s, :, None] * bt + torch.arange(bt, device=dev)).reshape(-1) for s in range(n_seq)]
+    q, out = rnd(n, heads, dim), torch.empty(n, heads, dim, device=dev)
+    start, past = _dev32([0, 12, 24, 36, 48], dev), _dev32([0] * n_seq, dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    ws = ikv.prefill_packed_workspace(n_seq, n, blocks * bt, heads, kv, dim)
+    assert ws is not None
+    call = lambda: ikv.attn_prefill_packed_paged(q, *pools, tables, bt, start, past, out=out, status=status,  # noqa: E731
+                                                 workspace=ws)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for sizes, before in (([12, 12, 12, 12], [0, 0, 0, 0]), ([40, 0, 3, 5], [3000, 10, 4000, 0]),
+                          ([1, 1, 1, 45], [300, 200, 0, 4050]), ([0, 0, 0, 48], [0, 4096, 0, 0]),
+                          ([0, 30, 0, 0], [0, 4066, 0, 0]), ([12, 12, 12, 12], [700, 1400, 2100, 2800])):
+        start.copy_(torch.from_numpy(starts(sizes)))
+        past.copy_(_dev32(before, dev))
+        q.normal_()
+        out.fill_(FILL)
+        ws.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        at = 0
+        for s, r in enumerate(sizes):
+            if r:
+                k, v = (p[keys[s][:before[s] + r]] for p in pools)
+                qs = q[at:at + r]
+                assert_near(out[at:at + r], attention64(qs, k, v, before[s]), attention_bound(qs, k, v))
+            at += r
+        assert (out[at:] == FILL).all()
+        again = torch.full_like(out, FILL)
+        ikv.attn_prefill_packed_paged(q, *pools, tables, bt, start, past, out=again, status=status)
+        assert torch.equal(out, again)
+    assert status.item() == 0
