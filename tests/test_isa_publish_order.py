@@ -127,3 +127,27 @@ def test_checker_catches_planted_mistakes():
         with pytest.raises(AssertionError):
             check_publish_order("planted", body)
     check_publish_order("one writer", no_barrier, many_writers=False)
+
+
+def arrival(body):
+    """A kernel's code from its first store of a pair to the atomic that counts the
+    workgroup (other counters' atomics come before or behind that)."""
+    pair = re.compile(r"^\s*global_store_dwordx2\b.*\bsc1\b")
+    first = next(i for i, l in enumerate(body) if pair.match(l))
+    at = next(i for i in range(first, len(body)) if ATOMIC_RET.match(body[i]))
+    return body[first:at + 1]
+
+
+def test_batched_decode_publishes_before_counting(tmp_path):
+    asm = device_asm(CSRC / "attn_decode_batch.hip", tmp_path)
+    found = [(n, b) for n, b in functions(asm) if "decode_batch_kernel" in n]
+    assert len(found) == 6 * 4 * 2  # head sizes, query heads at once, alignment
+    for name, body in found:
+        check_publish_order(name, arrival(body))  # every thread stores, one counts
+
+
+def test_sampling_publishes_before_counting(tmp_path):
+    asm = device_asm(CSRC / "sample.hip", tmp_path)
+    found = [(n, b) for n, b in functions(asm) if "sample_pick_kernel" in n]
+    assert len(found) == 1
+    check_publish_order(found[0][0], arrival(found[0][1]))
