@@ -83,6 +83,10 @@ int ikv_append_packed_f32(void *k_pool, void *v_pool, const void *k_rows, const 
  * grouping, scale and results as for ikv_attn_prefill_f32 (any head_dim up to
  * 512, any n_head that n_head_kv divides; else -ENOTSUP / -EINVAL; no
  * workspace), any alignment of 4 bytes. status: device int, or NULL.
+ * A result depends on n_seq and n_rows, and in the paged form on the tables' width
+ * and the other sequences' lengths, by the order of its sums (the kernel's form and
+ * the parts of the keys follow from them), and on nothing else of the other
+ * sequences; equal calls give equal bits.
  * -EOVERFLOW: n_rows * n_head past 2^27, or too many blocks for one launch.
  * ------------------------------------------------------------------- */
 int ikv_attn_prefill_packed_f32(const float *q, const float *k, const float *v,

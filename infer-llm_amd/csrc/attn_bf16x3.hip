@@ -102,8 +102,13 @@ __device__ __forceinline__ void load_dims(__amdgpu_buffer_rsrc_t r, unsigned off
 // up to seqs.parts parts, each a workgroup's. A part leaves its rows' sums and
 // maxima in the workspace, as the lanes hold them, and attn_join_kernel adds them
 // up. A block has as many parts as it holds times the load of a slot of the card
-// if all were equal, and kPartTiles: where the blocks fill the card, long ones are
-// split and the others are not.
+// if all were equal, and kPartTiles, rounded down: one that holds less than 1.9
+// times the load stays whole, and is the longest workgroup then (9 chunks of
+// 64-float heads: a load of 23 tiles, the two halves of blocks of up to 59 are 32 at
+// most, a whole block 43). Nothing is split in a launch of over kLaneSeqs sequences,
+// or where the blocks of as many sequences of the mean length would not fit the card
+// at once (heads of 128 over 8 KV heads: from 33 sequences on), however long one
+// history is.
 constexpr int kPartTiles = 8;
 constexpr int kMaxParts = 16;
 static_assert(kPartTiles % 4 == 0, "tiles of every key group");

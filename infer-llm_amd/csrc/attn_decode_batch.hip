@@ -29,7 +29,14 @@
 // 2.4 GB: 371, 6.6 TB/s; 37 of up to 5003, 12 heads of 64 over 4, 128 MB: 31, of
 // which 1 to the first load, 5 to join and for the last workgroup to be done; 3 of
 // up to 150 and an idle slot, 16 heads of 128: 10, three units one after the other.
-// Query groups of more than 8 read the keys once per 8 heads.
+// Query groups of more than 8 read the keys once per 8 heads, each time from behind
+// the L2 (FETCH_SIZE of 16 heads 1.9 times that of 8). Groups of 8 and more are far
+// from what the reads take: a wave on a SIMD, whose vector instructions are issued in
+// 44-49 % of its cycles and which waits in 34-38 %. 32 contexts of up to 5448, 40 MB, 6
+// at 6.6 TB/s: 8 heads of 80 over 1 37, 16 over 1 43; of 128, 64 MB, 10: 16 over 1 54,
+// 32 over 1 76. Heads of over 128 dims, the same contexts: 8 of 200 over 4, 402 MB, 80
+// (61 at that rate), of 256 88 (78), 8 of 512 over 2 102 (78); loads of 4 bytes: 16 of
+// 65 over 8, 262 MB, 157 (40).
 #include "batch.hpp"
 #include "coherent.hpp"
 

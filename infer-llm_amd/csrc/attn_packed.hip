@@ -5,15 +5,20 @@
 // the bf16-piece one (attn_bf16x3.hip) and, for head sizes and alignments that it
 // does not take, the generic one (attn_generic.hip). Each workgroup finds its
 // sequence from row_start (packed_block in batch.hpp) and then works as on a
-// prompt alone. In the bf16-piece kernel, where the blocks are more than fit the
-// card, those with the most keys start first; where they are fewer, the keys of
-// the long ones are split. It takes prompts of every length: 16 of 64 tokens, 16
-// heads of 128, 17 us against 33 in the generic one, one token 10.2 against 13.0.
+// prompt alone. In the bf16-piece kernel, up to 64 sequences, where the blocks are
+// more than fit the card, those with the most keys start first; where they are
+// fewer, the keys of the long ones are split (part_tiles). It takes prompts of every
+// length: 16 of 64 tokens, 16 heads of 128, 17 us against 33 in the generic one, one
+// token 10.2 against 13.0.
 // Measured (MI355X, us): 5 prompts of 8192 tokens together, 32 heads of 128 over
 // 8, behind up to 2000: 1620-1750, 173-187 TFLOP/s, 1.1 PFLOP/s of pieces; 16
 // prompts of 7001 tokens, 16 heads of 128: 162-173; 9 chunks of 1999 tokens, 12
 // heads of 64, behind up to 1500: 61-64 (in two launches); 6 prompts of 160, 16
-// heads of 128: 11 (the call; the kernel 9.7).
+// heads of 128: 11 (the call; the kernel 9.7), with histories and tables of 4096
+// tokens, so on the bf16-piece kernel, 18. The generic kernel, 16 prompts behind up
+// to 500, each case with the time of its flops at 154 TFLOP/s: 3605 tokens, 8 heads
+// of 200 over 4, 1160 (71); 2692, of 256, 740 (53); 3082, of 512 over 2, 1780 (153);
+// 1744, 16 heads of 65 over 8, 600 (17).
 #include "attn_bf16x3.hpp"
 #include "attn_generic.hpp"
 #include "attn_prefill.hpp"
