@@ -139,7 +139,10 @@ int ikv_argmax_ws_f32(const float *logits, int64_t n, int32_t *token, int32_t *t
  * min_p [n_rows] may each be NULL: 1, all, 1, 0. Parameters are device memory.
  * The masses are summed exactly in integers of 2^-44 of the heaviest token's
  * (n_vocab = 151936; 62 bits less those of n_vocab, 51 at most), so equal calls
- * give equal results.
+ * give equal results. Each weight is rounded to such an integer: a token below half
+ * of one weighs nothing and is never drawn, and where u is next to 1 and the tail is
+ * long (1 - 2^-24 and thousands of tokens of 2^-36) another token of the tail than
+ * by exact masses may be.
  * workspace: device memory of ikv_sample_workspace_bytes(n_rows, n_vocab)
  * bytes, 16-byte aligned (else -EINVAL); nothing is expected in it or left in
  * it, and it is enough for fewer rows. Launches that share it must be ordered.
