@@ -134,7 +134,7 @@ int ikv_argmax_ws_f32(const float *logits, int64_t n, int32_t *token, int32_t *t
  * the kept mass; logprob[row], if logprob is not NULL, is the logarithm of its
  * share of the kept mass. temperature <= 0 is greedy: the first of the largest
  * logits, logprob 0. -inf logits are never drawn. A NaN or +inf logit, all
- * logits -inf, a NaN parameter or an infinite temperature give token -1 and a
+ * logits -inf, a NaN parameter or a temperature of +inf give token -1 and a
  * NaN logprob. u is brought into [0, 1 - 2^-24]. temperature, top_k, top_p,
  * min_p [n_rows] may each be NULL: 1, all, 1, 0. Parameters are device memory.
  * The masses are summed exactly in integers of 2^-44 of the heaviest token's
