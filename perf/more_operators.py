@@ -234,8 +234,7 @@ def _quantised(x, e4m3):
     largest element takes the largest code. In 64 bits: a quotient next to a border
     decides the code."""
     top = x.abs().amax(-1, keepdim=True).double()
-    per = (448.0 if e4m3 else 127.0) / torch.where(top == 0, torch.ones_like(top), top)
-    y = x.double() * per
+    y = x.double() * (448.0 if e4m3 else 127.0) / torch.where(top == 0, torch.ones_like(top), top)
     codes = y.float().to(torch.float8_e4m3fn).view(torch.int8) if e4m3 else torch.round(y).to(torch.int8)
     return codes, (top[..., 0] / (448.0 if e4m3 else 127.0)).float()
 
