@@ -1,9 +1,11 @@
 /*
  * ikv_batch.h — C-ABI of a step over several sequences on the MI355X (gfx950):
  * the append of packed rows to a paged KV cache, causal attention over packed
- * prompts, the decode attention of one new token of each sequence, and the
- * sampler of every row of logits. The single-sequence forms are in ikv.h and
- * ikv_model.h; the reference runs one sequence at a time (src/model.cpp:
+ * prompts, the decode attention of one new token of each sequence, the same
+ * where sequences share a prefix, and a cache of 8 bits an element with its
+ * append, its decode attention and its way back to floats. The rules on every row
+ * of logits and their sampler are in ikv_model.h, the single-sequence forms in
+ * ikv.h and there; the reference runs one sequence at a time (src/model.cpp:
  * 164-311) and samples greedily (src/sampler.cpp:42-65), so these entry points
  * have no counterpart there. Conventions as in ikv.h: device pointers, stream
  * as void*, 0 / negative errno / positive hipError_t, nothing allocates, frees
@@ -154,6 +156,100 @@ int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,
                               const float *v_new, float *out, int n_head, int n_head_kv,
                               int head_dim, float scale, void *workspace, size_t workspace_bytes,
                               void *stream);
+
+/* ---------------------------------------------------------------------
+ * A paged KV cache of 8 bits an element: codes and, for each row of head_dim
+ * elements (a token's K or V of one KV head), an F32 scale. A code stands for
+ * code * scale. With top the row's largest magnitude,
+ *     IKV_Q8_INT8  scale = top / 127, code = 127 x / top, an integer;
+ *     IKV_Q8_E4M3  scale = top / 448, code = 448 x / top in 1-4-3 bits (the
+ *                  largest 448, no infinities), from the quotient as a float;
+ * the quotient in 64 bits, rounded to nearest, ties to even. A row of zeros has
+ * scale 0; one with an element that is not finite has a NaN scale and codes 0, so
+ * it reads back as NaNs. The block of ikv_kv_batch's table entry b holds
+ *     codes  [b][n_head_kv][block_tokens][head_dim] bytes
+ *     scales [b][n_head_kv][block_tokens] floats
+ * in each of the K and V arrays, head by head, so that a head's rows of a block
+ * are contiguous. codes and scales 16-byte aligned (else -EINVAL); head_dim a
+ * multiple of 16 up to 256 (else -ENOTSUP); -EOVERFLOW: n_head_kv * head_dim past
+ * 2^23.
+ * ------------------------------------------------------------------- */
+#define IKV_Q8_INT8 0
+#define IKV_Q8_E4M3 1
+
+typedef struct ikv_kv_q8 {
+    void *k_codes;
+    float *k_scales;
+    void *v_codes;
+    float *v_scales;
+    int32_t n_head_kv;
+    int32_t head_dim;
+    int32_t format; /* IKV_Q8_* */
+} ikv_kv_q8;
+
+/* ikv_append_packed_f32 into such a cache: rows [row_start[s], row_start[s+1]) of
+ * k_rows and v_rows [n_rows][n_head_kv][head_dim] (16-byte aligned) become
+ * sequence s's logical tokens first_token[s], first_token[s] + 1, ... */
+int ikv_append_packed_q8(const ikv_kv_q8 *cache, const float *k_rows, const float *v_rows,
+                         const ikv_kv_batch *batch, const int32_t *row_start,
+                         const int32_t *first_token, int64_t n_rows, void *stream);
+
+/* The way back: rows [row_start[s], row_start[s+1]) of k_rows and v_rows become
+ * the values (code * scale, rounded once) of sequence s's logical tokens
+ * first_token[s], first_token[s] + 1, ...; tokens from n_kv[s] on ([n_seq] int32,
+ * or NULL: none are) leave their rows as they were, as do rows behind
+ * row_start[n_seq]. With row_start at multiples of block_tokens k_rows and v_rows
+ * are themselves pools of ikv_kv_batch, sequence s's blocks one behind the other
+ * from row_start[s] / block_tokens on: so ikv_attn_prefill_packed_paged_f32 attends
+ * over a history that is held in 8 bits. */
+int ikv_read_packed_q8(const ikv_kv_q8 *cache, float *k_rows, float *v_rows,
+                       const ikv_kv_batch *batch, const int32_t *row_start,
+                       const int32_t *first_token, const int32_t *n_kv, int64_t n_rows,
+                       void *stream);
+
+/* ikv_attn_decode_batch_f32 over such a cache; q and out are F32, sums and softmax
+ * F32. With k_new and v_new (F32 [n_seq][n_head_kv][head_dim]) row n_kv[s] - 1 of
+ * sequence s is quantised, written and attended to as it is held: the result is
+ * that of ikv_append_packed_q8 and a call without them. q, k_new, v_new and out
+ * 16-byte aligned (else -EINVAL). The workspace is used as there (zero-filled
+ * once; one of this form serves only this form). */
+size_t ikv_attn_decode_batch_q8_workspace_bytes(int n_head, int n_head_kv, int head_dim);
+
+int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_kv_batch *batch,
+                             const int32_t *n_kv, const float *k_new, const float *v_new,
+                             float *out, int n_head, float scale, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------
+ * ikv_attn_decode_batch_f32 where groups of sequences share their first blocks (a
+ * system prompt, one document under many questions): those blocks' keys are read
+ * once for a group, not once for each of its sequences.
+ *   group_start    [n_groups + 1] int32, ascending from 0 to n_seq: group g is the
+ *                  sequences [group_start[g], group_start[g + 1])
+ *   shared_blocks  [n_groups] int32: the leading entries that the tables of group
+ *                  g's sequences have in common; they are read from the table of
+ *                  the group's first sequence. 0: nothing is shared.
+ * Every sequence has a key of its own: one of n_kv[s] <= shared_blocks[g] *
+ * block_tokens that is not idle (0) raises IKV_STATUS_POSITION and is taken for 0,
+ * as is one of no group within [0, n_seq]. A group of a negative shared_blocks, or of
+ * more than the table's width, raises it, too, and shares nothing. Rows that k_new and v_new bring must not lie in blocks that any other
+ * sequence reads.
+ *   workspace  as for ikv_attn_decode_batch_f32 (zero-filled once), of
+ *              ikv_attn_decode_shared_workspace_bytes() bytes for at least these
+ *              n_seq and n_groups.
+ * Heads of over 128 dims, or of a number of dims that 4 does not divide, and
+ * operands that are not 16-byte aligned have their shared blocks read once for each
+ * sequence. n_groups 0: nothing is shared.
+ * ------------------------------------------------------------------- */
+size_t ikv_attn_decode_shared_workspace_bytes(int64_t n_seq, int64_t n_groups, int n_head,
+                                              int n_head_kv, int head_dim);
+
+int ikv_attn_decode_shared_f32(const float *q, float *k_pool, float *v_pool,
+                               const ikv_kv_batch *batch, const int32_t *group_start,
+                               const int32_t *shared_blocks, int64_t n_groups, const int32_t *n_kv,
+                               const float *k_new, const float *v_new, float *out, int n_head,
+                               int n_head_kv, int head_dim, float scale, void *workspace,
+                               size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

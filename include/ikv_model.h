@@ -122,6 +122,56 @@ int ikv_argmax_ws_f32(const float *logits, int64_t n, int32_t *token, int32_t *t
                       void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------
+ * Rules on each row of logits [n_rows][n_vocab] ahead of the samplers (the
+ * reference has none, src/sampler.cpp:42-65): penalties for the tokens of the row's
+ * history, biases, and a mask of the tokens that a grammar allows. For a token
+ * that the row's history holds, and holds c times behind the prompt,
+ *     x = x > 0 ? x / repetition : x * repetition
+ *     x = x - frequency * c - presence   (where c > 0)
+ * then x = x + bias, then x = -inf where the mask does not allow the token; in F32,
+ * other tokens' bits unchanged. out may equal logits (and overlaps it in no other
+ * way). Each part is left out where its array is NULL:
+ *   history        [n_rows][history_stride] token ids: the prompt's, then the
+ *                  generated ones; n_history [n_rows] of them (NULL: all), the
+ *                  first n_prompt [n_rows] (NULL: none) from the prompt
+ *   repetition, presence, frequency  [n_rows] (NULL: 1, 0, 0); computed with as
+ *                  they stand, whatever they are
+ *   bias_tokens, bias_values  [n_rows][bias_stride], n_bias [n_rows] of them (NULL:
+ *                  all); of several for one token the last one counts
+ *   masks          [n_masks][(n_vocab + 31) / 32] words, token t bit t % 32 of word
+ *                  t / 32, 1: allowed; mask_of [n_rows] says which (NULL: mask 0),
+ *                  a negative one: none
+ * All arrays are device memory, read by the kernel, so a captured call serves
+ * growing histories. An id outside [0, n_vocab) is skipped and raises
+ * IKV_STATUS_TOKEN in *status; an n_history or n_bias outside its list raises
+ * IKV_STATUS_POSITION and is taken for 0, a mask_of past the last mask raises it and
+ * allows no token. A row that allows none is all -inf, which the samplers answer
+ * with token -1.
+ * -EINVAL: no rules, a negative stride, values or masks missing; -EOVERFLOW:
+ * n_vocab or a stride past 2^30, n_rows past 2^21, n_rows * ceil(n_vocab / 2048)
+ * past 2^24 - 1.
+ * ------------------------------------------------------------------- */
+typedef struct ikv_logit_rules {
+    const int32_t *history;
+    int64_t history_stride;
+    const int32_t *n_history;
+    const int32_t *n_prompt;
+    const float *repetition;
+    const float *presence;
+    const float *frequency;
+    const int32_t *bias_tokens;
+    const float *bias_values;
+    int64_t bias_stride;
+    const int32_t *n_bias;
+    const uint32_t *masks;
+    int64_t n_masks;
+    const int32_t *mask_of;
+} ikv_logit_rules;
+
+int ikv_adjust_logits_f32(const float *logits, float *out, const ikv_logit_rules *rules,
+                          int64_t n_rows, int64_t n_vocab, int32_t *status, void *stream);
+
+/* ---------------------------------------------------------------------
  * Sampling of each row of logits [n_rows][n_vocab] from a given uniform number
  * u[row] in [0, 1) (the reference samples greedily, src/sampler.cpp:42-65).
  * With y_i = (x_i - max) / temperature and w_i = exp(y_i), tokens in the order

@@ -37,8 +37,7 @@
 // 32 over 1 76. Heads of over 128 dims, the same contexts: 8 of 200 over 4, 402 MB, 80
 // (61 at that rate), of 256 88 (78), 8 of 512 over 2 102 (78); loads of 4 bytes: 16 of
 // 65 over 8, 262 MB, 157 (40).
-#include "batch.hpp"
-#include "coherent.hpp"
+#include "decode_runs.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -52,7 +51,6 @@ constexpr int kWaves = 4;       // of a workgroup
 // rounds: 16 heads of 80 over 1, 64 contexts of 380 tokens 33 us, with 256 20; 32 of
 // up to 5448 59 and 53.
 constexpr int groups_of(int nv, int gq) { return gq > 4 && nv > 2 ? kCUs : 2 * kCUs; }
-constexpr int kRuns = 8 * kCUs;  // most runs of units
 constexpr int kRunUnits = 16;        // units of a run where there are more runs than workgroups
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int kMaxDim = 512;
@@ -82,120 +80,6 @@ __device__ __forceinline__ int keys_of(const Args &a, int seq) {
   return n > 0 && n <= a.b.capacity ? n : 0;
 }
 
-__device__ __forceinline__ unsigned long long wave_prefix(unsigned long long x) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const unsigned long long y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
-// x of lane l (the same for the whole wave), in scalar registers.
-__device__ __forceinline__ unsigned long long lane_value(unsigned long long x, int l) {
-  const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(x), l);
-  const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(x >> 32), l);
-  return static_cast<unsigned long long>(hi) << 32 | lo;
-}
-
-// A place in the list of units: unit `tile` of `tiles` of head pass `item`.
-struct Place {
-  int seq, keys, tiles, item, tile;
-};
-
-template <int KT, int GROUPS>
-struct Plan {
-  using Units = unsigned long long;
-  Units total, chunk;  // all units, those of a run
-  int runs, whole;
-  unsigned items;  // head passes of a sequence
-  // the sequence s0 + lane of 64: its keys, and the units up to its end
-  int s0, keys;
-  Units upto;
-
-  __device__ static int tiles_of(int keys) { return (keys + KT - 1) / KT; }
-
-  __device__ void look(const Args &a, int first, Units before) {
-    const int s = first + static_cast<int>(threadIdx.x & 63);
-    s0 = first;
-    keys = s < a.b.n_seq ? keys_of(a, s) : 0;
-    upto = before + wave_prefix(static_cast<Units>(tiles_of(keys)) * items);
-  }
-
-  __device__ Plan(const Args &a) : items(a.n_head_kv * a.passes) {
-    total = 0;
-    for (int s = 0; s < a.b.n_seq; s += 64) {
-      look(a, s, total);
-      total = lane_value(upto, 63);
-    }
-    runs = static_cast<int>(min(max(total / kRunUnits, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
-    chunk = (total + runs - 1) / runs;
-    if (chunk == 0) chunk = 1;
-    whole = chunk > 1 ? static_cast<int>(min(chunk, static_cast<Units>(4))) + 3 : kWhole;
-  }
-
-  // whether a (sequence, head) of so many units stays with one run: up to kWhole, and
-  // up to three more than a run has where those are two or more and it is no whole
-  // number of them (a run of two parts then has two starts and two joins): 16 heads
-  // of 128 over 8, 16 contexts of 300 tokens 18.2 -> 13.0 us, 24 of 380, two whole
-  // runs each, 18.8 split and 22.5 not; of 200, runs of one unit, 9.8 and 11.3; over
-  // ragged lengths between 10 % more and as much less.
-  __device__ bool kept(int tiles) const {
-    return tiles <= kWhole || (tiles <= whole && static_cast<unsigned>(tiles) % static_cast<unsigned>(chunk) != 0);
-  }
-
-  // where unit u (< total) is
-  __device__ Place at(const Args &a, Units u) {
-    if (a.b.n_seq > 64) {
-      Units before = 0;
-      for (int s = 0; s < a.b.n_seq; s += 64) {
-        look(a, s, before);
-        before = lane_value(upto, 63);
-        if (before > u) break;
-      }
-    }
-    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > u));
-    Place p;
-    p.seq = s0 + l;
-    p.keys = __builtin_amdgcn_readlane(keys, l);
-    p.tiles = tiles_of(p.keys);
-    const Units r = u - (lane_value(upto, l) - static_cast<Units>(p.tiles) * items);
-    if (r >> 32) {
-      p.item = static_cast<int>(r / p.tiles);
-      p.tile = static_cast<int>(r % p.tiles);
-    } else {
-      p.item = static_cast<int>(static_cast<unsigned>(r) / p.tiles);
-      p.tile = static_cast<int>(static_cast<unsigned>(r) % p.tiles);
-    }
-    p.item = __builtin_amdgcn_readfirstlane(p.item);
-    p.tile = __builtin_amdgcn_readfirstlane(p.tile);
-    return p;
-  }
-
-  // the first unit of the next head pass
-  __device__ void next(const Args &a, Place &p) {
-    p.tile = 0;
-    if (++p.item < static_cast<int>(items)) return;
-    p.item = 0;
-    const int lane = threadIdx.x & 63;
-    for (int first = s0;; first += 64) {
-      if (first != s0) {
-        if (first >= a.b.n_seq) return;  // (behind the last sequence: nobody goes on)
-        look(a, first, 0);               // (upto is not asked again)
-      }
-      const unsigned long long some = __builtin_amdgcn_ballot_w64(keys > 0 && first + lane > p.seq);
-      if (some) {
-        const int l = __builtin_ctzll(some);
-        p.seq = first + l;
-        p.keys = __builtin_amdgcn_readlane(keys, l);
-        p.tiles = tiles_of(p.keys);
-        return;
-      }
-    }
-  }
-};
-
 template <int LPK>
 __device__ __forceinline__ float lanes_sum(float x) {  // over a key's lanes
   x += ikv::dpp<ikv::kDppXor1>(x);
@@ -223,44 +107,15 @@ __device__ __forceinline__ float across_keys(float x, F &&f) {
   return f(__uint_as_float(c[0]), __uint_as_float(c[1]));
 }
 
-__device__ __forceinline__ float weight(float m, float top) {  // of sums kept at maximum m
-  return m == -INFINITY ? 0.f : ikv::fast_exp2(m - top);
-}
-
-// The workspace: a counter a run (of the parts of the head pass that begins in it
-// and goes on behind it) and one of the runs that were fetched, then (maximum,
-// sum) of each part's heads and their values. Part 2 r is run r's of a head pass
-// that began before it, 2 r + 1 of one that goes on behind it. Stored and read at agent scope, as
-// the parts come from several XCDs.
-constexpr size_t kCounterBytes = sizeof(int) * (kRuns + 64);
-template <int GQ, int DP>
-struct Parts {
-  int *counters;  // [kRuns], then the fetched runs'
-  float *ml, *o;
-  __device__ explicit Parts(float *p)
-      : counters(reinterpret_cast<int *>(p)), ml(p + kCounterBytes / sizeof(float)),
-        o(ml + static_cast<size_t>(kRuns) * 2 * GQ * 2) {}
-  __device__ float *ml_of(int part, int h) const { return ml + (static_cast<size_t>(part) * GQ + h) * 2; }
-  __device__ float *o_of(int part, int h) const { return o + (static_cast<size_t>(part) * GQ + h) * DP; }
-};
-
-__device__ __forceinline__ float2 load2(const float *p) {
-  const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p),
-                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float(static_cast<unsigned>(x)), __uint_as_float(static_cast<unsigned>(x >> 32)));
-}
-
 template <int LPK, int NV, int GQ, bool VEC>
 __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_kernel(Args a) {
   constexpr int KPW = 64 / LPK;               // keys that a wave loads at once
   constexpr int KT = kWaves * kAhead * KPW;   // keys of a unit
   constexpr int DP = LPK * NV * 4;            // dims held
   static_assert(64 % KT == 0, "a unit stays within a block");
-  __shared__ float s_m[kWaves][GQ], s_l[kWaves][GQ];
-  __shared__ __attribute__((aligned(16))) float s_o[kWaves][GQ][DP];
+  __shared__ ikv::Meet<GQ, DP, kWaves> s_meet;
   __shared__ float4 s_q[GQ][NV][LPK];  // the query rows, scaled
   __shared__ float4 s_new[2][NV][LPK];  // the new token's K and V row
-  __shared__ int s_last;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = lane % LPK, grp = lane / LPK;
@@ -277,8 +132,8 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   }
 
   constexpr int kGroups = groups_of(NV, GQ);
-  Plan<KT, kGroups> plan(a);
-  const Parts<GQ, DP> parts(a.part);
+  ikv::Plan<Args, KT, kGroups, kRunUnits, kWhole> plan(a);
+  const ikv::Parts<GQ, DP> parts(a.part);
   unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
@@ -316,23 +171,11 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
 
   int run = blockIdx.x;
   unsigned long long u = plan.chunk * run, end = min(plan.total, u + plan.chunk);
-  Place p{};
+  ikv::Place p{};
   if (u < end) p = plan.at(a, u);
   for (;;) {
     if (u >= end) {
-      // the next run that nobody has: the first come, first served, so that no
-      // workgroup is left with more than a run at the end. Every workgroup fetches
-      // until there is none, runs times in all; the last fetch clears the counter.
-      if (plan.runs <= kGroups) return;
-      if (threadIdx.x == 0) {
-        int *const fetched = parts.counters + kRuns;
-        const int before = __hip_atomic_fetch_add(fetched, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (before == plan.runs - 1) __hip_atomic_store(fetched, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = before;
-      }
-      __syncthreads();
-      run = kGroups + __builtin_amdgcn_readfirstlane(s_last);
-      __syncthreads();
+      run = ikv::next_run<kGroups>(plan, parts, s_meet);
       if (run >= plan.runs) return;
       u = plan.chunk * run;
       end = min(plan.total, u + plan.chunk);
@@ -443,7 +286,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
         float top = m[h];
 #pragma unroll
         for (int i = 0; i < N; ++i) top = fmaxf(top, s[i][h]);
-        const float f = weight(m[h], top);
+        const float f = ikv::weight(m[h], top);
         m[h] = top;
         sum[h] *= f;
 #pragma unroll
@@ -529,7 +372,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     for (int h = 0; h < GQ; ++h) {
       __builtin_amdgcn_sched_barrier(0);
       const float top = across_keys<LPK>(m[h], [](float x, float y) { return fmaxf(x, y); });
-      const float f = weight(m[h], top);
+      const float f = ikv::weight(m[h], top);
       auto add = [](float x, float y) { return x + y; };
       const float all = across_keys<LPK>(sum[h] * f, add);
 #pragma unroll
@@ -537,101 +380,19 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
         const float4 x = ikv::scale4(f, o[h][n]);
         const float4 y = make_float4(across_keys<LPK>(x.x, add), across_keys<LPK>(x.y, add),
                                      across_keys<LPK>(x.z, add), across_keys<LPK>(x.w, add));
-        if (grp == 0) *reinterpret_cast<float4 *>(&s_o[wave][h][4 * (l + LPK * n)]) = y;
+        if (grp == 0) *reinterpret_cast<float4 *>(&s_meet.o[wave][h][4 * (l + LPK * n)]) = y;
       }
       if (lane == 0) {
-        s_m[wave][h] = top;
-        s_l[wave][h] = all;
+        s_meet.m[wave][h] = top;
+        s_meet.l[wave][h] = all;
       }
     }
     __syncthreads();
-    const bool whole = p.tile == 0 && last == p.tiles;
-    const int part = 2 * run + (p.tile == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < heads * DP / 2; i += kWaves * 64) {
-      const int h = 2 * i / DP, d = 2 * i % DP;
-      float top = s_m[0][h];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_m[w][h]);
-      float all = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = weight(s_m[w][h], top);
-        all = fmaf(f, s_l[w][h], all);
-        x = fmaf(f, s_o[w][h][d], x);
-        y = fmaf(f, s_o[w][h][d + 1], y);
-      }
-      if (whole) {
-        float *const o = a.out + (head0 + h) * a.dim + d;
-        if (d < a.dim) o[0] = x / all;
-        if (d + 1 < a.dim) o[1] = y / all;
-      } else {
-        ikv::store2_agent(parts.o_of(part, h) + d, x, y);
-        if (d == 0) ikv::store2_agent(parts.ml_of(part, h), top, all);
-      }
-    }
-    if (!whole) {
-      // this thread's stores have completed before the workgroup is counted
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      __builtin_amdgcn_s_waitcnt(0);
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      __syncthreads();
-      // the head pass's first unit, its first run, its runs
-      const unsigned long long begin = u - p.tile;
-      const int w0 = static_cast<int>(begin / plan.chunk);
-      const int n = static_cast<int>((begin + p.tiles - 1) / plan.chunk) - w0 + 1;
-      if (threadIdx.x == 0) {
-        int *const counter = parts.counters + w0;
-        s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (s_last) {
-        auto at = [&](int i) { return i == 0 ? 2 * w0 + 1 : 2 * (w0 + i); };
-        for (int h = wave; h < heads; h += kWaves) {
-          float top = -INFINITY;
-          for (int i = lane; i < n; i += 64) top = fmaxf(top, load2(parts.ml_of(at(i), h)).x);
-          top = ikv::wave_max(top);
-          float all = 0.f;
-          for (int i = lane; i < n; i += 64) {
-            const float2 ml = load2(parts.ml_of(at(i), h));
-            all = fmaf(weight(ml.x, top), ml.y, all);
-          }
-          all = ikv::wave_sum(all);
-          if (lane == 0) {
-            s_m[0][h] = top;
-            s_l[0][h] = all;
-          }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < heads * DP / 2; i += kWaves * 64) {
-          const int h = 2 * i / DP, d = 2 * i % DP;
-          if (d >= a.dim) continue;
-          const float top = s_m[0][h], all = s_l[0][h];
-          float x = 0.f, y = 0.f;
-          constexpr int kParts = 8;  // loaded at once
-          for (int j = 0; j < n; j += kParts) {
-            float2 ml[kParts], v[kParts];
-#pragma unroll
-            for (int z = 0; z < kParts; ++z) {
-              const int e = at(min(j + z, n - 1));
-              ml[z] = load2(parts.ml_of(e, h));
-              v[z] = load2(parts.o_of(e, h) + d);
-            }
-#pragma unroll
-            for (int z = 0; z < kParts; ++z) {
-              const float f = j + z < n ? weight(ml[z].x, top) : 0.f;
-              if (j + z < n) {
-                x = fmaf(f, v[z].x, x);
-                y = fmaf(f, v[z].y, y);
-              }
-            }
-          }
-          float *const o = a.out + (head0 + h) * a.dim + d;
-          o[0] = x / all;
-          if (d + 1 < a.dim) o[1] = y / all;
-        }
-      }
-    }
+    ikv::leave(s_meet, plan, parts, run, u, p, last, heads, a.dim, [&](int h, int d, float, float all, float x, float y) {
+      float *const o = a.out + (head0 + h) * a.dim + d;
+      if (d < a.dim) o[0] = x / all;
+      if (d + 1 < a.dim) o[1] = y / all;
+    });
     __syncthreads();
     u += last - p.tile;
     plan.next(a, p);
@@ -665,7 +426,7 @@ int launch(const Args &a, bool vec, hipStream_t s) {
 extern "C" size_t ikv_attn_decode_batch_workspace_bytes(int n_head, int n_head_kv, int head_dim) {
   if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || head_dim > kMaxDim) return 0;
   const Form f = form_of(n_head / n_head_kv, head_dim);
-  return kCounterBytes + static_cast<size_t>(kRuns) * 2 * f.gq * (f.lpk * f.nv * 4 + 2) * sizeof(float);
+  return ikv::parts_bytes(f.gq, f.lpk * f.nv * 4);
 }
 
 extern "C" int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,

@@ -47,6 +47,28 @@ class KvBatch(ctypes.Structure):
 
 _c_batch = ctypes.POINTER(KvBatch)
 
+
+class KvQ8(ctypes.Structure):
+    """ikv_kv_q8 (include/ikv_batch.h): a paged cache of 8 bits an element."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_codes", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("format", ctypes.c_int32)]
+
+
+_c_q8 = ctypes.POINTER(KvQ8)
+
+
+class LogitRules(ctypes.Structure):
+    """ikv_logit_rules (include/ikv_model.h)."""
+    _fields_ = [("history", ctypes.c_void_p), ("history_stride", ctypes.c_int64),
+                ("n_history", ctypes.c_void_p), ("n_prompt", ctypes.c_void_p),
+                ("repetition", ctypes.c_void_p), ("presence", ctypes.c_void_p),
+                ("frequency", ctypes.c_void_p), ("bias_tokens", ctypes.c_void_p),
+                ("bias_values", ctypes.c_void_p), ("bias_stride", ctypes.c_int64),
+                ("n_bias", ctypes.c_void_p), ("masks", ctypes.c_void_p), ("n_masks", ctypes.c_int64),
+                ("mask_of", ctypes.c_void_p)]
+
 # name -> (restype, argtypes); include/ikv.h, ikv_batch.h, then ikv_model.h
 SIGNATURES = {
     "ikv_version": (ctypes.c_char_p, []),
@@ -156,6 +178,28 @@ SIGNATURES = {
         [_c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
          _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_size_t, _c_void_p],
     ),
+    "ikv_append_packed_q8": (
+        _c_int,
+        [_c_q8, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_int64, _c_void_p],
+    ),
+    "ikv_read_packed_q8": (
+        _c_int,
+        [_c_q8, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_void_p],
+    ),
+    "ikv_attn_decode_batch_q8_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
+    "ikv_attn_decode_batch_q8": (
+        _c_int,
+        [_c_void_p, _c_q8, _c_batch, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_float,
+         _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "ikv_attn_decode_shared_workspace_bytes": (
+        _c_size_t, [_c_int64, _c_int64, _c_int, _c_int, _c_int]),
+    "ikv_attn_decode_shared_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_batch, _c_void_p, _c_void_p, _c_int64, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_size_t,
+         _c_void_p],
+    ),
     # include/ikv_model.h
     "ikv_mul_mat_f32": (
         _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_void_p]),
@@ -180,6 +224,9 @@ SIGNATURES = {
     "ikv_argmax_workspace_bytes": (_c_size_t, []),
     "ikv_argmax_ws_f32": (
         _c_int, [_c_void_p, _c_int64, _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "ikv_adjust_logits_f32": (
+        _c_int,
+        [_c_void_p, _c_void_p, ctypes.POINTER(LogitRules), _c_int64, _c_int64, _c_void_p, _c_void_p]),
     "ikv_sample_workspace_bytes": (_c_size_t, [_c_int64, _c_int64]),
     "ikv_sample_f32": (
         _c_int,
@@ -799,6 +846,203 @@ def attn_decode_batch(q, k_pool, v_pool, tables, block_tokens: int, n_kv, *, k_n
     return out
 
 
+def decode_shared_workspace(n_seq: int, n_groups: int, n_head: int, n_head_kv: int, head_dim: int,
+                            device="cuda"):
+    """Zero-filled workspace of attn_decode_shared for up to so many sequences and
+    groups, of any lengths (reusable across ordered launches)."""
+    torch = _torch()
+    nbytes = int(load().ikv_attn_decode_shared_workspace_bytes(n_seq, n_groups, n_head, n_head_kv,
+                                                               head_dim))
+    return torch.zeros((nbytes + 3) // 4, dtype=torch.float32, device=device)
+
+
+def attn_decode_shared(q, k_pool, v_pool, tables, block_tokens: int, group_start, shared_blocks, n_kv,
+                       *, k_new=None, v_new=None, out=None, scale: float = 0.0, status=None,
+                       workspace=None, stream=None):
+    """attn_decode_batch where the sequences [group_start[g], group_start[g + 1]) of
+    each group have the first shared_blocks[g] blocks of their tables in common:
+    these are read once for all of them."""
+    torch = _torch()
+    dev = q.device
+    _operands(dev, (q, k_pool, v_pool, k_new, v_new, out, workspace),
+              "q k_pool v_pool k_new v_new out workspace",
+              (tables, group_start, shared_blocks, n_kv, status),
+              "tables group_start shared_blocks n_kv status")
+    n_seq, n_head, D = q.shape
+    n_head_kv = k_pool.shape[-2]
+    _need_pools(k_pool, v_pool, n_head_kv, D)
+    bt = kv_batch(tables, block_tokens, k_pool, status)
+    if bt.n_seq != n_seq or n_kv.numel() != n_seq:
+        raise ValueError("tables and n_kv must hold an entry per row of q")
+    n_groups = shared_blocks.numel()
+    if group_start.numel() != n_groups + 1:
+        raise ValueError("group_start must hold n_groups + 1 sequences")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_new is not None and (k_new.shape != (n_seq, n_head_kv, D) or v_new.shape != k_new.shape):
+        raise ValueError("k_new and v_new must hold one token row per sequence")
+    if out is not None and out.shape != q.shape:
+        raise ValueError("out must be of q's shape")
+    with _on(dev, stream):
+        if out is None:
+            out = torch.empty_like(q)
+        if workspace is None:
+            workspace = decode_shared_workspace(n_seq, n_groups, n_head, n_head_kv, D, device=dev)
+        _check("ikv_attn_decode_shared_f32",
+               load().ikv_attn_decode_shared_f32(
+                   _ptr(q), _ptr(k_pool), _ptr(v_pool), ctypes.byref(bt), _ptr(group_start),
+                   _ptr(shared_blocks), n_groups, _ptr(n_kv), _ptr(k_new), _ptr(v_new), _ptr(out),
+                   n_head, n_head_kv, D, scale, _ptr(workspace), workspace.numel() * 4,
+                   _raw_stream(dev)))
+    return out
+
+
+# ----------------------------------------------------------------------------
+# a cache of 8 bits an element: (k_codes, k_scales, v_codes, v_scales), codes int8 or
+# float8_e4m3fn [blocks, n_head_kv, block_tokens, D], scales float32 [blocks, n_head_kv,
+# block_tokens]
+# ----------------------------------------------------------------------------
+
+def cache_q8(n_blocks: int, block_tokens: int, n_head_kv: int, head_dim: int, dtype=None,
+             device="cuda"):
+    """A paged cache of 8 bits an element, of int8 codes or of `dtype`
+    torch.float8_e4m3fn."""
+    torch = _torch()
+    if dtype is None:
+        dtype = torch.int8
+    if dtype not in (torch.int8, torch.float8_e4m3fn):
+        raise TypeError(f"dtype must be int8 or float8_e4m3fn, got {dtype}")
+    shape = (n_blocks, n_head_kv, block_tokens, head_dim)
+    codes = [torch.zeros(shape, dtype=torch.int8, device=device).view(dtype) for _ in range(2)]
+    scales = [torch.zeros(shape[:-1], dtype=torch.float32, device=device) for _ in range(2)]
+    return codes[0], scales[0], codes[1], scales[1]
+
+
+def _cache_q8(cache, tables, status):
+    """The descriptors of a cache and of block tables over it, and its shape."""
+    torch = _torch()
+    k, k_scales, v, v_scales = cache
+    shape = k.shape
+    if k.dtype is torch.int8:
+        fmt = 0
+    elif k.dtype is torch.float8_e4m3fn:
+        fmt = 1
+    else:
+        raise TypeError(f"codes must be int8 or float8_e4m3fn, got {k.dtype}")
+    if v.dtype is not k.dtype:
+        raise TypeError(f"k and v codes must be of one type, got {k.dtype} and {v.dtype}")
+    if k.device != v.device or not k.is_cuda:
+        raise ValueError("codes must be on one GPU")
+    if len(shape) != 4 or v.shape != shape or k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
+        raise ValueError("codes must be [blocks, n_head_kv, block_tokens, head_dim], scales one less")
+    if not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("codes must be contiguous")
+    if tables.dim() != 2:
+        raise ValueError("tables must be [n_seq, blocks]")
+    n_seq, width = tables.shape
+    return (KvQ8(k.data_ptr(), k_scales.data_ptr(), v.data_ptr(), v_scales.data_ptr(), shape[1], shape[3], fmt),
+            KvBatch(tables.data_ptr(), width, shape[2], shape[0], n_seq, _ptr(status)), shape)
+
+
+def append_packed_q8(cache, k_rows, v_rows, tables, row_start, first_token=None, *, status=None,
+                     stream=None) -> None:
+    """append_packed into a cache of 8 bits an element (cache_q8)."""
+    dev = k_rows.device
+    _operands(dev, (k_rows, v_rows, cache[1], cache[3]), "k_rows v_rows k_scales v_scales",
+              (tables, row_start, first_token, status), "tables row_start first_token status")
+    q8, bt, shape = _cache_q8(cache, tables, status)
+    if cache[0].get_device() != dev.index:
+        raise ValueError("codes must be on the device of the others")
+    if k_rows.dim() != 3 or k_rows.shape != v_rows.shape or k_rows.shape[1:] != (shape[1], shape[3]):
+        raise ValueError("k_rows and v_rows must be [rows, n_head_kv, head_dim] of the cache's heads")
+    if row_start.numel() != bt.n_seq + 1:
+        raise ValueError("row_start must hold n_seq + 1 rows")
+    if first_token is not None and first_token.numel() != bt.n_seq:
+        raise ValueError("first_token must hold a token per sequence")
+    with _on(dev, stream):
+        _check("ikv_append_packed_q8",
+               load().ikv_append_packed_q8(ctypes.byref(q8), _ptr(k_rows), _ptr(v_rows),
+                                           ctypes.byref(bt), _ptr(row_start), _ptr(first_token),
+                                           k_rows.shape[0], _raw_stream(dev)))
+
+
+def read_packed_q8(cache, tables, row_start, n_rows: int, first_token=None, n_kv=None, *, k_rows=None,
+                   v_rows=None, status=None, stream=None):
+    """Rows [row_start[s], row_start[s + 1]) of (k_rows, v_rows) [n_rows, n_head_kv, D]
+    become the values of sequence s's tokens first_token[s].. (0.. without it), but
+    for those from n_kv[s] on. Rows of no token are left as k_rows and v_rows have
+    them (where they are allocated here: undefined)."""
+    torch = _torch()
+    dev = cache[1].device
+    _operands(dev, (cache[1], cache[3], k_rows, v_rows), "k_scales v_scales k_rows v_rows",
+              (tables, row_start, first_token, n_kv, status), "tables row_start first_token n_kv status")
+    q8, bt, shape = _cache_q8(cache, tables, status)
+    if cache[0].get_device() != dev.index:
+        raise ValueError("codes must be on the device of the others")
+    if row_start.numel() != bt.n_seq + 1:
+        raise ValueError("row_start must hold n_seq + 1 rows")
+    for t in (first_token, n_kv):
+        if t is not None and t.numel() != bt.n_seq:
+            raise ValueError("first_token and n_kv must hold a token per sequence")
+    rows = (n_rows, shape[1], shape[3])
+    for t in (k_rows, v_rows):
+        if t is not None and t.shape != rows:
+            raise ValueError("k_rows and v_rows must be [n_rows, n_head_kv, head_dim]")
+    with _on(dev, stream):
+        if k_rows is None:
+            k_rows = torch.empty(rows, dtype=torch.float32, device=dev)
+        if v_rows is None:
+            v_rows = torch.empty(rows, dtype=torch.float32, device=dev)
+        _check("ikv_read_packed_q8",
+               load().ikv_read_packed_q8(ctypes.byref(q8), _ptr(k_rows), _ptr(v_rows),
+                                         ctypes.byref(bt), _ptr(row_start), _ptr(first_token),
+                                         _ptr(n_kv), n_rows, _raw_stream(dev)))
+    return k_rows, v_rows
+
+
+def decode_batch_q8_workspace(n_head: int, n_head_kv: int, head_dim: int, device="cuda"):
+    """decode_batch_workspace of attn_decode_batch_q8."""
+    torch = _torch()
+    nbytes = int(load().ikv_attn_decode_batch_q8_workspace_bytes(n_head, n_head_kv, head_dim))
+    return torch.zeros((nbytes + 3) // 4, dtype=torch.float32, device=device)
+
+
+def attn_decode_batch_q8(q, cache, tables, n_kv, *, k_new=None, v_new=None, out=None,
+                         scale: float = 0.0, status=None, workspace=None, stream=None):
+    """attn_decode_batch over a cache of 8 bits an element (cache_q8): the new rows
+    are quantised, appended and attended to as they are held."""
+    torch = _torch()
+    dev = q.device
+    _operands(dev, (q, cache[1], cache[3], k_new, v_new, out, workspace),
+              "q k_scales v_scales k_new v_new out workspace", (tables, n_kv, status),
+              "tables n_kv status")
+    q8, bt, shape = _cache_q8(cache, tables, status)
+    n_seq, n_head, D = q.shape
+    if cache[0].get_device() != dev.index:
+        raise ValueError("codes must be on the device of the others")
+    if shape[3] != D:
+        raise ValueError("the cache's heads differ from q's")
+    if bt.n_seq != n_seq or n_kv.numel() != n_seq:
+        raise ValueError("tables and n_kv must hold an entry per row of q")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_new is not None and (k_new.shape != (n_seq, shape[1], D) or v_new.shape != k_new.shape):
+        raise ValueError("k_new and v_new must hold one token row per sequence")
+    if out is not None and out.shape != q.shape:
+        raise ValueError("out must be of q's shape")
+    with _on(dev, stream):
+        if out is None:
+            out = torch.empty_like(q)
+        if workspace is None:
+            workspace = decode_batch_q8_workspace(n_head, shape[1], D, device=dev)
+        _check("ikv_attn_decode_batch_q8",
+               load().ikv_attn_decode_batch_q8(
+                   _ptr(q), ctypes.byref(q8), ctypes.byref(bt), _ptr(n_kv), _ptr(k_new), _ptr(v_new),
+                   _ptr(out), n_head, scale, _ptr(workspace), workspace.numel() * 4,
+                   _raw_stream(dev)))
+    return out
+
+
 def rms_norm(x, w, eps: float, out=None, stream=None):
     torch = _torch()
     _need_f32_dev("x", x)
@@ -969,6 +1213,52 @@ def argmax_workspace(device=None):
     torch = _torch()
     n = int(load().ikv_argmax_workspace_bytes())
     return torch.zeros(n, dtype=torch.uint8, device=device or "cuda")
+
+
+def adjust_logits(logits, *, history=None, n_history=None, n_prompt=None, repetition=None,
+                  presence=None, frequency=None, bias_tokens=None, bias_values=None, n_bias=None,
+                  masks=None, mask_of=None, out=None, status=None, stream=None):
+    """The rows of logits [n_rows, n_vocab] with penalties for the first n_history[r]
+    tokens of history [n_rows, .] (repetition for all, presence and frequency for those
+    behind the first n_prompt[r]), with the first n_bias[r] of bias_values added at
+    bias_tokens [n_rows, .], and -inf where the bits of masks [n_masks, words] (int32
+    words of 32 tokens; row mask_of[r], none where that is negative) are 0. `out` may
+    be logits."""
+    torch = _torch()
+    dev = logits.device
+    _operands(dev, (logits, out, repetition, presence, frequency, bias_values),
+              "logits out repetition presence frequency bias_values",
+              (history, n_history, n_prompt, bias_tokens, n_bias, masks, mask_of, status),
+              "history n_history n_prompt bias_tokens n_bias masks mask_of status")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [n_rows, n_vocab]")
+    n_rows, n_vocab = logits.shape
+    for t in (n_history, n_prompt, repetition, presence, frequency, n_bias, mask_of):
+        if t is not None and t.numel() != n_rows:
+            raise ValueError("lengths, penalties and mask_of must hold a value per row")
+    for t in (history, bias_tokens):
+        if t is not None and (t.dim() != 2 or t.shape[0] != n_rows):
+            raise ValueError("history and bias_tokens must be [n_rows, tokens]")
+    if (bias_tokens is None) != (bias_values is None):
+        raise ValueError("bias_tokens and bias_values go together")
+    if bias_tokens is not None and bias_tokens.shape != bias_values.shape:
+        raise ValueError("bias_tokens and bias_values must be of one shape")
+    if masks is not None and (masks.dim() != 2 or masks.shape[1] != (n_vocab + 31) // 32):
+        raise ValueError("masks must be [n_masks, (n_vocab + 31) // 32]")
+    if out is not None and out.shape != logits.shape:
+        raise ValueError("out must be of logits' shape")
+    with _on(dev, stream):
+        if out is None:
+            out = torch.empty_like(logits)
+        rules = LogitRules(_ptr(history), 0 if history is None else history.shape[1], _ptr(n_history),
+                           _ptr(n_prompt), _ptr(repetition), _ptr(presence), _ptr(frequency),
+                           _ptr(bias_tokens), _ptr(bias_values),
+                           0 if bias_tokens is None else bias_tokens.shape[1], _ptr(n_bias),
+                           _ptr(masks), 0 if masks is None else masks.shape[0], _ptr(mask_of))
+        _check("ikv_adjust_logits_f32",
+               load().ikv_adjust_logits_f32(_ptr(logits), _ptr(out), ctypes.byref(rules), n_rows, n_vocab,
+                                            _ptr(status), _raw_stream(dev)))
+    return out
 
 
 def sample_workspace(n_rows: int, n_vocab: int, device="cuda"):
