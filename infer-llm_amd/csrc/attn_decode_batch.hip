@@ -38,6 +38,7 @@
 // (61 at that rate), of 256 88 (78), 8 of 512 over 2 102 (78); loads of 4 bytes: 16 of
 // 65 over 8, 262 MB, 157 (40).
 #include "decode_runs.hpp"
+#include "decode_shared.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -80,6 +81,13 @@ __device__ __forceinline__ int keys_of(const Args &a, int seq) {
   return n > 0 && n <= a.b.capacity ? n : 0;
 }
 
+// With the first keys of each sequence attended to already (decode_shared.hpp): what
+// is read here is behind them.
+struct SharedArgs : Args {
+  ikv::SharedParts shared;
+};
+__device__ __forceinline__ int keys_of(const SharedArgs &a, int seq) { return a.shared.seqs[seq].keys; }
+
 template <int LPK>
 __device__ __forceinline__ float lanes_sum(float x) {  // over a key's lanes
   x += ikv::dpp<ikv::kDppXor1>(x);
@@ -107,8 +115,9 @@ __device__ __forceinline__ float across_keys(float x, F &&f) {
   return f(__uint_as_float(c[0]), __uint_as_float(c[1]));
 }
 
-template <int LPK, int NV, int GQ, bool VEC>
-__global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_kernel(Args a) {
+template <int LPK, int NV, int GQ, bool VEC, class A>
+__global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_kernel(A a) {
+  constexpr bool SHARED = std::is_same_v<A, SharedArgs>;
   constexpr int KPW = 64 / LPK;               // keys that a wave loads at once
   constexpr int KT = kWaves * kAhead * KPW;   // keys of a unit
   constexpr int DP = LPK * NV * 4;            // dims held
@@ -126,13 +135,14 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   // (from the last workgroups on: in a small call they have nothing else to do)
   for (int s = gridDim.x - 1 - blockIdx.x; s < a.b.n_seq; s += gridDim.x) {
     if (keys_of(a, s) > 0) continue;
-    if (a.n_kv[s] != 0 && threadIdx.x == 0) ikv::raise_status(a.b.status, IKV_STATUS_POSITION);
+    if constexpr (!SHARED)  // (there the launch before has flagged it)
+      if (a.n_kv[s] != 0 && threadIdx.x == 0) ikv::raise_status(a.b.status, IKV_STATUS_POSITION);
     float *o = a.out + static_cast<size_t>(s) * n_head * a.dim;
     for (int d = threadIdx.x; d < n_head * a.dim; d += kWaves * 64) o[d] = 0.f;
   }
 
   constexpr int kGroups = groups_of(NV, GQ);
-  ikv::Plan<Args, KT, kGroups, kRunUnits, kWhole> plan(a);
+  ikv::Plan<A, KT, kGroups, kRunUnits, kWhole> plan(a);
   const ikv::Parts<GQ, DP> parts(a.part);
   unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
 #pragma unroll
@@ -192,7 +202,8 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
         plan.kept(p.tiles) ? p.tiles : static_cast<int>(min<unsigned long long>(p.tiles, p.tile + (end - u)));
     const int g = p.item / a.passes, h0 = p.item % a.passes * GQ;
     const int heads = min(GQ, a.G - h0);
-    const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
+    ikv::Pages pg = ikv::pages_of(a.b, p.seq);
+    if constexpr (SHARED) pg.table += a.shared.seqs[p.seq].shared / pg.bt;
     const size_t head0 = static_cast<size_t>(p.seq) * n_head + g * a.G + h0;
     float4 o[GQ][NV];
     float m[GQ], sum[GQ];
@@ -388,8 +399,13 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
       }
     }
     __syncthreads();
-    ikv::leave(s_meet, plan, parts, run, u, p, last, heads, a.dim, [&](int h, int d, float, float all, float x, float y) {
+    ikv::leave(s_meet, plan, parts, run, u, p, last, heads, a.dim, [&](int h, int d, float top, float all, float x, float y) {
       float *const o = a.out + (head0 + h) * a.dim + d;
+      if constexpr (SHARED) {
+        const float2 both = ikv::join_shared(a.shared, p.seq, g, h0 + h, d, top, all, x, y);
+        if (d < a.dim) *reinterpret_cast<float2 *>(o) = both;
+        return;
+      }
       if (d < a.dim) o[0] = x / all;
       if (d + 1 < a.dim) o[1] = y / all;
     });
@@ -420,6 +436,48 @@ int launch(const Args &a, bool vec, hipStream_t s) {
     decode_batch_kernel<LPK, NV, GQ, false><<<groups_of(NV, GQ), kWaves * 64, 0, s>>>(a);
   return ikv::launch_status();
 }
+template <int LPK, int NV, int GQ>
+int launch(const SharedArgs &a, bool, hipStream_t s) {
+  decode_batch_kernel<LPK, NV, GQ, true><<<groups_of(NV, GQ), kWaves * 64, 0, s>>>(a);
+  return ikv::launch_status();
+}
+
+template <int LPK, int NV, class A>
+int launch_heads(const A &a, int gq, bool vec, hipStream_t s) {
+  switch (gq) {
+    case 1: return launch<LPK, NV, 1>(a, vec, s);
+    case 2: return launch<LPK, NV, 2>(a, vec, s);
+    case 4: return launch<LPK, NV, 4>(a, vec, s);
+    default: return launch<LPK, NV, 8>(a, vec, s);
+  }
+}
+// (up to 128 dims)
+template <class A>
+int launch_narrow(const A &a, const Form &f, bool vec, hipStream_t s) {
+  if (f.nv == 4) return launch_heads<8, 4>(a, f.gq, vec, s);
+  if (f.nv == 3) return launch_heads<8, 3>(a, f.gq, vec, s);
+  if (f.nv == 2) return launch_heads<8, 2>(a, f.gq, vec, s);
+  return launch_heads<8, 1>(a, f.gq, vec, s);
+}
+
+void set_args(Args &a, const float *q, float *k_pool, float *v_pool, const int32_t *n_kv, const float *k_new,
+              const float *v_new, float *out, int n_head, int n_head_kv, int head_dim, float scale, void *workspace) {
+  const int G = n_head / n_head_kv, gq = form_of(G, head_dim).gq;
+  if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
+  a.q = q;
+  a.k = k_pool;
+  a.v = v_pool;
+  a.k_new = k_new;
+  a.v_new = v_new;
+  a.out = out;
+  a.n_kv = n_kv;
+  a.n_head_kv = n_head_kv;
+  a.G = G;
+  a.dim = head_dim;
+  a.passes = (G + gq - 1) / gq;
+  a.scale_log2 = scale * ikv::kLog2e;
+  a.part = static_cast<float *>(workspace);
+}
 
 }  // namespace
 
@@ -445,40 +503,29 @@ extern "C" int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v
     return -EINVAL;
   // a unit's rows are one buffer range; a sequence's heads index in int
   if (n_head_kv > INT_MAX / (64 * 4) / head_dim || n_head > INT_MAX / head_dim) return -EOVERFLOW;
-  const int G = n_head / n_head_kv;
-  const Form f = form_of(G, head_dim);
-  if (!(scale > 0.0f)) scale = 1.0f / sqrtf(static_cast<float>(head_dim));
-  a.q = q;
-  a.k = k_pool;
-  a.v = v_pool;
-  a.k_new = k_new;
-  a.v_new = v_new;
-  a.out = out;
-  a.n_kv = n_kv;
-  a.n_head_kv = n_head_kv;
-  a.G = G;
-  a.dim = head_dim;
-  a.passes = (G + f.gq - 1) / f.gq;
-  a.scale_log2 = scale * ikv::kLog2e;
-  a.part = static_cast<float *>(workspace);
+  const Form f = form_of(n_head / n_head_kv, head_dim);
+  set_args(a, q, k_pool, v_pool, n_kv, k_new, v_new, out, n_head, n_head_kv, head_dim, scale, workspace);
   bool vec = head_dim % 4 == 0;
   for (const void *x : {static_cast<const void *>(q), static_cast<const void *>(k_pool),
                         static_cast<const void *>(v_pool), static_cast<const void *>(k_new),
                         static_cast<const void *>(v_new)})
     vec = vec && ikv::aligned16(x);
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define IKV_GQ(LPK, NV)                                 \
-  switch (f.gq) {                                       \
-    case 1: return launch<LPK, NV, 1>(a, vec, s);       \
-    case 2: return launch<LPK, NV, 2>(a, vec, s);       \
-    case 4: return launch<LPK, NV, 4>(a, vec, s);       \
-    default: return launch<LPK, NV, 8>(a, vec, s);      \
-  }
-  if (f.lpk == 32) IKV_GQ(32, 4)
-  if (f.lpk == 16) IKV_GQ(16, 4)
-  if (f.nv == 4) IKV_GQ(8, 4)
-  if (f.nv == 3) IKV_GQ(8, 3)
-  if (f.nv == 2) IKV_GQ(8, 2)
-  IKV_GQ(8, 1)
-#undef IKV_GQ
+  if (f.lpk == 32) return launch_heads<32, 4>(a, f.gq, vec, s);
+  if (f.lpk == 16) return launch_heads<16, 4>(a, f.gq, vec, s);
+  return launch_narrow(a, f, vec, s);
 }
+
+namespace ikv {
+
+int decode_behind_shared(const float *q, float *k_pool, float *v_pool, const BatchPages &b, const float *k_new,
+                         const float *v_new, float *out, int n_head, int n_head_kv, int head_dim, float scale,
+                         void *workspace, const SharedParts &parts, hipStream_t s) {
+  SharedArgs a;
+  a.b = b;
+  a.shared = parts;
+  set_args(a, q, k_pool, v_pool, nullptr, k_new, v_new, out, n_head, n_head_kv, head_dim, scale, workspace);
+  return launch_narrow(a, form_of(n_head / n_head_kv, head_dim), true, s);
+}
+
+}  // namespace ikv
