@@ -79,7 +79,10 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
   constexpr int DP = 64 * W;  // dims held
   constexpr int DB = 4 * W;   // of V, of a lane
   __shared__ ikv::Meet<GQ, DP, kWaves> s_meet;
+  constexpr int kSteps = 2 * W;  // of 32 dims (a lane's 8: 16 (quad + 4 w) + 8 z)
   __shared__ __attribute__((aligned(16))) uint8_t s_new[2][DP];  // the new token's codes
+  __shared__ bf16x8 s_q[kSteps][3][64];  // the query rows' pieces, as the lanes take them
+  __shared__ __attribute__((aligned(16))) float s_scale[kWaves][2][KT];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -133,27 +136,6 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
     const ikv::Pages pg = ikv::pages_of(a.b, p.seq);
     const size_t head0 = static_cast<size_t>(p.seq) * n_head + g * a.G + h0;
 
-    // the query rows' pieces: dims 16 (quad + 4 w) + 8 z .. + 7 of this lane's head
-    bf16x8 qp[W][2][3];
-    {
-      const float *const row = a.q + (head0 + min(col, heads - 1)) * dim;
-      unsigned none = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const int d = 16 * (quad + 4 * w);
-        floatx4 x[4] = {};
-        if (col < heads && d < dim) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const floatx4 *>(row + d + 4 * e) * a.scale_log2;
-        }
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const Pieces s = split8<false>(x[2 * z], x[2 * z + 1], none);
-#pragma unroll
-          for (int i = 0; i < 3; ++i) qp[w][z][i] = s.p[i];
-        }
-      }
-    }
     floatx4 o[DB];
 #pragma unroll
     for (int j = 0; j < DB; ++j) o[j] = floatx4{};
@@ -178,22 +160,22 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
     auto next_row = [&]() -> int64_t {
       const int e = __builtin_amdgcn_readlane(ent, blk - ent0);
       const int64_t row = ikv::row_q8(max(e, 0), a.n_head_kv, g, pg.bt, in_blk);
-      in_blk += kWaves * KT;
+      in_blk = ikv::uniform(in_blk + kWaves * KT);
       while (in_blk >= pg.bt) {
         in_blk -= pg.bt;
         ++blk;
       }
       if (blk - ent0 >= 64) entries();
-      return e < 0 ? ~row : row;
+      return ikv::uniform(e < 0 ? ~row : row);
     };
     uint4 kr[4][W];
     unsigned vr[2][8][W];
-    floatx4 ks[4], vs[4];
+    float ks, vs;  // of key `lane`
     auto rsrc = [&](const void *base, int64_t byte, int bytes) {
       return __builtin_amdgcn_make_buffer_rsrc(static_cast<uint8_t *>(const_cast<void *>(base)) + byte, 0, bytes,
                                                ikv::kBufWord3);
     };
-    auto rows_of = [&](int t) { return t < last ? max(0, min(KT, cached - t * KT)) : 0; };
+    auto rows_of = [&](int t) { return ikv::uniform(t < last ? max(0, min(KT, cached - t * KT)) : 0); };
     auto fetch_k = [&](int64_t row, int t) {
       const int rows = rows_of(t);
       row = row < 0 ? ~row : row;
@@ -205,10 +187,7 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
         for (int w = 0; w < W; ++w)
           kr[T][w] = __builtin_bit_cast(
               uint4, __builtin_amdgcn_raw_buffer_load_b128(r, k_off[w] + (32 * (T >> 1) + 4 * (T & 1)) * dim, 0, 0));
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        ks[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                rs, 4 * (32 * (i >> 1) + 8 * quad + 4 * (i & 1)), 0, 0));
+      ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, 4 * lane, 0, 0));
     };
     auto fetch_v = [&](int64_t row, int t) {
       const int rows = rows_of(t);
@@ -230,48 +209,68 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
             vr[z][i][0] = x.x, vr[z][i][1] = x.y, vr[z][i][2] = x.z, vr[z][i][3] = x.w;
           }
         }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vs[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                rs, 4 * (32 * (i >> 1) + 8 * quad + 4 * (i & 1)), 0, 0));
+      vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, 4 * lane, 0, 0));
     };
 
-    if (t0 < last) {
-      entries();
-      // the new token: its codes and scales, by the wave that has the last unit
-      float new_scale[2] = {0.f, 0.f};
-      const bool mine = has_new && (p.tiles - 1 - t0) % kWaves == 0;
-      if (mine) {
-        const size_t row = (static_cast<size_t>(p.seq) * a.n_head_kv + g) * dim;
-        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-        const bool there = 4 * lane < dim;
-        const float4 x[2] = {there ? *reinterpret_cast<const float4 *>(a.k_new + row + 4 * lane) : none,
-                             there ? *reinterpret_cast<const float4 *>(a.v_new + row + 4 * lane) : none};
+    entries();
+    // the query rows, a step a wave
+    floatx4 qr[(kSteps + kWaves - 1) / kWaves][2] = {};
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const ikv::Quant<E4M3> quant(ikv::lanes_max<64>(
-              max(max(ikv::abs_bits(x[z].x), ikv::abs_bits(x[z].y)), max(ikv::abs_bits(x[z].z), ikv::abs_bits(x[z].w)))));
-          new_scale[z] = quant.scale;
-          if (4 * lane < DP) *reinterpret_cast<unsigned *>(&s_new[z][4 * lane]) = quant.codes(x[z]);
-        }
-        const int e = pg.table[last_blk];
-        if (h0 == 0 && static_cast<unsigned>(e) < static_cast<unsigned>(pg.n_blocks)) {
-          const int64_t to = ikv::row_q8(e, a.n_head_kv, g, pg.bt, (p.keys - 1) % pg.bt);
-          if (there) {
-            *reinterpret_cast<unsigned *>(a.c.k + to * dim + 4 * lane) = *reinterpret_cast<const unsigned *>(&s_new[0][4 * lane]);
-            *reinterpret_cast<unsigned *>(a.c.v + to * dim + 4 * lane) = *reinterpret_cast<const unsigned *>(&s_new[1][4 * lane]);
-          }
-          if (lane == 0) {
-            a.c.k_scale[to] = new_scale[0];
-            a.c.v_scale[to] = new_scale[1];
-          }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+    for (int i = 0; i < (kSteps + kWaves - 1) / kWaves; ++i) {
+      const int step = wave + kWaves * i, d = 16 * (quad + 4 * (step >> 1)) + 8 * (step & 1);
+      const float *const row = a.q + (head0 + min(col, heads - 1)) * dim;
+      if (step < kSteps && col < heads && d < dim) {
+        qr[i][0] = *reinterpret_cast<const floatx4 *>(row + d);
+        qr[i][1] = *reinterpret_cast<const floatx4 *>(row + d + 4);
       }
-      int64_t row = next_row();
-      fetch_k(row, t0);
-      fetch_v(row, t0);
+    }
+    // the new token: its codes and scales, by the wave that has the last unit
+    float new_scale[2] = {0.f, 0.f};
+    const bool mine = has_new && t0 < last && (p.tiles - 1 - t0) % kWaves == 0;
+    float4 new_row[2] = {};
+    if (mine && 4 * lane < dim) {
+      const size_t at = (static_cast<size_t>(p.seq) * a.n_head_kv + g) * dim + 4 * lane;
+      new_row[0] = *reinterpret_cast<const float4 *>(a.k_new + at);
+      new_row[1] = *reinterpret_cast<const float4 *>(a.v_new + at);
+    }
+    int64_t row = next_row();
+    fetch_k(row, t0);
+    fetch_v(row, t0);
+#pragma unroll
+    for (int i = 0; i < (kSteps + kWaves - 1) / kWaves; ++i) {
+      const int step = wave + kWaves * i;
+      if (step >= kSteps) break;
+      unsigned none = 0;
+      const Pieces x = split8<false>(qr[i][0] * a.scale_log2, qr[i][1] * a.scale_log2, none);
+#pragma unroll
+      for (int z = 0; z < 3; ++z) s_q[step][z][lane] = x.p[z];
+    }
+    if (mine) {
+      unsigned codes[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const float4 x = new_row[z];
+        const ikv::Quant<E4M3> quant(ikv::lanes_max<64>(
+            max(max(ikv::abs_bits(x.x), ikv::abs_bits(x.y)), max(ikv::abs_bits(x.z), ikv::abs_bits(x.w)))));
+        new_scale[z] = quant.scale;
+        codes[z] = quant.codes(x);
+        if (4 * lane < DP) *reinterpret_cast<unsigned *>(&s_new[z][4 * lane]) = codes[z];
+      }
+      const int e = pg.table[last_blk];
+      if (h0 == 0 && static_cast<unsigned>(e) < static_cast<unsigned>(pg.n_blocks)) {
+        const int64_t to = ikv::row_q8(e, a.n_head_kv, g, pg.bt, (p.keys - 1) % pg.bt);
+        if (4 * lane < dim) {
+          *reinterpret_cast<unsigned *>(a.c.k + to * dim + 4 * lane) = codes[0];
+          *reinterpret_cast<unsigned *>(a.c.v + to * dim + 4 * lane) = codes[1];
+        }
+        if (lane == 0) {
+          a.c.k_scale[to] = new_scale[0];
+          a.c.v_scale[to] = new_scale[1];
+        }
+      }
+    }
+    __syncthreads();
+    {
       for (int t = t0; t < last; t += kWaves) {
         const bool fresh = mine && t == p.tiles - 1;
         const int at = cached - t * KT;  // the new token's place in the unit
@@ -290,25 +289,37 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
 #pragma unroll
                 for (int w = 0; w < W; ++w)
                   vr[z][i][w] = *reinterpret_cast<const unsigned *>(&s_new[1][DB * col + 4 * w]);
-                ks[2 * z + (i >> 2)][i & 3] = new_scale[0];
-                vs[2 * z + (i >> 2)][i & 3] = new_scale[1];
               }
+          if (lane == at) {
+            ks = new_scale[0];
+            vs = new_scale[1];
+          }
         }
+        s_scale[wave][0][lane] = ks;
+        s_scale[wave][1][lane] = vs;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        auto scales = [&](int z, int T) {  // of this lane's keys of tile T
+          return *reinterpret_cast<const floatx4 *>(&s_scale[wave][z][32 * (T >> 1) + 8 * quad + 4 * (T & 1)]);
+        };
         // scores of keys 32 (T / 2) + 8 quad + 4 (T % 2) + e with this lane's head
-        floatx4 s[4];
+        floatx4 s[4] = {};
 #pragma unroll
-        for (int T = 0; T < 4; ++T) {
-          s[T] = floatx4{};
+        for (int w = 0; w < W; ++w)
 #pragma unroll
-          for (int w = 0; w < W; ++w)
+          for (int z = 0; z < 2; ++z) {
+            bf16x8 qp[3];
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
+            for (int i = 0; i < 3; ++i) qp[i] = s_q[2 * w + z][i][lane];
+#pragma unroll
+            for (int T = 0; T < 4; ++T) {
               const bf16x8 x = bf16_of<E4M3>(z == 0 ? make_uint2(kr[T][w].x, kr[T][w].y) : make_uint2(kr[T][w].z, kr[T][w].w));
 #pragma unroll
-              for (int i = 2; i >= 0; --i) s[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qp[w][z][i], s[T], 0, 0, 0);
+              for (int i = 2; i >= 0; --i) s[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qp[i], s[T], 0, 0, 0);
             }
-          s[T] *= ks[T];
-        }
+          }
+#pragma unroll
+        for (int T = 0; T < 4; ++T) s[T] *= scales(0, T);
         row = next_row();
         fetch_k(row, t + kWaves);
         const int keys = p.keys - t * KT;
@@ -337,13 +348,15 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
         for (int z = 0; z < 2; ++z) {
           floatx4 x[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i) {
+            const floatx4 scale = scales(1, 2 * z + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float w = ikv::fast_exp2(s[2 * z + i][e] - ref);
               sum += w;
-              x[i][e] = w * vs[2 * z + i][e];
+              x[i][e] = w * scale[e];
             }
+          }
           unsigned none = 0;
           const Pieces pw = split8<false>(x[0], x[1], none);
 #pragma unroll

@@ -52,6 +52,15 @@ __device__ __forceinline__ Pages pages_of(const BatchPages &b, int seq) {
   return Pages{b.tables + seq * b.stride, b.bt, b.n_blocks, b.status};
 }
 
+// A value that the whole wave has, in scalar registers, where the compiler does not
+// see it: a buffer resource of vector registers is looped over, load by load.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
+  const int hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
+  return static_cast<int64_t>(hi) << 32 | lo;
+}
+
 // The last i in [0, n) for which at_most(i) holds, or -1, for a predicate that
 // holds up to some i and not behind it; by a whole wave, 64 probes a round (two
 // rounds up to 4096). Whatever the predicate says, the result is in [-1, n).
