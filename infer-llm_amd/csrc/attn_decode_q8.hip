@@ -30,7 +30,7 @@ using namespace ikv::pieces;
 
 constexpr int kWaves = 4;  // of a workgroup
 constexpr int KT = 64;     // keys of a unit
-constexpr int kRunUnits = 32, kWhole = 8;  // (decode_runs.hpp)
+constexpr int kRunUnits = 64, kWhole = 8;  // (decode_runs.hpp)
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int groups_of(int w) { return w > 2 ? 256 : 512; }
 
@@ -143,7 +143,9 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
 
     // block table entries, 64 at a time, one per lane, checked as they are read
     const int last_blk = (p.keys - 1) / pg.bt;
-    const int t0 = p.tile + wave;  // this wave's units: t0, t0 + kWaves, ...
+    // this wave's units, t0, t0 + kWaves, ..., those of its number in the whole list: each
+    // wave has as many of a run as any other, or one more
+    const int t0 = p.tile + ((wave - static_cast<int>(u)) & (kWaves - 1));
     int blk = t0 * KT / pg.bt, in_blk = t0 * KT % pg.bt, ent0 = blk, ent = 0;
     auto entries = [&]() {
       ent0 = blk;
@@ -175,41 +177,44 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
       return __builtin_amdgcn_make_buffer_rsrc(static_cast<uint8_t *>(const_cast<void *>(base)) + byte, 0, bytes,
                                                ikv::kBufWord3);
     };
-    auto rows_of = [&](int t) { return ikv::uniform(t < last ? max(0, min(KT, cached - t * KT)) : 0); };
-    auto fetch_k = [&](int64_t row, int t) {
-      const int rows = rows_of(t);
+    // A unit's resources: codes and scales; of a unit behind the run no memory is read.
+    // The row part of an offset is not checked against the size: rows behind the last
+    // token are read (they are in the block) and masked.
+    struct Unit {
+      __amdgpu_buffer_rsrc_t k, v, ks, vs;
+    };
+    auto unit_at = [&](int64_t row, int t) {
+      const int rows = ikv::uniform(t < last ? max(0, min(KT, cached - t * KT)) : 0);
       row = row < 0 ? ~row : row;
-      const auto r = rsrc(a.c.k, row * dim, rows * dim);
-      const auto rs = rsrc(a.c.k_scale, row * 4, rows * 4);
+      return Unit{rsrc(a.c.k, row * dim, rows * dim), rsrc(a.c.v, row * dim, rows * dim),
+                  rsrc(a.c.k_scale, row * 4, rows * 4), rsrc(a.c.v_scale, row * 4, rows * 4)};
+    };
+    auto fetch_k = [&](const Unit &r, int h) {  // the keys 32 h .. + 31
 #pragma unroll
-      for (int T = 0; T < 4; ++T)
+      for (int T = 2 * h; T < 2 * h + 2; ++T)
 #pragma unroll
         for (int w = 0; w < W; ++w)
           kr[T][w] = __builtin_bit_cast(
-              uint4, __builtin_amdgcn_raw_buffer_load_b128(r, k_off[w] + (32 * (T >> 1) + 4 * (T & 1)) * dim, 0, 0));
-      ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, 4 * lane, 0, 0));
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(r.k, k_off[w], (32 * h + 4 * (T & 1)) * dim, 0));
     };
-    auto fetch_v = [&](int64_t row, int t) {
-      const int rows = rows_of(t);
-      row = row < 0 ? ~row : row;
-      const auto r = rsrc(a.c.v, row * dim, rows * dim);
-      const auto rs = rsrc(a.c.v_scale, row * 4, rows * 4);
+    auto fetch_v = [&](const Unit &r, int h) {
 #pragma unroll
-      for (int z = 0; z < 2; ++z)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const unsigned at = v_off + (32 * z + i) * dim;
-          if constexpr (W == 1) {
-            vr[z][i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
-          } else if constexpr (W == 2) {
-            const auto x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
-            vr[z][i][0] = x.x, vr[z][i][1] = x.y;
-          } else {
-            const auto x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
-            vr[z][i][0] = x.x, vr[z][i][1] = x.y, vr[z][i][2] = x.z, vr[z][i][3] = x.w;
-          }
+      for (int i = 0; i < 8; ++i) {
+        const int at = (32 * h + i) * dim;
+        if constexpr (W == 1) {
+          vr[h][i][0] = __builtin_amdgcn_raw_buffer_load_b32(r.v, v_off, at, 0);
+        } else if constexpr (W == 2) {
+          const auto x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r.v, v_off, at, 0));
+          vr[h][i][0] = x.x, vr[h][i][1] = x.y;
+        } else {
+          const auto x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r.v, v_off, at, 0));
+          vr[h][i][0] = x.x, vr[h][i][1] = x.y, vr[h][i][2] = x.z, vr[h][i][3] = x.w;
         }
-      vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, 4 * lane, 0, 0));
+      }
+    };
+    auto fetch_scales = [&](const Unit &r) {
+      ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r.ks, 4 * lane, 0, 0));
+      vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r.vs, 4 * lane, 0, 0));
     };
 
     entries();
@@ -233,9 +238,14 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
       new_row[0] = *reinterpret_cast<const float4 *>(a.k_new + at);
       new_row[1] = *reinterpret_cast<const float4 *>(a.v_new + at);
     }
-    int64_t row = next_row();
-    fetch_k(row, t0);
-    fetch_v(row, t0);
+    {
+      const Unit r = unit_at(next_row(), t0);
+      fetch_scales(r);
+      fetch_k(r, 0);
+      fetch_k(r, 1);
+      fetch_v(r, 0);
+      fetch_v(r, 1);
+    }
 #pragma unroll
     for (int i = 0; i < (kSteps + kWaves - 1) / kWaves; ++i) {
       const int step = wave + kWaves * i;
@@ -270,8 +280,7 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
       }
     }
     __syncthreads();
-    {
-      for (int t = t0; t < last; t += kWaves) {
+    for (int t = t0; t < last; t += kWaves) {
         const bool fresh = mine && t == p.tiles - 1;
         const int at = cached - t * KT;  // the new token's place in the unit
         if (fresh) {
@@ -303,25 +312,31 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
           return *reinterpret_cast<const floatx4 *>(&s_scale[wave][z][32 * (T >> 1) + 8 * quad + 4 * (T & 1)]);
         };
         // scores of keys 32 (T / 2) + 8 quad + 4 (T % 2) + e with this lane's head
+        // each half of the codes is loaded again as soon as it is in the products
+        const Unit r = unit_at(next_row(), t + kWaves);
+        fetch_scales(r);
         floatx4 s[4] = {};
 #pragma unroll
-        for (int w = 0; w < W; ++w)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
+          for (int step = 0; step < kSteps; ++step) {
             bf16x8 qp[3];
 #pragma unroll
-            for (int i = 0; i < 3; ++i) qp[i] = s_q[2 * w + z][i][lane];
+            for (int i = 0; i < 3; ++i) qp[i] = s_q[step][i][lane];
 #pragma unroll
-            for (int T = 0; T < 4; ++T) {
-              const bf16x8 x = bf16_of<E4M3>(z == 0 ? make_uint2(kr[T][w].x, kr[T][w].y) : make_uint2(kr[T][w].z, kr[T][w].w));
+            for (int T = 2 * h; T < 2 * h + 2; ++T) {
+              const uint4 y = kr[T][step / 2];
+              const bf16x8 x = bf16_of<E4M3>(step % 2 == 0 ? make_uint2(y.x, y.y) : make_uint2(y.z, y.w));
 #pragma unroll
               for (int i = 2; i >= 0; --i) s[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qp[i], s[T], 0, 0, 0);
             }
           }
+          __builtin_amdgcn_sched_barrier(0);
+          fetch_k(r, h);
+          __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int T = 0; T < 4; ++T) s[T] *= scales(0, T);
-        row = next_row();
-        fetch_k(row, t + kWaves);
         const int keys = p.keys - t * KT;
         if (keys < KT) {
 #pragma unroll
@@ -329,6 +344,15 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (32 * (T >> 1) + 8 * quad + 4 * (T & 1) + e >= keys) s[T][e] = -INFINITY;
+          // (a weight of 0 would not silence a NaN)
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (32 * z + 8 * quad + i >= keys) {
+#pragma unroll
+                for (int w = 0; w < W; ++w) vr[z][i][w] = 0;
+              }
         }
         float mt = s[0][0];
 #pragma unroll
@@ -375,9 +399,10 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
                 o[4 * w + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pw.p[i], o[4 * w + d], 0, 0, 0);
             }
           }
+          __builtin_amdgcn_sched_barrier(0);
+          fetch_v(r, z);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        fetch_v(row, t + kWaves);
-      }
     }
 
     // the waves meet: this lane has dims DB (4 quad + e) + j of its head
