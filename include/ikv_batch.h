@@ -237,7 +237,7 @@ int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_k
  *   workspace  as for ikv_attn_decode_batch_f32 (zero-filled once), of
  *              ikv_attn_decode_shared_workspace_bytes() bytes for at least these
  *              n_seq and n_groups.
- * Heads of over 128 dims, or of a number of dims that 4 does not divide, and
+ * Heads of over 128 dims, or of a number of dims that 8 does not divide, and
  * operands that are not 16-byte aligned have their shared blocks read once for each
  * sequence. n_groups 0: nothing is shared.
  * ------------------------------------------------------------------- */

@@ -169,8 +169,15 @@ struct Plan {
     p.tiles = __builtin_amdgcn_readlane(tiles, l);
     p.items = __builtin_amdgcn_readlane(items, l);
     const Units r = u - (ikv::lane_value(upto, l) - static_cast<Units>(p.tiles) * p.items);
-    p.item = __builtin_amdgcn_readfirstlane(static_cast<int>(r / p.tiles));
-    p.tile = __builtin_amdgcn_readfirstlane(static_cast<int>(r % p.tiles));
+    if (r >> 32) {
+      p.item = static_cast<int>(r / p.tiles);
+      p.tile = static_cast<int>(r % p.tiles);
+    } else {
+      p.item = static_cast<int>(static_cast<unsigned>(r) / p.tiles);
+      p.tile = static_cast<int>(static_cast<unsigned>(r) % p.tiles);
+    }
+    p.item = ikv::uniform(p.item);
+    p.tile = ikv::uniform(p.tile);
     first = __builtin_amdgcn_readlane(item_upto, l) - p.items;
     return p;
   }
@@ -210,7 +217,8 @@ __device__ __forceinline__ float pair_sum(float x) {
 template <int DT, int RB>
 __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
   constexpr int KG = kWaves / RB, R = 32 * RB, DP = 32 * DT, KJ = 4 * DT;
-  __shared__ float s_x[KG > 1 ? (KG - 1) * RB * (16 * DT + 2) * 64 : 1];  // the key groups' states
+  __shared__ float s_x[kWaves * (16 * DT + 2) * 64];  // the waves' states
+  __shared__ floatx4 s_q[RB][KJ][64];  // the query rows, scaled, as the lanes take them
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave / RB, rb = wave % RB;
@@ -226,11 +234,10 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
   const int run = static_cast<int>(blockIdx.x % 8 * (kRuns / 8) + blockIdx.x / 8);
   unsigned long long u = plan.chunk * run;
   const unsigned long long end = min(plan.total, u + plan.chunk);
-  unsigned k_off[KJ];  // this lane's pieces of a tile's K rows and its dims of the V rows
+  // this lane's pieces of a tile's K rows, j 32 bytes further each, and its dims of the V rows
   constexpr unsigned kOut = 0x80000000u;
-#pragma unroll
-  for (int j = 0; j < KJ; ++j)
-    k_off[j] = 8 * j + 4 * c2 < a.dim ? static_cast<unsigned>(r32 * stride + 8 * j + 4 * c2) * 4u : kOut;
+  const unsigned k_off = static_cast<unsigned>(r32 * stride + 4 * c2) * 4u;
+  auto piece = [&](int j) { return j < KJ - 3 || 8 * j < a.dim; };  // whether there is a j
   unsigned v_off[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i)
@@ -246,23 +253,13 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
     const bool row_ok = row - row0 < rows;
     const bool busy = 32 * rb < rows;  // whether this wave has rows
 
-    floatx4 qf[KJ];
-    if (busy) {
-      const int seq = p.g.first + min(row, p.g.seqs * a.G - 1) / a.G, h = min(row, p.g.seqs * a.G - 1) % a.G;
-      const float *const qr = a.q + (static_cast<size_t>(seq) * a.n_head_kv * a.G + g * a.G + h) * a.dim;
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        qf[j] = floatx4{};
-        if (row_ok && 8 * j + 4 * c2 < a.dim) qf[j] = *reinterpret_cast<const floatx4 *>(qr + 8 * j + 4 * c2) * a.scale_log2;
-      }
-    }
     floatx16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = floatx16{};
     float m = -INFINITY, sum = 0.f;
 
     const int t0 = p.tile + kg;
-    if (busy && t0 < last) {
+    {
       const int32_t *const table = a.b.tables + p.g.first * a.b.stride;
       int blk = t0 * BN / a.b.bt, in_blk = t0 * BN % a.b.bt, ent0 = 0, ent = 0;
       auto entries = [&]() {
@@ -274,6 +271,16 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
         }
       };
       entries();
+      constexpr int kMine = (KJ + KG - 1) / KG;  // of the rows' pieces: j = kg, kg + KG, ...
+      floatx4 qr[kMine] = {};
+      if (row_ok) {
+        const int at = row % a.G;
+        const float *const from =
+            a.q + (static_cast<size_t>(p.g.first + row / a.G) * a.n_head_kv * a.G + g * a.G + at) * a.dim + 4 * c2;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if (kg + KG * i < KJ && piece(kg + KG * i)) qr[i] = *reinterpret_cast<const floatx4 *>(from + 8 * (kg + KG * i));
+      }
       auto next_row = [&]() -> long long {  // the tile's row of the pools, moved on to the next one
         const long long r = static_cast<long long>(__builtin_amdgcn_readlane(ent, blk - ent0)) * a.b.bt + in_blk;
         in_blk += KG * BN;
@@ -286,33 +293,53 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
       };
       auto rsrc = [&](const float *base, long long r, int t) {  // (none of a tile behind the run)
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base + r * stride + g * a.dim), 0,
-                                                 t < last ? ((BN - 1) * stride + a.dim) * 4 : 0, ikv::kBufWord3);
+                                                 busy && t < last ? ((BN - 1) * stride + a.dim) * 4 : 0, ikv::kBufWord3);
       };
       floatx4 kf[KJ];
       float vf[16][DT];
-      auto load_k = [&](long long r, int t) {
-        const auto x = rsrc(a.k, r, t);
-#pragma unroll
-        for (int j = 0; j < KJ; ++j)
-          kf[j] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(x, k_off[j], 0, 0));
+      auto load_k = [&](__amdgpu_buffer_rsrc_t x, int j) {
+        kf[j] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(x, piece(j) ? k_off + 32 * j : kOut, 0, 0));
       };
-      auto load_v = [&](long long r, int t) {
-        const auto x = rsrc(a.v, r, t);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          load_dims<DT>(x, v_off, static_cast<unsigned>((8 * (e >> 2) + (e & 3)) * stride * 4), vf[e]);
+      auto load_v = [&](__amdgpu_buffer_rsrc_t x, int e) {
+        load_dims<DT>(x, v_off, static_cast<unsigned>((8 * (e >> 2) + (e & 3)) * stride * 4), vf[e]);
       };
-      long long r = next_row();
-      load_k(r, t0);
-      load_v(r, t0);
-      for (int t = t0; t < last; t += KG) {
+      {
+        const long long r = next_row();
+        const auto rk = rsrc(a.k, r, t0), rv = rsrc(a.v, r, t0);
+        // (in the order of the loop's: else its first product waits for what was loaded
+        // last, here as there)
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          load_k(rk, j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          load_v(rv, e);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (kg + KG * i < KJ) s_q[rb][kg + KG * i][lane] = qr[i] * a.scale_log2;
+      __syncthreads();
+      for (int t = t0; busy && t < last; t += KG) {
+        // (each piece of the next tile's as soon as this one's is in the product)
+        const long long r = next_row();
+        const auto rk = rsrc(a.k, r, t + KG), rv = rsrc(a.v, r, t + KG);
         floatx16 s{};
+        floatx4 next = s_q[rb][0][lane];
 #pragma unroll
-        for (int j = 0; j < KJ; ++j)
+        for (int j = 0; j < KJ; ++j) {
+          const floatx4 qf = next;
+          if (j + 1 < KJ) next = s_q[rb][j + 1][lane];
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j][e], qf[j][e], s, 0, 0, 0);
-        r = next_row();
-        load_k(r, t + KG);
+          for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j][e], qf[e], s, 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          load_k(rk, j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         float mt = s[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[e]);
@@ -325,66 +352,72 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
           for (int i = 0; i < DT; ++i) o[i] *= f;
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float w[16];
+        // (a weight is formed behind the products of the one before it)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          w[e] = ikv::fast_exp2(s[e] - ref);
-          sum += w[e];
+          const float w = ikv::fast_exp2(s[e] - ref);
+          sum += w;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[e][i], w, o[i], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          load_v(rv, e);
+          __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-#pragma unroll
-          for (int i = 0; i < DT; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[e][i], w[e], o[i], 0, 0, 0);
-        load_v(r, t + KG);
       }
     }
     sum = pair_sum(sum);
-    if constexpr (KG > 1) {  // groups 1 .. hand their states to group 0
-      constexpr int XW = 16 * DT + 2;
-      if (kg > 0) {
-        float *const x = s_x + ((kg - 1) * RB + rb) * XW * 64 + lane;
+    // the key groups' states meet in LDS; a wave joins and stores every KG-th part of
+    // its rows' dims
+    constexpr int XW = 16 * DT + 2;
+    {
+      float *const x = s_x + (kg * RB + rb) * XW * 64 + lane;
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
+      for (int i = 0; i < DT; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[(16 * i + e) * 64] = o[i][e];
-        x[16 * DT * 64] = m;
-        x[(16 * DT + 1) * 64] = sum;
+        for (int e = 0; e < 16; ++e) x[(16 * i + e) * 64] = o[i][e];
+      x[16 * DT * 64] = m;
+      x[(16 * DT + 1) * 64] = sum;
+    }
+    __syncthreads();
+    const int slot = item0 + p.item + run;
+    if (row_ok && slot < a.slots) {  // (all of them, unless the groups overlap)
+      const size_t at = static_cast<size_t>(slot) * R + 32 * rb + r32;
+      float f[KG], top = -INFINITY, all = 0.f;
+#pragma unroll
+      for (int z = 0; z < KG; ++z) {
+        f[z] = s_x[((z * RB + rb) * XW + 16 * DT) * 64 + lane];
+        top = fmaxf(top, f[z]);
       }
-      __syncthreads();
-      if (kg == 0) {
 #pragma unroll
-        for (int z = 1; z < KG; ++z) {
-          const float *const x = s_x + ((z - 1) * RB + rb) * XW * 64 + lane;
-          const float mb = x[16 * DT * 64], top = fmaxf(m, mb);
-          const float fa = ikv::weight(m, top), fb = ikv::weight(mb, top);
-          sum = sum * fa + x[(16 * DT + 1) * 64] * fb;
+      for (int z = 0; z < KG; ++z) {
+        f[z] = ikv::weight(f[z], top);
+        all = fmaf(f[z], s_x[((z * RB + rb) * XW + 16 * DT + 1) * 64 + lane], all);
+      }
+      if (kg == 0 && c2 == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(top, all);
+      // four of a lane's 16 DT values at a time: rows 8 q + 4 c2 .. + 3 of a product
+      for (int z0 = kg; z0 < 4; z0 += KG) {
 #pragma unroll
-          for (int i = 0; i < DT; ++i)
+        for (int e = 0; e < 4; ++e) {
+          float v[DT] = {};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][e] = o[i][e] * fa + x[(16 * i + e) * 64] * fb;
-          m = top;
+          for (int z = 0; z < KG; ++z)
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+              v[i] = fmaf(f[z], s_x[((z * RB + rb) * XW + 16 * i + 4 * z0 + e) * 64 + lane], v[i]);
+          const int mrow = 8 * z0 + 4 * c2 + e;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) a.o[at * DP + dim_of<DT>(mrow, i)] = v[i];
         }
       }
-      __syncthreads();
     }
-    const int slot = item0 + p.item + run;
-    if (kg == 0 && row_ok && slot < a.slots) {  // (all, unless the groups overlap)
-      const size_t at = static_cast<size_t>(slot) * R + 32 * rb + r32;
-      if (c2 == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(m, sum);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int mrow = 8 * (e >> 2) + 4 * c2 + (e & 3);
-#pragma unroll
-        for (int i = 0; i < DT; ++i) a.o[at * DP + dim_of<DT>(mrow, i)] = o[i][e];
-      }
-    }
+    __syncthreads();
     u += last - p.tile;
   }
 }
 
 // Whether the matrix kernel takes these operands.
 bool on_matrices(int head_dim, std::initializer_list<const void *> operands) {
-  if (head_dim % 4 != 0 || head_dim > 128) return false;
+  if (head_dim % 8 != 0 || head_dim > 128) return false;
   for (const void *p : operands)
     if (!ikv::aligned16(p)) return false;
   return true;
@@ -408,7 +441,7 @@ struct Space {
   Space(int64_t n_seq, int64_t n_groups, int n_head, int n_head_kv, int head_dim) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     seqs = up(ikv_attn_decode_batch_workspace_bytes(n_head, n_head_kv, head_dim));
-    if (head_dim % 4 != 0 || head_dim > 128) {  // the lengths alone
+    if (head_dim % 8 != 0 || head_dim > 128) {  // the lengths alone
       all = seqs + static_cast<size_t>(n_seq) * sizeof(int32_t);
       return;
     }
