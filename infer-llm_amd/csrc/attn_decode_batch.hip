@@ -203,7 +203,11 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     const int g = p.item / a.passes, h0 = p.item % a.passes * GQ;
     const int heads = min(GQ, a.G - h0);
     ikv::Pages pg = ikv::pages_of(a.b, p.seq);
-    if constexpr (SHARED) pg.table += a.shared.seqs[p.seq].shared / pg.bt;
+    ikv::SharedSeq behind;
+    if constexpr (SHARED) {
+      behind = a.shared.seqs[p.seq];
+      pg.table += behind.shared / pg.bt;
+    }
     const size_t head0 = static_cast<size_t>(p.seq) * n_head + g * a.G + h0;
     float4 o[GQ][NV];
     float m[GQ], sum[GQ];
@@ -402,8 +406,9 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
     ikv::leave(s_meet, plan, parts, run, u, p, last, heads, a.dim, [&](int h, int d, float top, float all, float x, float y) {
       float *const o = a.out + (head0 + h) * a.dim + d;
       if constexpr (SHARED) {
-        const float2 both = ikv::join_shared(a.shared, p.seq, g, h0 + h, d, top, all, x, y);
-        if (d < a.dim) *reinterpret_cast<float2 *>(o) = both;
+        if (d >= a.dim) return;
+        const ikv::SharedRow row(a.shared, behind, g, h0 + h);
+        *reinterpret_cast<float2 *>(o) = ikv::join_shared(a.shared, row, d, top, all, x, y);
         return;
       }
       if (d < a.dim) o[0] = x / all;

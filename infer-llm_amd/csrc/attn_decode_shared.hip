@@ -53,10 +53,14 @@ __device__ __forceinline__ Group group_of(const ikv::BatchPages &b, const Groups
   return {first, end - first, blocks >= 0 && blocks <= b.stride ? blocks : 0};
 }
 
-// A sequence's keys and group: by a thread.
-__device__ __forceinline__ ikv::SharedSeq seq_of(const ikv::BatchPages &b, const Groups &groups, const int32_t *n_kv,
-                                                 int seq, int G) {
-  ikv::SharedSeq s{0, 0, 0, 0};
+// A sequence's keys and group (-1: none): by a thread.
+struct Keys {
+  int own, shared, group, row;  // row: its first of the group's
+};
+__device__ __forceinline__ Keys keys_of(const ikv::BatchPages &b, const Groups &groups, const int32_t *n_kv, int seq,
+                                        int G) {
+  Keys s{0, 0, -1, 0};
+  const int n = n_kv[seq];
   bool found = groups.n == 0, bad = false;
   if (groups.n > 0) {
     int lo = 0, hi = groups.n;  // the last group that begins at or before seq is in [lo, hi)
@@ -76,9 +80,8 @@ __device__ __forceinline__ ikv::SharedSeq seq_of(const ikv::BatchPages &b, const
       bad = groups.blocks[lo] != g.blocks;
     }
   }
-  const int n = n_kv[seq];
   if (found && n > s.shared && n <= b.capacity)
-    s.keys = n - s.shared;
+    s.own = n - s.shared;
   else
     bad |= n != 0;
   if (bad) ikv::raise_status(b.status, IKV_STATUS_POSITION);
@@ -91,8 +94,8 @@ __global__ __launch_bounds__(kThreads) void shared_lengths_kernel(ikv::BatchPage
                                                                   const int32_t *n_kv, int32_t *keys) {
   const int seq = blockIdx.x * kThreads + threadIdx.x;
   if (seq >= b.n_seq) return;
-  const ikv::SharedSeq s = seq_of(b, groups, n_kv, seq, 1);
-  keys[seq] = s.keys > 0 ? s.shared + s.keys : 0;
+  const Keys s = keys_of(b, groups, n_kv, seq, 1);
+  keys[seq] = s.own > 0 ? s.shared + s.own : 0;
 }
 
 struct Args {
@@ -103,15 +106,13 @@ struct Args {
   int n_head_kv, G, dim;
   float scale_log2;
   ikv::SharedSeq *seqs;
-  ikv::SharedGroup *group;
-  unsigned long long *chunk;
   float *ml, *o;
   int slots;
 };
 
-// A place in the list of tiles: tile `tile` of `tiles` of item `item` of a group.
+// A place in the list of tiles: tile `tile` of `tiles` of item `item` of group g.
 struct Place {
-  int group, item, tile, tiles, items;
+  int item, tile, tiles, items;
   Group g;
 };
 
@@ -136,18 +137,35 @@ struct Plan {
     upto = before + ikv::wave_prefix(static_cast<Units>(items) * tiles);
     item_upto = items_before + static_cast<int>(ikv::wave_prefix(items));
   }
-  __device__ explicit Plan(const Args &a, ikv::SharedGroup *write) {
+  __device__ explicit Plan(const Args &a) {
     total = 0;
-    int n = 0;
-    for (int s = 0; s < a.groups.n; s += 64) {
+    for (int s = 0, n = 0; s < a.groups.n; s += 64) {
       look(a, s, total, n);
-      const int i = s + static_cast<int>(threadIdx.x & 63);
-      if (write && i < a.groups.n)
-        write[i] = {upto - static_cast<Units>(items) * tiles, item_upto - items, tiles};
       total = ikv::lane_value(upto, 63);
       n = __builtin_amdgcn_readlane(item_upto, 63);
     }
     chunk = max((total + kRuns - 1) / kRuns, Units{kWaves});
+  }
+  // what the next launch has to know of a lane's sequence
+  __device__ ikv::SharedSeq about(const Args &a, const Keys &k) {
+    ikv::SharedSeq x{k.own, k.shared, k.row, 0, 0, chunk, 0, {}};
+    Units before = 0;
+    for (int s = 0, n = 0; s < a.groups.n; s += 64) {
+      if (a.groups.n > 64) look(a, s, before, n);
+      const int l = k.group - s;
+      const bool here = l >= 0 && l < 64;
+      const Units b = upto - static_cast<Units>(items) * tiles;
+      const unsigned lo = __shfl(static_cast<unsigned>(b), l & 63, 64), hi = __shfl(static_cast<unsigned>(b >> 32), l & 63, 64);
+      const int first = __shfl(item_upto - items, l & 63, 64), each = __shfl(tiles, l & 63, 64);
+      if (here) {
+        x.begin = static_cast<Units>(hi) << 32 | lo;
+        x.item = first;
+        x.tiles = each;
+      }
+      before = ikv::lane_value(upto, 63);
+      n = __builtin_amdgcn_readlane(item_upto, 63);
+    }
+    return x;
   }
   // where unit u (< total) is; `first`: the item's place among all
   __device__ Place at(const Args &a, Units u, int &first) {
@@ -163,7 +181,6 @@ struct Plan {
     }
     const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > u));
     Place p;
-    p.group = g0 + l;
     p.g = {__builtin_amdgcn_readlane(g.first, l), __builtin_amdgcn_readlane(g.seqs, l),
            __builtin_amdgcn_readlane(g.blocks, l)};
     p.tiles = __builtin_amdgcn_readlane(tiles, l);
@@ -225,10 +242,13 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
   const int r32 = lane & 31, c2 = lane >> 5;
   const int stride = a.n_head_kv * a.dim;
 
-  for (int s = blockIdx.x * kThreads + threadIdx.x; s < a.b.n_seq; s += gridDim.x * kThreads)
-    a.seqs[s] = seq_of(a.b, a.groups, a.n_kv, s, a.G);
-  Plan<R> plan(a, blockIdx.x == 0 && wave == 0 ? a.group : nullptr);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.chunk = plan.chunk;
+  Plan<R> plan(a);
+  // (by whole waves, from the last workgroups on: in a small call they have no run)
+  for (int s0 = (gridDim.x - 1 - blockIdx.x) * kThreads + 64 * wave; s0 < a.b.n_seq; s0 += gridDim.x * kThreads) {
+    const int seq = min(s0 + lane, a.b.n_seq - 1);
+    const ikv::SharedSeq x = plan.about(a, keys_of(a.b, a.groups, a.n_kv, seq, a.G));
+    if (s0 + lane < a.b.n_seq) a.seqs[seq] = x;
+  }
 
   // runs of one XCD next to each other: they read the same KV heads
   const int run = static_cast<int>(blockIdx.x % 8 * (kRuns / 8) + blockIdx.x / 8);
@@ -437,7 +457,7 @@ int64_t part_rows(int64_t n_seq, int64_t n_groups, int G, int n_head_kv) {
 
 // The workspace behind that of the batched decode, in bytes.
 struct Space {
-  size_t seqs, group, chunk, ml, o, all;
+  size_t seqs, ml, o, all;
   Space(int64_t n_seq, int64_t n_groups, int n_head, int n_head_kv, int head_dim) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     seqs = up(ikv_attn_decode_batch_workspace_bytes(n_head, n_head_kv, head_dim));
@@ -446,9 +466,7 @@ struct Space {
       return;
     }
     const size_t rows = static_cast<size_t>(part_rows(n_seq, n_groups, n_head / n_head_kv, n_head_kv));
-    group = up(seqs + n_seq * sizeof(ikv::SharedSeq));
-    chunk = up(group + n_groups * sizeof(ikv::SharedGroup));
-    ml = chunk + 256;
+    ml = up(seqs + n_seq * sizeof(ikv::SharedSeq));
     o = up(ml + rows * 2 * sizeof(float));
     all = o + rows * dims_of(head_dim) * sizeof(float);
   }
@@ -504,8 +522,6 @@ extern "C" int ikv_attn_decode_shared_f32(const float *q, float *k_pool, float *
   a.dim = head_dim;
   a.scale_log2 = scale * ikv::kLog2e;
   a.seqs = reinterpret_cast<ikv::SharedSeq *>(space + at.seqs);
-  a.group = reinterpret_cast<ikv::SharedGroup *>(space + at.group);
-  a.chunk = reinterpret_cast<unsigned long long *>(space + at.chunk);
   a.ml = reinterpret_cast<float *>(space + at.ml);
   a.o = reinterpret_cast<float *>(space + at.o);
   const int rb = blocks_of(n_seq, n_groups, a.G);
@@ -526,7 +542,7 @@ extern "C" int ikv_attn_decode_shared_f32(const float *q, float *k_pool, float *
   else
     launch(std::integral_constant<int, 4>{});
   if (const int rc = ikv::launch_status()) return rc;
-  const ikv::SharedParts parts{a.seqs, a.group, a.chunk, a.ml, a.o, 32 * rb, dims, a.slots, n_head_kv};
+  const ikv::SharedParts parts{a.seqs, a.ml, a.o, 32 * rb, dims, a.slots, n_head_kv};
   return ikv::decode_behind_shared(q, k_pool, v_pool, a.b, k_new, v_new, out, n_head, n_head_kv, head_dim, scale,
                                    workspace, parts, s);
 }
