@@ -56,6 +56,12 @@ constexpr int kRunUnits = 16;        // units of a run where there are more runs
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int kMaxDim = 512;
 constexpr int kWhole = 3;  // units of a (sequence, head) that are not split anywhere
+// The same behind shared keys, where most sequences have few units of their own and a
+// (sequence, head) costs its start and its join, whatever it holds: runs of two units,
+// taken as workgroups come free (48 sequences of up to 1500 keys of their own, 32 heads
+// of 128, 52.6 -> 39.5 us; 37 of up to 511, heads of 64, 14.1, runs of one workgroup's
+// share or of two; five units whole 15.6 there).
+constexpr int kSharedUnits = 2, kSharedWhole = 4;
 // Cache policy of a load: rows of the pools are read once (non-temporal: 48 long
 // contexts of the 8B heads 410 -> 373 us).
 constexpr std::integral_constant<int, 0> kKept{};
@@ -142,7 +148,7 @@ __global__ __launch_bounds__(kWaves * 64, GQ <= 4 ? 2 : 1) void decode_batch_ker
   }
 
   constexpr int kGroups = groups_of(NV, GQ);
-  ikv::Plan<A, KT, kGroups, kRunUnits, kWhole> plan(a);
+  ikv::Plan<A, KT, kGroups, SHARED ? kSharedUnits : kRunUnits, SHARED ? kSharedWhole : kWhole> plan(a);
   const ikv::Parts<GQ, DP> parts(a.part);
   unsigned off[NV];  // of this lane's pieces in a row; out of range past head_dim
 #pragma unroll
