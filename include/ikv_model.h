@@ -148,8 +148,8 @@ int ikv_argmax_ws_f32(const float *logits, int64_t n, int32_t *token, int32_t *t
  * allows no token. A row that allows none is all -inf, which the samplers answer
  * with token -1.
  * -EINVAL: no rules, a negative stride, values or masks missing; -EOVERFLOW:
- * n_vocab or a stride past 2^30, n_rows past 2^21, n_rows * ceil(n_vocab / 2048)
- * past 2^24 - 1.
+ * n_vocab or a stride past 2^30, n_rows past 2^21, n_rows * ceil(n_vocab / 4096)
+ * past 2^23 - 1.
  * ------------------------------------------------------------------- */
 typedef struct ikv_logit_rules {
     const int32_t *history;

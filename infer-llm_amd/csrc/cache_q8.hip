@@ -33,12 +33,13 @@ __global__ __launch_bounds__(kRowWaves * 64) void append_q8_kernel(
       ikv::raise_status(b.status, IKV_STATUS_POSITION);
       continue;
     }
-    const int blk = b.tables[seq * b.stride + t / b.bt];
+    const int in_table = static_cast<unsigned>(t) / static_cast<unsigned>(b.bt);
+    const int at = static_cast<int>(t) - in_table * b.bt;
+    const int blk = b.tables[seq * b.stride + in_table];
     if (static_cast<unsigned>(blk) >= static_cast<unsigned>(b.n_blocks)) {
       ikv::raise_status(b.status, IKV_STATUS_BLOCK);  // dropped: no block to write
       continue;
     }
-    const int at = static_cast<int>(t % b.bt);
     const float *const kr = k_rows + i * c.n_head_kv * c.dim, *const vr = v_rows + i * c.n_head_kv * c.dim;
     for (int g0 = 0; g0 < c.n_head_kv; g0 += kHeads * kAhead) {
       float4 x[2][kAhead];
@@ -88,12 +89,13 @@ __global__ __launch_bounds__(kRowWaves * 64) void read_q8_kernel(
       ikv::raise_status(b.status, IKV_STATUS_POSITION);
       continue;
     }
-    int blk = b.tables[seq * b.stride + t / b.bt];
+    const int in_table = static_cast<unsigned>(t) / static_cast<unsigned>(b.bt);
+    const int at = static_cast<int>(t) - in_table * b.bt;
+    int blk = b.tables[seq * b.stride + in_table];
     if (static_cast<unsigned>(blk) >= static_cast<unsigned>(b.n_blocks)) {
       ikv::raise_status(b.status, IKV_STATUS_BLOCK);
       blk = 0;
     }
-    const int at = static_cast<int>(t % b.bt);
     float *const kr = k_rows + i * c.n_head_kv * c.dim, *const vr = v_rows + i * c.n_head_kv * c.dim;
     for (int g0 = 0; g0 < c.n_head_kv; g0 += kHeads * kAhead) {
       unsigned w[2][kAhead];

@@ -15,9 +15,11 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kSlice = 4096;  // tokens of a workgroup
-constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;  // of 256 threads: 2^32 in a launch
+constexpr int kPer = kSlice / kThreads;
+constexpr int kAhead = 4;  // tokens of a history that a thread loads at once
+constexpr int64_t kMaxWorkgroups = (1 << 23) - 1;  // of 512 threads: 2^32 in a launch
 
 struct Args {
   const float *logits;
@@ -51,77 +53,101 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(Args a) {
       none = true;
       if (first == 0 && tid == 0) ikv::raise_status(a.status, IKV_STATUS_POSITION);
     } else if (which >= 0) {
-      mask = a.r.masks + which * a.mask_words;
+      mask = a.r.masks + which * a.mask_words + first / 32;
     }
   }
-  if (n_history > 0 || n_bias > 0) {
-    for (int i = tid; i < kSlice; i += kThreads) {
-      s_seen[i] = 0;
-      s_bias[i] = 0;
+  const float repetition = a.r.repetition ? a.r.repetition[row] : 1.0f;
+  const float presence = a.r.presence ? a.r.presence[row] : 0.0f;
+  const float frequency = a.r.frequency ? a.r.frequency[row] : 0.0f;
+
+  // this thread's logits and mask words, on their way while the lists are gone over
+  constexpr int E = VEC ? 4 : 1;
+  auto place = [&](int j) { return E * (tid + kThreads * (j / E)) + j % E; };
+  const float *const x = a.logits + row * a.n_vocab + first;
+  float *const y = a.out + row * a.n_vocab + first;
+  float v[kPer];
+  unsigned word[kPer / E];
+#pragma unroll
+  for (int j = 0; j < kPer; j += E) {
+    const int i = place(j);
+    word[j / E] = none ? 0u : ~0u;
+    if (i >= n) continue;
+    if constexpr (VEC) {
+      const float4 z = *reinterpret_cast<const float4 *>(x + i);
+      v[j] = z.x, v[j + 1] = z.y, v[j + 2] = z.z, v[j + 3] = z.w;
+    } else {
+      v[j] = x[i];
     }
-    __syncthreads();
-    const int32_t *const history = a.r.history + row * a.r.history_stride;
-    const int64_t n_prompt = a.r.n_prompt ? a.r.n_prompt[row] : 0;
+    if (mask) word[j / E] = mask[i >> 5];
+  }
+  // f(token) of a list's tokens, several of a thread loaded at once; whether one is
+  // none of the vocabulary
+  auto each = [&](const int32_t *list, int64_t length, auto &&f) {
     bool bad = false;
-    for (int64_t i = tid; i < n_history; i += kThreads) {
-      const int token = history[i], at = token - first;
-      bad |= static_cast<unsigned>(token) >= static_cast<unsigned>(a.n_vocab);
-      if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
+    for (int64_t i0 = tid; i0 < length; i0 += kAhead * kThreads) {
+      int token[kAhead];
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) token[z] = i0 + z * kThreads < length ? list[i0 + z * kThreads] : first;
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        if (i0 + z * kThreads >= length) break;
+        bad |= static_cast<unsigned>(token[z]) >= static_cast<unsigned>(a.n_vocab);
+        const unsigned at = static_cast<unsigned>(token[z] - first);
+        if (at < static_cast<unsigned>(n)) f(at, i0 + z * kThreads);
+      }
+    }
+    if (bad && first == 0) ikv::raise_status(a.status, IKV_STATUS_TOKEN);
+  };
+  if (n_history > 0) {
+    for (int i = 4 * tid; i < kSlice; i += 4 * kThreads) *reinterpret_cast<uint4 *>(s_seen + i) = uint4{};
+    __syncthreads();
+    const int64_t n_prompt = a.r.n_prompt ? a.r.n_prompt[row] : 0;
+    each(a.r.history + row * a.r.history_stride, n_history, [&](unsigned at, int64_t i) {
       if (i < n_prompt)
         atomicOr(&s_seen[at], 0x80000000u);
       else
         atomicAdd(&s_seen[at], 1u);
-    }
-    const int32_t *const named = a.r.bias_tokens + row * a.r.bias_stride;
-    for (int64_t i = tid; i < n_bias; i += kThreads) {
-      const int token = named[i], at = token - first;
-      bad |= static_cast<unsigned>(token) >= static_cast<unsigned>(a.n_vocab);
-      if (static_cast<unsigned>(at) < static_cast<unsigned>(n)) atomicMax(&s_bias[at], static_cast<int>(i + 1));
-    }
-    if (bad && first == 0) ikv::raise_status(a.status, IKV_STATUS_TOKEN);
-    __syncthreads();
+    });
   }
-  const bool ruled = n_history > 0 || n_bias > 0;
-  const float repetition = a.r.repetition ? a.r.repetition[row] : 1.0f;
-  const float presence = a.r.presence ? a.r.presence[row] : 0.0f;
-  const float frequency = a.r.frequency ? a.r.frequency[row] : 0.0f;
-  const float *const x = a.logits + row * a.n_vocab + first;
-  float *const y = a.out + row * a.n_vocab + first;
-  auto adjusted = [&](float v, unsigned seen, int bias) {
-    if (seen) {
-      const unsigned count = seen & 0x7fffffffu;
-      v = v > 0.0f ? v / repetition : v * repetition;
-      if (count) v = v - frequency * static_cast<float>(count) - presence;
-    }
-    if (bias) v += a.r.bias_values[row * a.r.bias_stride + bias - 1];
-    return v;
-  };
-  auto allowed = [&](unsigned word, int i) { return (word >> (i & 31) & 1u) != 0; };
-  if constexpr (VEC) {
-    for (int i = 4 * tid; i < n; i += 4 * kThreads) {
-      float4 v = *reinterpret_cast<const float4 *>(x + i);
-      if (ruled) {
-        const uint4 seen = *reinterpret_cast<const uint4 *>(s_seen + i);
-        const int4 bias = *reinterpret_cast<const int4 *>(s_bias + i);
-        v.x = adjusted(v.x, seen.x, bias.x);
-        v.y = adjusted(v.y, seen.y, bias.y);
-        v.z = adjusted(v.z, seen.z, bias.z);
-        v.w = adjusted(v.w, seen.w, bias.w);
+  if (n_bias > 0) {
+    for (int i = 4 * tid; i < kSlice; i += 4 * kThreads) *reinterpret_cast<int4 *>(s_bias + i) = int4{};
+    __syncthreads();
+    each(a.r.bias_tokens + row * a.r.bias_stride, n_bias,
+         [&](unsigned at, int64_t i) { atomicMax(&s_bias[at], static_cast<int>(i + 1)); });
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; j += E) {
+    const int i = place(j);
+    if (i >= n) continue;
+    if (n_history > 0) {
+      unsigned seen[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) seen[e] = s_seen[i + e];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (seen[e] == 0) continue;
+        float z = v[j + e];
+        z = z > 0.0f ? z / repetition : z * repetition;
+        const unsigned count = seen[e] & 0x7fffffffu;
+        if (count) z = z - frequency * static_cast<float>(count) - presence;
+        v[j + e] = z;
       }
-      const unsigned word = none ? 0u : mask ? mask[(first + i) >> 5] : ~0u;
-      v.x = allowed(word, i) ? v.x : -INFINITY;
-      v.y = allowed(word, i + 1) ? v.y : -INFINITY;
-      v.z = allowed(word, i + 2) ? v.z : -INFINITY;
-      v.w = allowed(word, i + 3) ? v.w : -INFINITY;
-      *reinterpret_cast<float4 *>(y + i) = v;
     }
-  } else {
-    for (int i = tid; i < n; i += kThreads) {
-      float v = x[i];
-      if (ruled) v = adjusted(v, s_seen[i], s_bias[i]);
-      const unsigned word = none ? 0u : mask ? mask[(first + i) >> 5] : ~0u;
-      y[i] = allowed(word, i) ? v : -INFINITY;
+    if (n_bias > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int from = s_bias[i + e];
+        if (from) v[j + e] += a.r.bias_values[row * a.r.bias_stride + from - 1];
+      }
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if ((word[j / E] >> ((i + e) & 31) & 1u) == 0) v[j + e] = -INFINITY;
+    if constexpr (VEC)
+      *reinterpret_cast<float4 *>(y + i) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    else
+      y[i] = v[j];
   }
 }
 
