@@ -101,11 +101,22 @@ __device__ __forceinline__ float4 values_q8(unsigned w) {
 
 __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// The largest over the 16, 32 or 64 lanes that hold a row.
+// The largest over the 16, 32 or 64 lanes that hold a row (DPP and lane swaps).
 template <int LANES>
 __device__ __forceinline__ unsigned lanes_max(unsigned x) {
-#pragma unroll
-  for (int o = 1; o < LANES; o *= 2) x = max(x, static_cast<unsigned>(__shfl_xor(static_cast<int>(x), o, 64)));
+  auto with = [&](int other) { x = max(x, static_cast<unsigned>(other)); };
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kDppXor1, 0xF, 0xF, false));
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kDppXor2, 0xF, 0xF, false));
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kDppHalfMirror, 0xF, 0xF, false));
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kDppMirror, 0xF, 0xF, false));
+  if constexpr (LANES >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+  }
+  if constexpr (LANES >= 64) {
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max(b[0], b[1]);
+  }
   return x;
 }
 
