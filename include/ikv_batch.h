@@ -237,9 +237,11 @@ int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_k
  *   workspace  as for ikv_attn_decode_batch_f32 (zero-filled once), of
  *              ikv_attn_decode_shared_workspace_bytes() bytes for at least these
  *              n_seq and n_groups.
- * Heads of over 128 dims, or of a number of dims that 8 does not divide, and
- * operands that are not 16-byte aligned have their shared blocks read once for each
- * sequence. n_groups 0: nothing is shared.
+ * Heads of over 128 dims, or of a number of dims that 8 does not divide, operands
+ * that are not 16-byte aligned, and calls whose tables hold so few keys (96 MB, all
+ * sequences' together) that a launch for the shared ones takes longer than reading
+ * them have their shared blocks read once for each sequence, from its own table.
+ * n_groups 0: nothing is shared.
  * ------------------------------------------------------------------- */
 size_t ikv_attn_decode_shared_workspace_bytes(int64_t n_seq, int64_t n_groups, int n_head,
                                               int n_head_kv, int head_dim);

@@ -88,8 +88,8 @@ __device__ __forceinline__ Keys keys_of(const ikv::BatchPages &b, const Groups &
   return s;
 }
 
-// Heads that the matrix kernel does not take: the keys of each sequence, for a decode
-// that reads all of them.
+// What the matrix kernel does not take, or is not worth its launch: the keys of each
+// sequence, for a decode that reads all of them.
 __global__ __launch_bounds__(kThreads) void shared_lengths_kernel(ikv::BatchPages b, Groups groups,
                                                                   const int32_t *n_kv, int32_t *keys) {
   const int seq = blockIdx.x * kThreads + threadIdx.x;
@@ -443,6 +443,16 @@ bool on_matrices(int head_dim, std::initializer_list<const void *> operands) {
   return true;
 }
 
+// Whether all sequences' keys, as many as their tables hold, are so few that reading
+// them for each sequence takes less than the launch for the shared ones, whose start
+// and joins are some 15 us: 16 heads of 128 over 8, 6 sequences behind 1024 tokens (53
+// MB of keys and values) 21.3 us and with the launch 25.2, 48 behind 128 15.5 and 30.6;
+// 6 behind 2048 (104 MB) 29.5 and 25.5, 2 behind 8192 36 and 32.
+constexpr int64_t kFewBytes = 96 << 20;
+bool few_keys(const ikv::BatchPages &b, int n_head_kv, int head_dim) {
+  return static_cast<int64_t>(b.n_seq) * b.capacity <= kFewBytes / (8 * n_head_kv * head_dim);
+}
+
 int dims_of(int head_dim) { return (head_dim + 31) / 32 * 32; }
 
 // Row blocks of a workgroup, for the mean rows of a group.
@@ -506,7 +516,8 @@ extern "C" int ikv_attn_decode_shared_f32(const float *q, float *k_pool, float *
   const Space at(n_seq, n_groups, n_head, n_head_kv, head_dim);
   char *const space = static_cast<char *>(workspace);
   a.groups = {group_start, shared_blocks, static_cast<int>(n_groups)};
-  if (n_groups == 0 || !on_matrices(head_dim, {q, k_pool, v_pool, k_new, v_new, out})) {
+  if (n_groups == 0 || few_keys(a.b, n_head_kv, head_dim) ||
+      !on_matrices(head_dim, {q, k_pool, v_pool, k_new, v_new, out})) {
     int32_t *const keys = reinterpret_cast<int32_t *>(space + at.seqs);
     shared_lengths_kernel<<<(a.b.n_seq + kThreads - 1) / kThreads, kThreads, 0, s>>>(a.b, a.groups, n_kv, keys);
     return ikv_attn_decode_batch_f32(q, k_pool, v_pool, batch, keys, k_new, v_new, out, n_head, n_head_kv, head_dim,

@@ -49,9 +49,15 @@ def _tables(sizes, shared, own, bt, seed):
     return start, tables, total, n_kv
 
 
-def _setup(dev, case, heads, kv, dim, bt, seed, new=True):
+def _setup(dev, case, heads, kv, dim, bt, seed, new=True, wide=True):
+    """wide: tables of as many columns as a server's largest contexts would need, which
+    has the shared blocks attended to by a launch of their own."""
     sizes, shared, own = CASES[case] if isinstance(case, str) else case
     start, tables, blocks, n_kv = _tables(sizes, shared, own, bt, seed)
+    if wide:
+        columns = 1 + (100 << 20) // (8 * kv * dim * bt * len(n_kv))
+        more = np.full((len(n_kv), max(0, columns - tables.shape[1])), -1, np.int32)
+        tables = np.ascontiguousarray(np.concatenate([tables, more], 1))
     g = torch.Generator(device=dev)
     g.manual_seed(seed)
     rnd = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
@@ -89,12 +95,12 @@ def _check(out, q, own, scale=None, rel=NORMAL_REL):
                     attention_bound(q[s], k, v, scale), rel)
 
 
-@pytest.mark.parametrize("new", [True, False], ids=["append", "read"])
+@pytest.mark.parametrize("form", ["append", "read", "narrow"])
 @pytest.mark.parametrize("heads,kv,dim", HEADS)
 @pytest.mark.parametrize("case", CASES)
-def test_against_64_bits(dev, case, heads, kv, dim, new):
-    bt = 64 if dim != 96 else 192
-    args, tables, n_kv = _setup(dev, case, heads, kv, dim, bt, seed=dim + len(case), new=new)
+def test_against_64_bits(dev, case, heads, kv, dim, form):
+    bt, new = 64 if dim != 96 else 192, form != "read"
+    args, tables, n_kv = _setup(dev, case, heads, kv, dim, bt, seed=dim + len(case), new=new, wide=form != "narrow")
     before = [args[x].clone() for x in ("k_pool", "v_pool")]
     own = _own(args, tables, n_kv)
     status = torch.zeros(1, dtype=torch.int32, device=dev)
