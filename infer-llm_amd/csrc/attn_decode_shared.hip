@@ -92,6 +92,7 @@ __device__ __forceinline__ Keys keys_of(const ikv::BatchPages &b, const Groups &
 // sequence, for a decode that reads all of them.
 __global__ __launch_bounds__(kThreads) void shared_lengths_kernel(ikv::BatchPages b, Groups groups,
                                                                   const int32_t *n_kv, int32_t *keys) {
+  ikv::check_row_start(groups.start, groups.n, b.n_seq, b.status);
   const int seq = blockIdx.x * kThreads + threadIdx.x;
   if (seq >= b.n_seq) return;
   const Keys s = keys_of(b, groups, n_kv, seq, 1);
@@ -242,6 +243,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
   const int r32 = lane & 31, c2 = lane >> 5;
   const int stride = a.n_head_kv * a.dim;
 
+  ikv::check_row_start(a.groups.start, a.groups.n, a.b.n_seq, a.b.status);
   Plan<R> plan(a);
   // (by whole waves, from the last workgroups on: in a small call they have no run)
   for (int s0 = (gridDim.x - 1 - blockIdx.x) * kThreads + 64 * wave; s0 < a.b.n_seq; s0 += gridDim.x * kThreads) {
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
     }
     __syncthreads();
     const int slot = item0 + p.item + run;
-    if (row_ok && slot < a.slots) {  // (all of them, unless the groups overlap)
+    if (row_ok && static_cast<unsigned>(slot) < static_cast<unsigned>(a.slots)) {  // (all of them, unless the groups overlap)
       const size_t at = static_cast<size_t>(slot) * R + 32 * rb + r32;
       float f[KG], top = -INFINITY, all = 0.f;
 #pragma unroll

@@ -50,7 +50,8 @@ struct SharedRow {
       w1 = static_cast<int>(static_cast<unsigned>(end) / static_cast<unsigned>(s.chunk));
     }
     slot = s.item + item + w0;
-    n = max(0, min(w1 - w0 + 1, p.slots - slot));  // (all of them, unless the groups overlap)
+    // (all of them, unless the groups overlap)
+    n = static_cast<unsigned>(slot) < static_cast<unsigned>(p.slots) ? min(w1 - w0 + 1, p.slots - slot) : 0;
   }
 };
 

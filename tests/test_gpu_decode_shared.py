@@ -171,6 +171,42 @@ def test_groups_out_of_range_share_nothing(dev):
         assert status.item() == 1
 
 
+@pytest.mark.parametrize("wide", [True, False], ids=["wide", "narrow"])
+def test_groups_that_overlap_stay_in_bounds(dev, wide):
+    """Far more items than the workspace has slots for; flagged, nothing faults, and
+    the workspace serves the next call."""
+    args, tables, n_kv = _setup(dev, ([6], [2], [7, 9, 3, 1, 20, 64]), 16, 8, 128, 64, seed=12, new=False, wide=wide)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    work = ikv.decode_shared_workspace(6, 501, 16, 8, 128)
+    want = ikv.attn_decode_shared(**args)
+    ikv.attn_decode_shared(**{**args, "group_start": dev32([0, 6] * 251, dev),
+                              "shared_blocks": dev32([2] * 501, dev)}, status=status, workspace=work)
+    assert status.item() == 1
+    assert torch.equal(want, ikv.attn_decode_shared(**args, workspace=work))
+
+
+def test_two_captured_calls_share_a_workspace(dev):
+    work = ikv.decode_shared_workspace(9, 4, 32, 8, 128)
+    calls, graphs = [], []
+    for case, seed in (("long", 40), ("groups", 41)):
+        args, *_ = _setup(dev, case, 32, 8, 128, 64, seed=seed, new=False)
+        calls.append((args, torch.zeros_like(args["q"]), ikv.attn_decode_shared(**args)))
+    torch.cuda.synchronize()
+    for args, out, _ in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ikv.attn_decode_shared(**args, out=out, workspace=work)
+    for order in ((0, 1), (1, 1, 0), (0, 0, 1)):
+        for _, out, _ in calls:
+            out.fill_(-7.0)
+        for i in order:
+            graphs[i].replay()
+        ikv.attn_decode_shared(**calls[order[0]][0], workspace=work)
+        torch.cuda.synchronize()
+        for _, out, want in calls:
+            assert torch.equal(out, want)
+
+
 def test_a_bad_block_is_flagged(dev):
     args, tables, n_kv = _setup(dev, ([3], [3], [7, 9, 3]), 8, 4, 64, 64, seed=8, new=False)
     args["k_pool"].nan_to_num_(0.0), args["v_pool"].nan_to_num_(0.0)
