@@ -17,7 +17,17 @@
 //   * The key's K scale multiplies its scores, its V scale its weights.
 //   * A lane reads its K codes 16 bytes at a time and its V codes, 8 keys by 4 W
 //     dims, a key at a time; V's transpose is the choice of registers when two
-//     converted codes are packed.
+//     converted codes are packed. The registers of half a unit's codes are loaded
+//     again, with the next unit's, as soon as the half is in the products (48 long
+//     contexts 122 -> 113 us).
+// Measured (MI355X, us): 48 contexts of up to 16384 tokens, 32 heads of 128 over 8, 556
+// MB: 113, 4.9 TB/s; the same cache in F32, 2.1 GB, 371. 37 of up to 5003, 12 heads of
+// 64 over 4, 33 MB: 19, most of it the start (lengths, tables, first codes), two units
+// one behind the other in a wave and the join; 3 of up to 150 and an idle slot 10.
+// Neither pipe bounds the long ones: matrix instructions are issued in 17 % of the
+// cycles, vector ones in 34 %, and without the conversions they take 111, with one
+// piece of three 110. 23 % of the waves' time is waits for memory, 46 % for a place to
+// issue, and the last workgroup is done 10 % after the mean.
 #include "cache_q8.hpp"
 #include "bf16x3.hpp"
 #include "decode_runs.hpp"
@@ -31,6 +41,11 @@ using namespace ikv::pieces;
 constexpr int kWaves = 4;  // of a workgroup
 constexpr int KT = 64;     // keys of a unit
 constexpr int kRunUnits = 64, kWhole = 8;  // (decode_runs.hpp)
+// Fewest units of a run of long contexts: the workgroup that joins a context's parts
+// reads all of them, and they grow with the query heads. 16 heads of 80 over 1: 2
+// contexts of 16000 tokens 131 us in runs of one unit, 34 of eight, 15 of up to 13800 53
+// and 36; but 16 heads of 128 over 8, 16 contexts of up to 1500, 20.7 and 24.
+constexpr int least_of(int gq) { return gq / 2; }
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int groups_of(int w) { return w > 2 ? 256 : 512; }
 
@@ -97,7 +112,7 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
   }
 
   constexpr int kGroups = groups_of(W);
-  ikv::Plan<Args, KT, kGroups, kRunUnits, kWhole> plan(a);
+  ikv::Plan<Args, KT, kGroups, kRunUnits, kWhole, least_of(GQ)> plan(a);
   const ikv::Parts<GQ, DP> parts(a.part);
   // this lane's bytes of a unit's rows: of K row 32 (T / 2) + 8 (col / 4) + 4 (T % 2)
   // + col % 4 of tile T (so that the two tiles of a product with V leave lane quarter

@@ -36,8 +36,9 @@ struct Place {
 };
 
 // UNITS: of a run where there are more runs than workgroups; WHOLE: units of a
-// (sequence, head) that are not split anywhere.
-template <class Args, int KT, int GROUPS, int UNITS, int WHOLE>
+// (sequence, head) that are not split anywhere; LEAST: of a run, where a (sequence,
+// head) has as many on average.
+template <class Args, int KT, int GROUPS, int UNITS, int WHOLE, int LEAST = 1>
 struct Plan {
   using Units = unsigned long long;
   Units total, chunk;  // all units, those of a run
@@ -65,6 +66,8 @@ struct Plan {
     runs = static_cast<int>(min(max(total / UNITS, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
     chunk = (total + runs - 1) / runs;
     if (chunk == 0) chunk = 1;
+    if constexpr (LEAST > 1)
+      chunk = max(chunk, min(static_cast<Units>(LEAST), total / (static_cast<Units>(a.b.n_seq) * items)));
     whole = chunk > 1 ? static_cast<int>(min(chunk, static_cast<Units>(4))) + 3 : WHOLE;
   }
 

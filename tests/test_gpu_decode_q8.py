@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 # more; 64, 128 and 256 dims held, whole and in part)
 HEADS = [(16, 8, 128), (32, 8, 128), (12, 4, 64), (16, 1, 80), (8, 8, 96), (6, 2, 16), (16, 2, 128),
          (20, 1, 64), (7, 7, 256), (40, 2, 144), (34, 2, 48)]
-CONTEXTS = [[1], [2, 0, 64, 65, 1, 63], [300, 1, 0, 700, 128], [5] * 150, [0, 0], [2500, 3]]
+CONTEXTS = [[1], [2, 0, 64, 65, 1, 63], [300, 1, 0, 700, 128], [5] * 150, [0, 0], [2500, 3], [9000]]
 
 
 def _setup(dev, n_kv, bt, heads, kv, dim, dtype, seed):
