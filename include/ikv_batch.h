@@ -170,7 +170,8 @@ int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,
  *     codes  [b][n_head_kv][block_tokens][head_dim] bytes
  *     scales [b][n_head_kv][block_tokens] floats
  * in each of the K and V arrays, head by head, so that a head's rows of a block
- * are contiguous. codes and scales 16-byte aligned (else -EINVAL); head_dim a
+ * are contiguous. Scales below 2^-100 and values next to the largest float are held
+ * and read back, but lose bits or leave the range in sums of many of them. codes and scales 16-byte aligned (else -EINVAL); head_dim a
  * multiple of 16 up to 256 (else -ENOTSUP); -EOVERFLOW: n_head_kv * head_dim past
  * 2^23.
  * ------------------------------------------------------------------- */

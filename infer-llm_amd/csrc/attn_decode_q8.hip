@@ -21,13 +21,14 @@
 //     again, with the next unit's, as soon as the half is in the products (48 long
 //     contexts 122 -> 113 us).
 // Measured (MI355X, us): 48 contexts of up to 16384 tokens, 32 heads of 128 over 8, 556
-// MB: 113, 4.9 TB/s; the same cache in F32, 2.1 GB, 371. 37 of up to 5003, 12 heads of
+// MB: 108, 5.1 TB/s; as many in F32, 2.4 GB, 371. 37 of up to 5003, 12 heads of
 // 64 over 4, 33 MB: 19, most of it the start (lengths, tables, first codes), two units
 // one behind the other in a wave and the join; 3 of up to 150 and an idle slot 10.
 // Neither pipe bounds the long ones: matrix instructions are issued in 17 % of the
-// cycles, vector ones in 34 %, and without the conversions they take 111, with one
+// cycles, vector ones in 34 %; without the conversions they took 111 of 114, with one
 // piece of three 110. 23 % of the waves' time is waits for memory, 46 % for a place to
-// issue, and the last workgroup is done 10 % after the mean.
+// issue. Workgroups are done between 55 and 115, but shorter runs, or a long one and
+// then short ones as workgroups come free, took 120 and 116: the memory is shared.
 #include "cache_q8.hpp"
 #include "bf16x3.hpp"
 #include "decode_runs.hpp"
@@ -46,6 +47,9 @@ constexpr int kRunUnits = 64, kWhole = 8;  // (decode_runs.hpp)
 // contexts of 16000 tokens 131 us in runs of one unit, 34 of eight, 15 of up to 13800 53
 // and 36; but 16 heads of 128 over 8, 16 contexts of up to 1500, 20.7 and 24.
 constexpr int least_of(int gq) { return gq / 2; }
+// Cache policy of the values' loads: non-temporal, as each line is read once (48 long
+// contexts 115 -> 108.5 us; 110 with the keys' too, of which two loads read a line).
+constexpr int kOnce = 2;
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int groups_of(int w) { return w > 2 ? 256 : 512; }
 
@@ -217,12 +221,12 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
       for (int i = 0; i < 8; ++i) {
         const int at = (32 * h + i) * dim;
         if constexpr (W == 1) {
-          vr[h][i][0] = __builtin_amdgcn_raw_buffer_load_b32(r.v, v_off, at, 0);
+          vr[h][i][0] = __builtin_amdgcn_raw_buffer_load_b32(r.v, v_off, at, kOnce);
         } else if constexpr (W == 2) {
-          const auto x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r.v, v_off, at, 0));
+          const auto x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r.v, v_off, at, kOnce));
           vr[h][i][0] = x.x, vr[h][i][1] = x.y;
         } else {
-          const auto x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r.v, v_off, at, 0));
+          const auto x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r.v, v_off, at, kOnce));
           vr[h][i][0] = x.x, vr[h][i][1] = x.y, vr[h][i][2] = x.z, vr[h][i][3] = x.w;
         }
       }

@@ -118,6 +118,24 @@ def test_rows_that_are_not_finite_stay_in_their_sequence_and_head(dev):
     assert torch.equal(out[2], good[2])
 
 
+def test_codes_past_32_bits(dev):
+    kv, dim, bt, blocks = 8, 256, 256, 9000  # 4.7 GB of codes each
+    cache = ikv.cache_q8(blocks, bt, kv, dim, torch.int8, device=dev)
+    tables = torch.tensor([[blocks - 1, 0], [8500, blocks - 2]], dtype=torch.int32)
+    g = torch.Generator(device=dev)
+    g.manual_seed(1)
+    rows, n_kv = [torch.randn(600, kv, dim, generator=g, device=dev) for _ in range(2)], [200, 400]
+    t = tables.to(dev)
+    ikv.append_packed_q8(cache, *rows, t, dev32([0, 200, 600], dev))
+    q = torch.randn(2, 16, dim, generator=g, device=dev)
+    new = [torch.randn(2, kv, dim, generator=g, device=dev) for _ in range(2)]
+    out = ikv.attn_decode_batch_q8(q, cache, t, dev32([201, 401], dev), k_new=new[0], v_new=new[1])
+    for s, (first, n) in enumerate(zip((0, 200), n_kv)):
+        k, v = (values(*quantised(torch.cat([x[first:first + n], y[s:s + 1]]), torch.int8)) for x, y in zip(rows, new))
+        assert_near(out[s:s + 1], attention64(q[s:s + 1], k, v, n), decode_bound(q[s], k, v))
+    assert (cache[0][0] == 0).all() and (cache[0][300] == 0).all()
+
+
 def test_scale_and_out(dev):
     q, cache, tables, _ = _setup(dev, [90, 33], 64, 4, 2, 64, torch.int8, seed=8)
     out = torch.empty_like(q)
