@@ -21,7 +21,7 @@
 //     again, with the next unit's, as soon as the half is in the products (48 long
 //     contexts 122 -> 113 us).
 // Measured (MI355X, us): 48 contexts of up to 16384 tokens, 32 heads of 128 over 8, 556
-// MB: 108, 5.1 TB/s; as many in F32, 2.4 GB, 371. 37 of up to 5003, 12 heads of
+// MB: 106, 5.2 TB/s; as many in F32, 2.4 GB, 371. 37 of up to 5003, 12 heads of
 // 64 over 4, 33 MB: 19, most of it the start (lengths, tables, first codes), two units
 // one behind the other in a wave and the join; 3 of up to 150 and an idle slot 10.
 // Neither pipe bounds the long ones: matrix instructions are issued in 17 % of the
