@@ -228,8 +228,8 @@ int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_k
  *   group_start    [n_groups + 1] int32, ascending from 0 to n_seq: group g is the
  *                  sequences [group_start[g], group_start[g + 1])
  *   shared_blocks  [n_groups] int32: the leading entries that the tables of group
- *                  g's sequences have in common; they are read from the table of
- *                  the group's first sequence. 0: nothing is shared.
+ *                  g's sequences have in common (idle ones' tables, here too, are
+ *                  not read). 0: nothing is shared.
  * Every sequence has a key of its own: one of n_kv[s] <= shared_blocks[g] *
  * block_tokens that is not idle (0) raises IKV_STATUS_POSITION and is taken for 0,
  * as is one of no group within [0, n_seq]. A group of a negative shared_blocks, or of

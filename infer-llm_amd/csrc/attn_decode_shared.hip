@@ -95,6 +95,20 @@ __device__ __forceinline__ Keys keys_of(const ikv::BatchPages &b, const Groups &
   return s;
 }
 
+// The first of a group's sequences that has keys of its own, counted from its first
+// one (-1: none), by a whole wave, where lane l has n_kv of sequence l of the group
+// (of the last one, where there are fewer).
+__device__ __forceinline__ int first_live(const ikv::BatchPages &b, const Group &g, const int32_t *n_kv, int n) {
+  const int lane = threadIdx.x & 63, shared = g.blocks * b.bt;
+  for (int s = 0;;) {
+    const unsigned long long some = __builtin_amdgcn_ballot_w64(n > shared && n <= b.capacity);
+    if (some) return s + __builtin_ctzll(some);
+    s += 64;
+    if (s >= g.seqs) return -1;
+    n = n_kv[g.first + min(s + lane, g.seqs - 1)];
+  }
+}
+
 // What the matrix kernel does not take, or is not worth its launch: the keys of each
 // sequence, for a decode that reads all of them.
 __global__ __launch_bounds__(kThreads) void shared_lengths_kernel(ikv::BatchPages b, Groups groups,
@@ -289,17 +303,32 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
 
     const int t0 = p.tile + kg;
     {
-      const int32_t *const table = a.b.tables + p.g.first * a.b.stride;
+      // The blocks are those of the group's first sequence that has keys: an idle slot's
+      // entries may be anything. The first slot's are loaded together with the lengths,
+      // as it seldom is an idle one.
+      const int32_t *table = a.b.tables + p.g.first * a.b.stride;
       int blk = t0 * BN / a.b.bt, in_blk = t0 * BN % a.b.bt, ent0 = 0, ent = 0;
-      auto entries = [&]() {
+      auto load_entries = [&]() {
         ent0 = blk;
         ent = table[min(blk + lane, p.g.blocks - 1)];
+      };
+      auto check_entries = [&]() {
         if (static_cast<unsigned>(ent) >= static_cast<unsigned>(a.b.n_blocks)) {
           ikv::raise_status(a.b.status, IKV_STATUS_BLOCK);
           ent = 0;
         }
       };
-      entries();
+      load_entries();
+      const int live = first_live(a.b, p.g, a.n_kv, a.n_kv[p.g.first + min(lane, p.g.seqs - 1)]);
+      if (live < 0) {  // (nobody asks for the sums; by all waves alike)
+        u += last - p.tile;
+        continue;
+      }
+      if (live > 0) {
+        table += live * a.b.stride;
+        load_entries();
+      }
+      check_entries();
       constexpr int kMine = (KJ + KG - 1) / KG;  // of the rows' pieces: j = kg, kg + KG, ...
       floatx4 qr[kMine] = {};
       if (row_ok) {
@@ -317,7 +346,10 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_kernel(Args a) {
           in_blk -= a.b.bt;
           ++blk;
         }
-        if (blk - ent0 >= 64) entries();
+        if (blk - ent0 >= 64) {
+          load_entries();
+          check_entries();
+        }
         return r;
       };
       auto rsrc = [&](const float *base, long long r, int t) {  // (none of a tile behind the run)
