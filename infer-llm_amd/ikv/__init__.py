@@ -1243,8 +1243,11 @@ def adjust_logits(logits, *, history=None, n_history=None, n_prompt=None, repeti
         raise ValueError("bias_tokens and bias_values go together")
     if bias_tokens is not None and bias_tokens.shape != bias_values.shape:
         raise ValueError("bias_tokens and bias_values must be of one shape")
-    if masks is not None and (masks.dim() != 2 or masks.shape[1] != (n_vocab + 31) // 32):
-        raise ValueError("masks must be [n_masks, (n_vocab + 31) // 32]")
+    if masks is None:
+        if mask_of is not None:
+            raise ValueError("mask_of goes with masks")
+    elif masks.dim() != 2 or masks.shape[0] == 0 or masks.shape[1] != (n_vocab + 31) // 32:
+        raise ValueError("masks must be [n_masks, (n_vocab + 31) // 32], one at least")
     if out is not None and out.shape != logits.shape:
         raise ValueError("out must be of logits' shape")
     with _on(dev, stream):
