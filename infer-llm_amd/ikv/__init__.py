@@ -1253,9 +1253,12 @@ def adjust_logits(logits, *, history=None, n_history=None, n_prompt=None, repeti
     with _on(dev, stream):
         if out is None:
             out = torch.empty_like(logits)
-        rules = LogitRules(_ptr(history), 0 if history is None else history.shape[1], _ptr(n_history),
+        # (an empty list has no address, but its lengths are looked at)
+        at = [None if t is None else t.data_ptr() or logits.data_ptr()
+              for t in (history, bias_tokens, bias_values)]
+        rules = LogitRules(at[0], 0 if history is None else history.shape[1], _ptr(n_history),
                            _ptr(n_prompt), _ptr(repetition), _ptr(presence), _ptr(frequency),
-                           _ptr(bias_tokens), _ptr(bias_values),
+                           at[1], at[2],
                            0 if bias_tokens is None else bias_tokens.shape[1], _ptr(n_bias),
                            _ptr(masks), 0 if masks is None else masks.shape[0], _ptr(mask_of))
         _check("ikv_adjust_logits_f32",
