@@ -41,7 +41,12 @@ using namespace ikv::pieces;
 
 constexpr int kWaves = 4;  // of a workgroup
 constexpr int KT = 64;     // keys of a unit
-constexpr int kRunUnits = 64, kWhole = 8;  // (decode_runs.hpp)
+// One run a workgroup, however many units (decode_runs.hpp). 48 contexts of 32 heads of
+// 128 over 8, equal shares against runs of 64 units, taken as workgroups come free: 39000
+// units 118 and 130 us, 57000 162 and 179, 113000 304 and 320, 297000 770 and 785; heads
+// of 64, 33000 units 57 and 75; of 256, 21000 160 and 198. (As many whole rounds of equal
+// runs: 133, 183, 322, 782, 70 and 161.)
+constexpr int kRunUnits = 0, kWhole = 8;
 // Fewest units of a run of long contexts: the workgroup that joins a context's parts
 // reads all of them, and they grow with the query heads. 16 heads of 80 over 1: 2
 // contexts of 16000 tokens 131 us in runs of one unit, 34 of eight, 15 of up to 13800 53
@@ -130,19 +135,12 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
   }
   const unsigned v_off = DB * col < dim ? static_cast<unsigned>(8 * quad * dim + DB * col) : kOut;
 
-  int run = blockIdx.x;
-  unsigned long long u = plan.chunk * run, end = min(plan.total, u + plan.chunk);
+  const int run = blockIdx.x;
+  unsigned long long u = plan.chunk * run;
+  const unsigned long long end = min(plan.total, u + plan.chunk);
   ikv::Place p{};
   if (u < end) p = plan.at(a, u);
-  for (;;) {
-    if (u >= end) {
-      run = ikv::next_run<kGroups>(plan, parts, s_meet);
-      if (run >= plan.runs) return;
-      u = plan.chunk * run;
-      end = min(plan.total, u + plan.chunk);
-      if (u < end) p = plan.at(a, u);
-      continue;
-    }
+  while (u < end) {
     if (plan.kept(p.tiles) && p.tile > 0) {  // (with the run that holds its first unit)
       u += p.tiles - p.tile;
       plan.next(a, p);

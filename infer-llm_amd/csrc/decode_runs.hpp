@@ -35,7 +35,7 @@ struct Place {
   int seq, keys, tiles, item, tile;
 };
 
-// UNITS: of a run where there are more runs than workgroups; WHOLE: units of a
+// UNITS: of a run where there are more runs than workgroups (0: there never are); WHOLE: units of a
 // (sequence, head) that are not split anywhere; LEAST: of a run, where a (sequence,
 // head) has as many on average.
 template <class Args, int KT, int GROUPS, int UNITS, int WHOLE, int LEAST = 1>
@@ -63,7 +63,8 @@ struct Plan {
       look(a, s, total);
       total = lane_value(upto, 63);
     }
-    runs = static_cast<int>(min(max(total / UNITS, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
+    runs = GROUPS;
+    if constexpr (UNITS > 0) runs = static_cast<int>(min(max(total / UNITS, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
     chunk = (total + runs - 1) / runs;
     if (chunk == 0) chunk = 1;
     if constexpr (LEAST > 1)
