@@ -65,10 +65,11 @@ struct Quant {
     some = top_bits - 1u < 0x7f7fffffu;
     scale = some ? static_cast<float>(top * (1.0 / (E4M3 ? 448.0 : 127.0))) : top_bits == 0 ? 0.0f : NAN;
   }
-  // the quotient, its last bit by what the first one leaves (so exact ones are exact)
+  // the quotient, its last bit by what the first one leaves (so exact ones are exact; the
+  // signs are so that -0 stays -0)
   __device__ __forceinline__ double of(float v) const {
     const double a = static_cast<double>(v) * (E4M3 ? 448.0 : 127.0), q = a * inv;
-    return fma(fma(-q, top, a), inv, q);
+    return fma(-fma(q, top, -a), inv, q);
   }
   // four codes, the first in the low byte
   __device__ __forceinline__ unsigned codes(const float4 x) const {
