@@ -170,10 +170,8 @@ int ikv_attn_decode_batch_f32(const float *q, float *k_pool, float *v_pool,
  *     codes  [b][n_head_kv][block_tokens][head_dim] bytes
  *     scales [b][n_head_kv][block_tokens] floats
  * in each of the K and V arrays, head by head, so that a head's rows of a block
- * are contiguous. Scales below 2^-100 and values next to the largest float are held
- * and read back, but lose bits or leave the range in sums of many of them. codes and scales 16-byte aligned (else -EINVAL); head_dim a
- * multiple of 16 up to 256 (else -ENOTSUP); -EOVERFLOW: n_head_kv * head_dim past
- * 2^23.
+ * are contiguous. codes and scales 16-byte aligned (else -EINVAL); head_dim a multiple
+ * of 16 up to 256 (else -ENOTSUP); -EOVERFLOW: n_head_kv * head_dim past 2^23.
  * ------------------------------------------------------------------- */
 #define IKV_Q8_INT8 0
 #define IKV_Q8_E4M3 1
@@ -213,7 +211,11 @@ int ikv_read_packed_q8(const ikv_kv_q8 *cache, float *k_rows, float *v_rows,
  * sequence s is quantised, written and attended to as it is held: the result is
  * that of ikv_append_packed_q8 and a call without them. q, k_new, v_new and out
  * 16-byte aligned (else -EINVAL). The workspace is used as there (zero-filled
- * once; one of this form serves only this form). */
+ * once; one of this form serves only this form).
+ * Queries, and weights times V's scales, are multiplied as three bf16 pieces: V scales
+ * below 2^-100 lose bits that F32 would keep, and with scales above 2^80 sums may leave
+ * F32's range, as scores do whose query and key are too large for it. (All of them are
+ * held and read back as they are.) */
 size_t ikv_attn_decode_batch_q8_workspace_bytes(int n_head, int n_head_kv, int head_dim);
 
 int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_kv_batch *batch,
@@ -228,21 +230,22 @@ int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_k
  *   group_start    [n_groups + 1] int32, ascending from 0 to n_seq: group g is the
  *                  sequences [group_start[g], group_start[g + 1])
  *   shared_blocks  [n_groups] int32: the leading entries that the tables of group
- *                  g's sequences have in common (idle ones' tables, here too, are
- *                  not read). 0: nothing is shared.
+ *                  g's sequences have in common (an idle slot's table is not
+ *                  read). 0: nothing is shared.
  * Every sequence has a key of its own: one of n_kv[s] <= shared_blocks[g] *
  * block_tokens that is not idle (0) raises IKV_STATUS_POSITION and is taken for 0,
  * as is one of no group within [0, n_seq]. A group of a negative shared_blocks, or of
- * more than the table's width, raises it, too, and shares nothing. Rows that k_new and v_new bring must not lie in blocks that any other
- * sequence reads.
+ * more than the table's width, raises it, too, and shares nothing. Rows that k_new and
+ * v_new bring must not lie in blocks that any other sequence reads.
  *   workspace  as for ikv_attn_decode_batch_f32 (zero-filled once), of
  *              ikv_attn_decode_shared_workspace_bytes() bytes for at least these
  *              n_seq and n_groups.
  * Heads of over 128 dims, or of a number of dims that 8 does not divide, operands
  * that are not 16-byte aligned, and calls whose tables hold so few keys (96 MB, all
  * sequences' together) that a launch for the shared ones takes longer than reading
- * them have their shared blocks read once for each sequence, from its own table.
- * n_groups 0: nothing is shared.
+ * them have their shared blocks read once for each sequence, from its own table. That
+ * goes by table_stride, so tables of another width may give results that differ by
+ * roundings. n_groups 0: nothing is shared.
  * ------------------------------------------------------------------- */
 size_t ikv_attn_decode_shared_workspace_bytes(int64_t n_seq, int64_t n_groups, int n_head,
                                               int n_head_kv, int head_dim);

@@ -20,15 +20,14 @@
 //     converted codes are packed. The registers of half a unit's codes are loaded
 //     again, with the next unit's, as soon as the half is in the products (48 long
 //     contexts 122 -> 113 us).
-// Measured (MI355X, us): 48 contexts of up to 16384 tokens, 32 heads of 128 over 8, 556
-// MB: 106, 5.2 TB/s; as many in F32, 2.4 GB, 371. 37 of up to 5003, 12 heads of
-// 64 over 4, 33 MB: 19, most of it the start (lengths, tables, first codes), two units
-// one behind the other in a wave and the join; 3 of up to 150 and an idle slot 10.
-// Neither pipe bounds the long ones: matrix instructions are issued in 17 % of the
-// cycles, vector ones in 34 %; without the conversions they took 111 of 114, with one
-// piece of three 110. 23 % of the waves' time is waits for memory, 46 % for a place to
-// issue. Workgroups are done between 55 and 115, but shorter runs, or a long one and
-// then short ones as workgroups come free, took 120 and 116: the memory is shared.
+// Measured (MI355X, us): 48 contexts of up to 16384 tokens, 32 heads of 128 over 8, 554
+// MB: 105, 5.3 TB/s, with the append 4 more; of up to 110000, 5 GB: 763, 6.6 TB/s; as
+// much in e4m3. The first in F32, 2.4 GB: 371. 37 of up to 5003, 12 heads of 64 over 4,
+// 33 MB: 19, with the append 20.5, most of it the start (lengths, tables, first codes),
+// two units one behind the other in a wave and the join; three of up to 52 and an idle
+// slot 8 by the trace, one unit each. Neither pipe bounds the 554 MB: matrix
+// instructions are issued in 19 % of the cycles, vector ones in 36 %; 23 % of the waves'
+// time is waits for memory, 43 % for a place to issue.
 #include "cache_q8.hpp"
 #include "bf16x3.hpp"
 #include "decode_runs.hpp"
@@ -49,11 +48,12 @@ constexpr int KT = 64;     // keys of a unit
 constexpr int kRunUnits = 0, kWhole = 8;
 // Fewest units of a run of long contexts: the workgroup that joins a context's parts
 // reads all of them, and they grow with the query heads. 16 heads of 80 over 1: 2
-// contexts of 16000 tokens 131 us in runs of one unit, 34 of eight, 15 of up to 13800 53
-// and 36; but 16 heads of 128 over 8, 16 contexts of up to 1500, 20.7 and 24.
+// contexts of 16000 tokens 116 us in runs of one unit, 33 of eight, 15 of up to 13800 53
+// and 33; but 16 heads of 128 over 8, 16 contexts of up to 1500, 19.4 and 22.4.
 constexpr int least_of(int gq) { return gq / 2; }
 // Cache policy of the values' loads: non-temporal, as each line is read once (48 long
-// contexts 115 -> 108.5 us; 110 with the keys' too, of which two loads read a line).
+// contexts 115 -> 108.5 us; 110 with the keys' too, of which two loads read a line; both
+// before a workgroup had one run).
 constexpr int kOnce = 2;
 constexpr float kRescale = 8.0f;  // log2 headroom before the running maximum is moved
 constexpr int groups_of(int w) { return w > 2 ? 256 : 512; }

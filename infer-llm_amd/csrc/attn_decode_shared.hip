@@ -19,12 +19,14 @@
 //   * The (chunk, KV head) items' tiles are dealt to the workgroups in equal runs,
 //     from the groups as they stand on the device; what a run has of an item goes to
 //     the workspace.
-// Measured (MI355X, us), the shared part and the decode behind it: 48 sequences behind
-// 16384 tokens, 32 heads of 128 over 8, 127 + 40 (the shared part 12.9 GF, 101 TFLOP/s
-// of the 151 of a large F32 product; of a workgroup's 113 on average 10 are its start
-// and 8 % the softmax and waits, the clock falls to 2.2 GHz, and the last workgroup is
-// done 12 after the mean, one with parts of two items); 37 sequences in 3 groups of
-// 64-float heads 15 + 14: starts, joins and launches; unshared 46.9 and, the 48, 1002.
+// Measured (MI355X, us, traced), the shared part and the decode behind it: 48 sequences
+// behind 16384 tokens, 32 heads of 128 over 8, 130 + 39 (the shared part 12.9 GF, 99
+// TFLOP/s of the 151 of a large F32 product; with 127, of a workgroup's 113 on average 10
+// were its start and 8 % the softmax and waits, the clock fell to 2.2 GHz, and the last
+// workgroup was done 12 after the mean, one with parts of two items); 37 sequences in 3
+// groups of 64-float heads 16.5 + 14.4: starts, joins and launches; unshared 46.9 and,
+// the 48, 1002. The running sums of a row are a chain of additions over a wave's keys:
+// the errors of the 48 are 6.5e-7 (2-norm), unshared 2.6e-7.
 // Tried and not kept: two waves a SIMD (spilled; 140), two sums of S (the same).
 #include "decode_shared.hpp"
 #include "coherent.hpp"
@@ -486,9 +488,11 @@ bool on_matrices(int head_dim, std::initializer_list<const void *> operands) {
 
 // Whether all sequences' keys, as many as their tables hold, are so few that reading
 // them for each sequence takes less than the launch for the shared ones, whose start
-// and joins are some 15 us: 16 heads of 128 over 8, 6 sequences behind 1024 tokens (53
-// MB of keys and values) 21.3 us and with the launch 25.2, 48 behind 128 15.5 and 30.6;
-// 6 behind 2048 (104 MB) 29.5 and 25.5, 2 behind 8192 36 and 32.
+// and joins are some 15 us: 16 heads of 128 over 8, 6 sequences behind 1024 tokens (57
+// MB of keys and values) 20.8 us and with the launch 25.4, 48 behind 128 (96 MB) 15.2 and
+// 30.7; 6 behind 2048 (105 MB) 28.7 and 25.6, 2 behind 8192 (131 MB) 34.0 and 33.7. The
+// host sees the tables' width, not the lengths: short contexts in wide tables take the
+// launch.
 constexpr int64_t kFewBytes = 96 << 20;
 bool few_keys(const ikv::BatchPages &b, int n_head_kv, int head_dim) {
   return static_cast<int64_t>(b.n_seq) * b.capacity <= kFewBytes / (8 * n_head_kv * head_dim);

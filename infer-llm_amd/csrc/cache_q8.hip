@@ -7,10 +7,10 @@
 // over the row's heads, a row of a head on 16, 32 or 64 lanes, four elements a
 // lane, so that the largest magnitude is a maximum over those lanes and codes and
 // floats move in whole lines.
-// Measured (MI355X, us): 8190 rows of 8 heads of 128 written 21-22 (84 MB, 3.9 TB/s:
+// Measured (MI355X, us): 8190 rows of 8 heads of 128 written 22 (84 MB, 3.8 TB/s:
 // the quotients in 64 bits, which leave 20 where they are a product instead), read back
-// 16 (5.2 TB/s, the rate of a copy); 123000 rows read 199 (5.2 TB/s); 211 rows of 5
-// sequences written 5.6, 1300 read 6.0: a launch and four loads one after the other.
+// 16 (5.3 TB/s, the rate of a copy); 103356 rows read 199 (1.07 GB, 5.3 TB/s); 211 rows
+// of 5 sequences written 5.6, 1398 read 6.1: a launch and four loads one after the other.
 #include "cache_q8.hpp"
 
 #include <algorithm>

@@ -861,7 +861,7 @@ def attn_decode_shared(q, k_pool, v_pool, tables, block_tokens: int, group_start
                        workspace=None, stream=None):
     """attn_decode_batch where the sequences [group_start[g], group_start[g + 1]) of
     each group have the first shared_blocks[g] blocks of their tables in common:
-    these are read once for all of them."""
+    these are read once for all of them. The tables of idle slots are not read."""
     torch = _torch()
     dev = q.device
     _operands(dev, (q, k_pool, v_pool, k_new, v_new, out, workspace),
