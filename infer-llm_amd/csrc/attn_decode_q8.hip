@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kWaves * 64, W > 2 ? 1 : 2) void decode_q8_kernel(A
 
   constexpr int kGroups = groups_of(W);
   ikv::Plan<Args, KT, kGroups, kRunUnits, kWhole, least_of(GQ)> plan(a);
-  const ikv::Parts<GQ, DP> parts(a.part);
+  const ikv::Parts<GQ, DP, kGroups> parts(a.part);
   // this lane's bytes of a unit's rows: of K row 32 (T / 2) + 8 (col / 4) + 4 (T % 2)
   // + col % 4 of tile T (so that the two tiles of a product with V leave lane quarter
   // quad the scores of keys 8 quad .. + 7), of V rows 32 u + 8 quad + i
@@ -456,7 +456,8 @@ extern "C" size_t ikv_attn_decode_batch_q8_workspace_bytes(int n_head, int n_hea
   if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || head_dim <= 0 || head_dim % 16 != 0 ||
       head_dim > ikv::kMaxDimQ8)
     return 0;
-  return ikv::parts_bytes(heads_of(n_head / n_head_kv), 64 * wide_of(head_dim));
+  const int w = wide_of(head_dim);
+  return ikv::parts_bytes(heads_of(n_head / n_head_kv), 64 * w, groups_of(w));
 }
 
 extern "C" int ikv_attn_decode_batch_q8(const float *q, const ikv_kv_q8 *cache, const ikv_kv_batch *batch,

@@ -142,14 +142,15 @@ __device__ __forceinline__ float weight(float m, float top) {  // of sums kept a
 // sum) of each part's heads and their values. Part 2 r is run r's of a head pass
 // that began before it, 2 r + 1 of one that goes on behind it. Stored and read at
 // agent scope, as the parts come from several XCDs.
+// (RUNS: most runs of the kernel.)
 constexpr size_t kCounterBytes = sizeof(int) * (kRuns + 64);
-template <int GQ, int DP>
+template <int GQ, int DP, int RUNS = kRuns>
 struct Parts {
   int *counters;  // [kRuns], then the fetched runs'
   float *ml, *o;
   __device__ explicit Parts(float *p)
       : counters(reinterpret_cast<int *>(p)), ml(p + kCounterBytes / sizeof(float)),
-        o(ml + static_cast<size_t>(kRuns) * 2 * GQ * 2) {}
+        o(ml + static_cast<size_t>(RUNS) * 2 * GQ * 2) {}
   __device__ float *ml_of(int part, int h) const { return ml + (static_cast<size_t>(part) * GQ + h) * 2; }
   __device__ float *o_of(int part, int h) const { return o + (static_cast<size_t>(part) * GQ + h) * DP; }
 };
@@ -160,8 +161,8 @@ __device__ __forceinline__ float2 load2(const float *p) {
   return make_float2(__uint_as_float(static_cast<unsigned>(x)), __uint_as_float(static_cast<unsigned>(x >> 32)));
 }
 
-inline size_t parts_bytes(int gq, int dims) {
-  return kCounterBytes + static_cast<size_t>(kRuns) * 2 * gq * (dims + 2) * sizeof(float);
+inline size_t parts_bytes(int gq, int dims, int runs = kRuns) {
+  return kCounterBytes + static_cast<size_t>(runs) * 2 * gq * (dims + 2) * sizeof(float);
 }
 
 // Where the waves of a workgroup meet: each wave's maxima, sums and weighted values.
@@ -196,9 +197,9 @@ __device__ __forceinline__ int next_run(const Plan &plan, const Parts<GQ, DP> &p
 // sum, value, the next dim's value), for every other dim, where that is all of it;
 // else the part goes to the workspace, and the workgroup that is counted last joins
 // the parts, in their order, and writes.
-template <int GQ, int DP, int WAVES, class Plan, class F>
-__device__ __forceinline__ void leave(Meet<GQ, DP, WAVES> &s, const Plan &plan, const Parts<GQ, DP> &parts, int run,
-                                      unsigned long long u, const Place &p, int last, int heads, int dim, F &&write) {
+template <int GQ, int DP, int WAVES, int RUNS, class Plan, class F>
+__device__ __forceinline__ void leave(Meet<GQ, DP, WAVES> &s, const Plan &plan, const Parts<GQ, DP, RUNS> &parts,
+                                      int run, unsigned long long u, const Place &p, int last, int heads, int dim, F &&write) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool whole = p.tile == 0 && last == p.tiles;

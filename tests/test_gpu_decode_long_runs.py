@@ -57,3 +57,21 @@ def test_with_shared_blocks(dev, heads, kv, dim, sizes, shared, own):
             assert (got[s] == 0).all()
     live = [s for s, n in enumerate(few) if n]
     assert (got[live] - out[live]).norm() <= 2 * NORMAL_REL * out[live].norm()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (12, 4, 64), (16, 1, 80), (16, 1, 256), (12, 3, 144)])
+def test_a_workspace_of_8_bits_is_as_large_as_it_is_said_to_be(dev, heads, kv, dim):
+    """Nothing behind its end is written where nearly every run leaves two parts, and it
+    has room for one run a workgroup, no more: 8 MB at most."""
+    n_kv = [1500 + 64 * (i % 7) for i in range(40)] if dim < 256 else [9000] * 4
+    g = torch.Generator(device=dev)
+    g.manual_seed(dim)
+    cache, tables = filled_cache(dev, g, n_kv, 64, kv, dim, torch.int8, seed=kv)
+    q = torch.randn(len(n_kv), heads, dim, generator=g, device=dev)
+    floats = ikv.load().ikv_attn_decode_batch_q8_workspace_bytes(heads, kv, dim) // 4
+    space = torch.zeros(floats + 4096, device=dev)
+    space[floats:] = -3.0
+    out = ikv.attn_decode_batch_q8(q, cache, dev32(tables, dev), dev32(n_kv, dev), workspace=space)
+    check_q8(out, q, [held(cache, tables, s, 64, c) for s, c in enumerate(n_kv)])
+    assert (space[floats:] == -3.0).all()
+    assert floats * 4 <= (8 << 20) + (1 << 18)
