@@ -35,9 +35,9 @@ struct Place {
   int seq, keys, tiles, item, tile;
 };
 
-// UNITS: of a run where there are more runs than workgroups (0: there never are); WHOLE: units of a
-// (sequence, head) that are not split anywhere; LEAST: of a run, where a (sequence,
-// head) has as many on average.
+// UNITS: of a run where there are more runs than workgroups (0: there never are);
+// WHOLE: units of a (sequence, head) that are not split anywhere; LEAST: of a run, where
+// a (sequence, head) has as many on average.
 template <class Args, int KT, int GROUPS, int UNITS, int WHOLE, int LEAST = 1>
 struct Plan {
   using Units = unsigned long long;
@@ -64,7 +64,8 @@ struct Plan {
       total = lane_value(upto, 63);
     }
     runs = GROUPS;
-    if constexpr (UNITS > 0) runs = static_cast<int>(min(max(total / UNITS, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
+    if constexpr (UNITS > 0)
+      runs = static_cast<int>(min(max(total / UNITS, static_cast<Units>(GROUPS)), static_cast<Units>(kRuns)));
     chunk = (total + runs - 1) / runs;
     if (chunk == 0) chunk = 1;
     if constexpr (LEAST > 1)
@@ -141,8 +142,7 @@ __device__ __forceinline__ float weight(float m, float top) {  // of sums kept a
 // and goes on behind it) and one of the runs that were fetched, then (maximum,
 // sum) of each part's heads and their values. Part 2 r is run r's of a head pass
 // that began before it, 2 r + 1 of one that goes on behind it. Stored and read at
-// agent scope, as the parts come from several XCDs.
-// (RUNS: most runs of the kernel.)
+// agent scope, as the parts come from several XCDs. RUNS: most runs of the kernel.
 constexpr size_t kCounterBytes = sizeof(int) * (kRuns + 64);
 template <int GQ, int DP, int RUNS = kRuns>
 struct Parts {
@@ -199,7 +199,8 @@ __device__ __forceinline__ int next_run(const Plan &plan, const Parts<GQ, DP> &p
 // the parts, in their order, and writes.
 template <int GQ, int DP, int WAVES, int RUNS, class Plan, class F>
 __device__ __forceinline__ void leave(Meet<GQ, DP, WAVES> &s, const Plan &plan, const Parts<GQ, DP, RUNS> &parts,
-                                      int run, unsigned long long u, const Place &p, int last, int heads, int dim, F &&write) {
+                                      int run, unsigned long long u, const Place &p, int last, int heads, int dim,
+                                      F &&write) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool whole = p.tile == 0 && last == p.tiles;
